@@ -11,6 +11,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <cmath>
 #include <exception>
 #include <thread>
 #include <vector>
@@ -1176,6 +1177,289 @@ int dw_hip_yolo_postprocess(dw_hip_backend* be, const dw_hip_buffer* raw, size_t
     for (int i = 0; i < len; ++i) memcpy(&o[i], entry(slot[(size_t)i]), sizeof(dw_detection));
   }
   if (over) dw::fail(DW_ERR_INVALID, "postprocess: more detections than cap in an image (see counts)");
+  API_END
+}
+
+// Layers in 4 bits: MXFP4 rows, products with MXFP4 weights, rotary positions
+// and attention over an MXFP4 cache.  What needs no device (sizes, types,
+// options) is checked before the handles.
+namespace {
+
+constexpr size_t kMostMx = (size_t)1 << 24;  // of each of a product's sizes, and of a cache's tokens and pages
+
+// A buffer of exactly `bytes` on the backend's device.
+void need_on(const Backend* b, const dw_hip_buffer* x, size_t bytes, const char* what) {
+  need(x, bytes, what);
+  if (x->be->device != b->device)
+    dw::fail(DW_ERR_INVALID, std::string(what) + ": on device " + std::to_string(x->be->device) + ", the backend is on " +
+                                 std::to_string(b->device));
+}
+
+size_t float_bytes(int dtype, const char* what) {
+  if (dtype != DW_DTYPE_F32 && dtype != DW_DTYPE_F16)
+    dw::fail(DW_ERR_UNSUPPORTED, std::string(what) + ": dtype must be f32 or f16");
+  return dw::dtype_size(dtype);
+}
+
+void check_mx_rows(size_t rows, size_t k, const char* what) {
+  if (!rows || !k) dw::fail(DW_ERR_INVALID, std::string(what) + ": zero size");
+  if (rows > INT32_MAX || k > INT32_MAX || rows * ((k + 31) / 32) > ((size_t)1 << 40))
+    dw::fail(DW_ERR_UNSUPPORTED, std::string(what) + ": size");
+}
+
+void check_act(int act, const char* what) {
+  if (act != DW_ACT_NONE && act != DW_ACT_RELU && act != DW_ACT_SILU)
+    dw::fail(DW_ERR_INVALID, std::string(what) + ": unknown activation");
+}
+
+// `heads` heads of `dim` elements from column `off` of rows of `stride`.
+void check_columns(size_t stride, size_t off, size_t heads, size_t dim, const char* what) {
+  if (stride > kMostMx || off > stride || heads * dim > stride - off)
+    dw::fail(DW_ERR_INVALID, std::string(what) + ": the heads do not fit the row");
+}
+
+// The sizes that append and attention share.
+void check_kv(size_t tokens, size_t batch, size_t kv_heads, size_t d, size_t page, size_t num_pages, size_t max_pages,
+              const char* what) {
+  const std::string w(what);
+  if (!tokens || !batch || !kv_heads || !num_pages || !max_pages) dw::fail(DW_ERR_INVALID, w + ": zero size");
+  if (d != 64 && d != 128 && d != 256) dw::fail(DW_ERR_UNSUPPORTED, w + ": head_dim must be 64, 128 or 256");
+  if (page < 16 || page > 65536 || (page & (page - 1)))
+    dw::fail(DW_ERR_UNSUPPORTED, w + ": page_size must be a power of two from 16 to 65536");
+  if (tokens >= kMostMx || batch > 65535 || kv_heads > 1024 || num_pages > INT32_MAX || max_pages > kMostMx ||
+      max_pages * page > INT32_MAX)
+    dw::fail(DW_ERR_UNSUPPORTED, w + ": size");
+}
+
+dw::KvArgs kv_args(const Backend* b, dw_hip_buffer* kc, dw_hip_buffer* ks, dw_hip_buffer* vc, dw_hip_buffer* vs,
+                   const dw_hip_buffer* table, const dw_hip_buffer* start, const dw_hip_buffer* len, size_t tokens,
+                   size_t batch, size_t kv_heads, size_t d, size_t page, size_t num_pages, size_t max_pages) {
+  const size_t rows = num_pages * kv_heads * page;
+  need_on(b, kc, rows * d / 2, "key cache");
+  need_on(b, ks, rows * d / 32, "key scales");
+  need_on(b, vc, rows * d / 2, "value cache");
+  need_on(b, vs, rows * d / 32, "value scales");
+  need_on(b, table, batch * max_pages * 4, "block table");
+  need_on(b, start, (batch + 1) * 4, "q_start");
+  need_on(b, len, batch * 4, "kv_len");
+  dw::KvArgs a{};
+  a.kc = (uint32_t*)kc->ptr;
+  a.ks = (uint8_t*)ks->ptr;
+  a.vc = (uint32_t*)vc->ptr;
+  a.vs = (uint8_t*)vs->ptr;
+  a.table = (const int32_t*)table->ptr;
+  a.start = (const int32_t*)start->ptr;
+  a.len = (const int32_t*)len->ptr;
+  a.tokens = (int)tokens;
+  a.batch = (int)batch;
+  a.kv_heads = (int)kv_heads;
+  a.d = (int)d;
+  a.page_shift = __builtin_ctzll(page);
+  a.num_pages = (int)num_pages;
+  a.max_pages = (int)max_pages;
+  return a;
+}
+
+}  // namespace
+
+int dw_hip_quantize_mxfp4(dw_hip_backend* be, int dtype, const dw_hip_buffer* x, dw_hip_buffer* q,
+                          dw_hip_buffer* scales, size_t rows, size_t k) {
+  API_BEGIN
+  const size_t es = float_bytes(dtype, "quantize_mxfp4");
+  check_mx_rows(rows, k, "quantize_mxfp4");
+  Backend* b = B(be);
+  std::lock_guard<std::mutex> lock(b->mu);
+  const size_t blocks = (k + 31) / 32;
+  need_on(b, x, rows * k * es, "quantize_mxfp4: input");
+  need_on(b, q, rows * blocks * 16, "quantize_mxfp4: packed rows");
+  need_on(b, scales, rows * blocks, "quantize_mxfp4: scales");
+  dw::launch_quantize_mxfp4(b->stream, dtype, x->ptr, q->ptr, scales->ptr, rows, k);
+  API_END
+}
+
+int dw_hip_dequantize_mxfp4(dw_hip_backend* be, int dtype, const dw_hip_buffer* q, const dw_hip_buffer* scales,
+                            dw_hip_buffer* y, size_t rows, size_t k) {
+  API_BEGIN
+  const size_t es = float_bytes(dtype, "dequantize_mxfp4");
+  check_mx_rows(rows, k, "dequantize_mxfp4");
+  Backend* b = B(be);
+  std::lock_guard<std::mutex> lock(b->mu);
+  const size_t blocks = (k + 31) / 32;
+  need_on(b, q, rows * blocks * 16, "dequantize_mxfp4: packed rows");
+  need_on(b, scales, rows * blocks, "dequantize_mxfp4: scales");
+  need_on(b, y, rows * k * es, "dequantize_mxfp4: output");
+  dw::launch_dequantize_mxfp4(b->stream, dtype, q->ptr, scales->ptr, y->ptr, rows, k);
+  API_END
+}
+
+int dw_hip_gemm_mxfp4(dw_hip_backend* be, int a_dtype, const dw_hip_buffer* a, const dw_hip_buffer* a_scales,
+                      const dw_hip_buffer* w, const dw_hip_buffer* w_scales, const dw_hip_buffer* bias, int c_dtype,
+                      dw_hip_buffer* c, size_t m, size_t n, size_t k, int act) {
+  API_BEGIN
+  if (a_dtype != DW_DTYPE_F16 && a_dtype != DW_DTYPE_MXFP4)
+    dw::fail(DW_ERR_UNSUPPORTED, "gemm_mxfp4: A must be f16 or MXFP4");
+  const size_t es = float_bytes(c_dtype, "gemm_mxfp4: C");
+  check_act(act, "gemm_mxfp4");
+  if (!m || !n || !k) dw::fail(DW_ERR_INVALID, "gemm_mxfp4: zero size");
+  if (m > kMostMx || n > kMostMx || k > kMostMx) dw::fail(DW_ERR_UNSUPPORTED, "gemm_mxfp4: a size above 2^24");
+  const bool mx = a_dtype == DW_DTYPE_MXFP4;
+  if (mx != (a_scales != nullptr)) dw::fail(DW_ERR_INVALID, "gemm_mxfp4: scales of A for MXFP4 rows, and only for them");
+  Backend* b = B(be);
+  std::lock_guard<std::mutex> lock(b->mu);
+  const size_t blocks = (k + 31) / 32;
+  need_on(b, a, mx ? m * blocks * 16 : m * k * 2, "gemm_mxfp4: A");
+  if (mx) need_on(b, a_scales, m * blocks, "gemm_mxfp4: scales of A");
+  need_on(b, w, n * blocks * 16, "gemm_mxfp4: W");
+  need_on(b, w_scales, n * blocks, "gemm_mxfp4: scales of W");
+  if (bias) need_on(b, bias, n * es, "gemm_mxfp4: bias");
+  need_on(b, c, m * n * es, "gemm_mxfp4: C");
+  if (c == a || c == a_scales || c == w || c == w_scales || c == bias)
+    dw::fail(DW_ERR_INVALID, "gemm_mxfp4: C is an operand");
+  dw::GemmMxArgs g{};
+  g.a = a->ptr;
+  g.as = mx ? (const uint8_t*)a_scales->ptr : nullptr;
+  g.w = (const uint8_t*)w->ptr;
+  g.ws = (const uint8_t*)w_scales->ptr;
+  g.bias = bias ? bias->ptr : nullptr;
+  g.c = c->ptr;
+  g.m = (int)m;
+  g.n = (int)n;
+  g.k = (int)k;
+  g.act = act;
+  g.c_half = c_dtype == DW_DTYPE_F16;
+  dw::launch_gemm_mx(b->stream, g);
+  API_END
+}
+
+int dw_hip_rope_axes(dw_hip_backend* be, int dtype, const dw_hip_buffer* x, size_t x_stride, size_t x_off,
+                     dw_hip_buffer* y, size_t y_stride, size_t y_off, const dw_hip_buffer* positions, size_t tokens,
+                     size_t heads, size_t head_dim, size_t rotary_dim, const size_t* sections, size_t axes, int order,
+                     int pairs, int freq, double base) {
+  API_BEGIN
+  const size_t es = float_bytes(dtype, "rope_axes");
+  if (!tokens || !heads || !head_dim || !rotary_dim || !axes || !sections) dw::fail(DW_ERR_INVALID, "rope_axes: zero size");
+  if (rotary_dim % 2 || rotary_dim > head_dim)
+    dw::fail(DW_ERR_INVALID, "rope_axes: rotary_dim must be even and at most head_dim");
+  if (rotary_dim > 256 || head_dim > 4096 || heads > 4096 || axes > 8 || tokens >= kMostMx)
+    dw::fail(DW_ERR_UNSUPPORTED, "rope_axes: size");
+  if ((order != 0 && order != 1) || (pairs != 0 && pairs != 1) || (freq != 0 && freq != 1))
+    dw::fail(DW_ERR_INVALID, "rope_axes: unknown option");
+  if (!(base > 0) || !std::isfinite(base)) dw::fail(DW_ERR_INVALID, "rope_axes: base must be positive");
+  const size_t half = rotary_dim / 2;
+  size_t sum = 0;
+  for (size_t i = 0; i < axes; ++i) {
+    if (sections[i] > half) dw::fail(DW_ERR_INVALID, "rope_axes: sections must add up to rotary_dim / 2");
+    sum += sections[i];
+  }
+  if (sum != half) dw::fail(DW_ERR_INVALID, "rope_axes: sections must add up to rotary_dim / 2");
+  check_columns(x_stride, x_off, heads, head_dim, "rope_axes: input");
+  check_columns(y_stride, y_off, heads, head_dim, "rope_axes: output");
+  if (x && x == y) {
+    const size_t w = heads * head_dim;
+    if (x_stride != y_stride || (x_off != y_off && x_off < y_off + w && y_off < x_off + w))
+      dw::fail(DW_ERR_INVALID, "rope_axes: input and output overlap");
+  }
+  Backend* b = B(be);
+  std::lock_guard<std::mutex> lock(b->mu);
+  need_on(b, x, tokens * x_stride * es, "rope_axes: input");
+  need_on(b, y, tokens * y_stride * es, "rope_axes: output");
+  need_on(b, positions, axes * tokens * 4, "rope_axes: positions");
+  if (positions == y) dw::fail(DW_ERR_INVALID, "rope_axes: the positions are the output");
+  dw::RopeArgs a{};
+  a.x = x->ptr;
+  a.y = y->ptr;
+  a.pos = (const int32_t*)positions->ptr;
+  a.x_stride = x_stride;
+  a.x_off = x_off;
+  a.y_stride = y_stride;
+  a.y_off = y_off;
+  a.tokens = tokens;
+  a.heads = (int)heads;
+  a.head_dim = (int)head_dim;
+  a.half = (int)half;
+  a.copy = !(x == y && x_off == y_off);
+  // the axis of each pair, and its frequency base^(-2 i / rotary_dim), i the
+  // pair's index in the head (freq 0) or base^(-j / n), j its index among the
+  // n pairs of its axis (freq 1): powers by repeated products in 80 bits
+  size_t used[8] = {};
+  long double power[9], step[9];
+  for (size_t i = 0; i <= axes; ++i) {
+    const size_t n = i < axes ? sections[i] : half;
+    step[i] = n ? expl(-logl((long double)base) / (long double)n) : 1.0L;
+    power[i] = 1.0L;
+  }
+  constexpr long double kTurn = 6.283185307179586476925286766559005768L;
+  for (size_t i = 0, next = 0; i < half; ++i) {
+    while (used[next] == sections[next]) next = (next + 1) % axes;  // some axis has pairs left
+    a.table.axis[i] = (uint8_t)next;
+    const size_t f = freq ? next : axes;
+    a.table.freq[i] = (double)(power[f] / kTurn);
+    power[f] *= step[f];
+    ++used[next];
+    if (order) next = (next + 1) % axes;
+  }
+  dw::launch_rope(b->stream, dtype, a, pairs);
+  API_END
+}
+
+int dw_hip_kv_append_mxfp4(dw_hip_backend* be, const dw_hip_buffer* k, size_t k_stride, size_t k_off,
+                           const dw_hip_buffer* v, size_t v_stride, size_t v_off, dw_hip_buffer* k_cache,
+                           dw_hip_buffer* k_scales, dw_hip_buffer* v_cache, dw_hip_buffer* v_scales,
+                           const dw_hip_buffer* block_table, const dw_hip_buffer* q_start, const dw_hip_buffer* kv_len,
+                           size_t tokens, size_t batch, size_t kv_heads, size_t head_dim, size_t page_size,
+                           size_t num_pages, size_t max_pages) {
+  API_BEGIN
+  check_kv(tokens, batch, kv_heads, head_dim, page_size, num_pages, max_pages, "kv_append_mxfp4");
+  check_columns(k_stride, k_off, kv_heads, head_dim, "kv_append_mxfp4: keys");
+  check_columns(v_stride, v_off, kv_heads, head_dim, "kv_append_mxfp4: values");
+  if (k_cache && (k_cache == v_cache || k_scales == v_scales))
+    dw::fail(DW_ERR_INVALID, "kv_append_mxfp4: keys and values share a cache");
+  Backend* b = B(be);
+  std::lock_guard<std::mutex> lock(b->mu);
+  need_on(b, k, tokens * k_stride * 2, "kv_append_mxfp4: keys");
+  need_on(b, v, tokens * v_stride * 2, "kv_append_mxfp4: values");
+  const dw::KvArgs a = kv_args(b, k_cache, k_scales, v_cache, v_scales, block_table, q_start, kv_len, tokens, batch,
+                               kv_heads, head_dim, page_size, num_pages, max_pages);
+  for (const dw_hip_buffer* w : {k_cache, k_scales, v_cache, v_scales})
+    if (w == k || w == v || w == block_table || w == q_start || w == kv_len)
+      dw::fail(DW_ERR_INVALID, "kv_append_mxfp4: the cache is an input");
+  dw::launch_kv_append(b->stream, a, k->ptr, k_stride, k_off, v->ptr, v_stride, v_off);
+  API_END
+}
+
+int dw_hip_attention_mxfp4(dw_hip_backend* be, const dw_hip_buffer* q, size_t q_stride, size_t q_off,
+                           const dw_hip_buffer* k_cache, const dw_hip_buffer* k_scales, const dw_hip_buffer* v_cache,
+                           const dw_hip_buffer* v_scales, const dw_hip_buffer* block_table,
+                           const dw_hip_buffer* q_start, const dw_hip_buffer* kv_len, dw_hip_buffer* y, size_t tokens,
+                           size_t batch, size_t heads, size_t kv_heads, size_t head_dim, size_t page_size,
+                           size_t num_pages, size_t max_pages, float scale, int causal, size_t window) {
+  API_BEGIN
+  check_kv(tokens, batch, kv_heads, head_dim, page_size, num_pages, max_pages, "attention_mxfp4");
+  if (!heads || heads % kv_heads) dw::fail(DW_ERR_INVALID, "attention_mxfp4: heads must be a multiple of kv_heads");
+  if (heads > 4096) dw::fail(DW_ERR_UNSUPPORTED, "attention_mxfp4: more than 4096 heads");
+  if (!std::isfinite(scale)) dw::fail(DW_ERR_INVALID, "attention_mxfp4: scale must be finite");
+  if (causal != 0 && causal != 1) dw::fail(DW_ERR_INVALID, "attention_mxfp4: causal must be 0 or 1");
+  if (window && !causal) dw::fail(DW_ERR_UNSUPPORTED, "attention_mxfp4: a window needs causal attention");
+  check_columns(q_stride, q_off, heads, head_dim, "attention_mxfp4: queries");
+  Backend* b = B(be);
+  std::lock_guard<std::mutex> lock(b->mu);
+  need_on(b, q, tokens * q_stride * 2, "attention_mxfp4: queries");
+  need_on(b, y, tokens * heads * head_dim * 2, "attention_mxfp4: output");
+  const dw::KvArgs a = kv_args(b, const_cast<dw_hip_buffer*>(k_cache), const_cast<dw_hip_buffer*>(k_scales),
+                               const_cast<dw_hip_buffer*>(v_cache), const_cast<dw_hip_buffer*>(v_scales), block_table,
+                               q_start, kv_len, tokens, batch, kv_heads, head_dim, page_size, num_pages, max_pages);
+  for (const dw_hip_buffer* r : {q, k_cache, k_scales, v_cache, v_scales, block_table, q_start, kv_len})
+    if (r == y) dw::fail(DW_ERR_INVALID, "attention_mxfp4: the output is an input");
+  dw::AttnArgs g{};
+  g.q = (const uint16_t*)q->ptr;
+  g.q_stride = q_stride;
+  g.q_off = q_off;
+  g.y = (uint16_t*)y->ptr;
+  g.heads = (int)heads;
+  g.causal = causal;
+  g.window = window > (size_t)INT32_MAX ? 0 : (long long)window;
+  g.scale = scale;
+  dw::launch_attention(b->stream, a, g);
   API_END
 }
 

@@ -440,4 +440,62 @@ void launch_copy_channels(hipStream_t st, View src, View dst, int pixels, int ch
 void launch_minmax_init(hipStream_t st, float* out);
 void launch_minmax(hipStream_t st, View x, int pixels, int channels, float* out);
 
+
+// MXFP4 rows (k_mxfp4.hip): dtype F32 or F16; q rows of ceil(k / 32) * 16
+// bytes, scales rows of ceil(k / 32).
+void launch_quantize_mxfp4(hipStream_t st, int dtype, const void* x, void* q, void* scales, size_t rows, size_t k);
+void launch_dequantize_mxfp4(hipStream_t st, int dtype, const void* q, const void* scales, void* y, size_t rows,
+                             size_t k);
+
+// C = act(A W^T + bias): W MXFP4 [n][k]; A f16 [m][k], or MXFP4 with its
+// scales in `as`; C and bias f16 (c_half) or f32.
+struct GemmMxArgs {
+  const void* a;
+  const uint8_t* as;
+  const uint8_t* w;
+  const uint8_t* ws;
+  const void* bias;
+  void* c;
+  int m, n, k, act, c_half;
+};
+void launch_gemm_mx(hipStream_t st, const GemmMxArgs& a);
+
+// Rotary positions: heads of x [tokens][x_stride] from column x_off, to y.
+struct RopeTable {
+  double freq[128];  // turns a position
+  uint8_t axis[128];
+};
+struct RopeArgs {
+  const void* x;
+  void* y;
+  const int32_t* pos;  // [axes][tokens]
+  size_t x_stride, x_off, y_stride, y_off, tokens;
+  int heads, head_dim, half, copy;  // copy: elements that do not turn, too
+  RopeTable table;
+};
+void launch_rope(hipStream_t st, int dtype, const RopeArgs& a, int adjacent);
+
+// A cache of keys and values in MXFP4 pages (k_kv_mxfp4.hip).
+struct KvArgs {
+  uint32_t* kc;  // [num_pages][kv_heads][page][d / 8] words
+  uint8_t* ks;   // [num_pages][kv_heads][page][d / 32]
+  uint32_t* vc;
+  uint8_t* vs;
+  const int32_t* table;  // [batch][max_pages]
+  const int32_t* start;  // [batch + 1]
+  const int32_t* len;    // [batch]
+  int tokens, batch, kv_heads, d, page_shift, num_pages, max_pages;
+};
+struct AttnArgs {
+  const uint16_t* q;
+  size_t q_stride, q_off;
+  uint16_t* y;  // [tokens][heads][d]
+  int heads, causal;
+  long long window;
+  float scale;
+};
+void launch_kv_append(hipStream_t st, const KvArgs& a, const void* k, size_t k_stride, size_t k_off, const void* v,
+                      size_t v_stride, size_t v_off);
+void launch_attention(hipStream_t st, const KvArgs& a, const AttnArgs& g);
+
 }  // namespace dw

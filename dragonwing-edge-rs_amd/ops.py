@@ -14,6 +14,7 @@ from ._lib import check, load
 
 ACT_NONE, ACT_RELU, ACT_SILU = 0, 1, 2
 DTYPE_F32, DTYPE_F16, DTYPE_I8, DTYPE_U8, DTYPE_I32 = 0, 1, 2, 3, 4
+DTYPE_MXFP4 = 5  # an operand of gemm_mxfp4
 
 
 def _h(b):
@@ -245,6 +246,53 @@ def qgemm_u8s8(be, a, b, bias, y, m, n, k, a_scale, a_zp, b_scales, y_scale, y_z
 def qlinear_global_avg_pool_u8(be, x, y, n, h, w, c, x_scale, x_zp, y_scale, y_zp):
     check(load().dw_hip_qlinear_global_avg_pool_u8(be.handle, x.handle, y.handle, n, h, w, c, float(x_scale),
                                                    int(x_zp), float(y_scale), int(y_zp)))
+
+
+# --- layers in 4 bits: MXFP4 products, rotary positions, attention -------------
+
+def quantize_mxfp4(be, dtype, x, q, scales, rows, k):
+    """Rows of x (dtype F32 or F16) as MXFP4: q [rows, ceil(k/32) * 16] bytes, scales [rows, ceil(k/32)]."""
+    check(load().dw_hip_quantize_mxfp4(be.handle, dtype, _h(x), _h(q), _h(scales), rows, k))
+
+
+def dequantize_mxfp4(be, dtype, q, scales, y, rows, k):
+    """The values of MXFP4 rows in y (dtype F32 or F16)."""
+    check(load().dw_hip_dequantize_mxfp4(be.handle, dtype, _h(q), _h(scales), _h(y), rows, k))
+
+
+def gemm_mxfp4(be, a_dtype, a, a_scales, w, w_scales, bias, c_dtype, c, m, n, k, act=ACT_NONE):
+    """c [m, n] = act(a [m, k] w [n, k]^T + bias): w in MXFP4 rows, a f16 (a_scales None) or MXFP4 rows
+    (DTYPE_MXFP4); bias (or None) has c's type."""
+    check(load().dw_hip_gemm_mxfp4(be.handle, a_dtype, _h(a), _h(a_scales), _h(w), _h(w_scales), _h(bias), c_dtype,
+                                   _h(c), m, n, k, act))
+
+
+def rope_axes(be, dtype, x, x_stride, x_off, y, y_stride, y_off, positions, tokens, heads, head_dim, rotary_dim,
+              sections, order=0, pairs=0, freq=0, base=10000.0):
+    """Rotary positions over len(sections) axes; positions [axes, tokens] int32 (see dw_hip.h for the options)."""
+    n = (C.c_size_t * len(sections))(*sections)
+    check(load().dw_hip_rope_axes(be.handle, dtype, _h(x), x_stride, x_off, _h(y), y_stride, y_off, _h(positions),
+                                  tokens, heads, head_dim, rotary_dim, n, len(sections), order, pairs, freq,
+                                  float(base)))
+
+
+def kv_append_mxfp4(be, k, k_stride, k_off, v, v_stride, v_off, k_cache, k_scales, v_cache, v_scales, block_table,
+                    q_start, kv_len, tokens, batch, kv_heads, head_dim, page_size, num_pages, max_pages):
+    """New tokens' keys and values (f16) into the pages of an MXFP4 cache."""
+    check(load().dw_hip_kv_append_mxfp4(be.handle, _h(k), k_stride, k_off, _h(v), v_stride, v_off, _h(k_cache),
+                                        _h(k_scales), _h(v_cache), _h(v_scales), _h(block_table), _h(q_start),
+                                        _h(kv_len), tokens, batch, kv_heads, head_dim, page_size, num_pages,
+                                        max_pages))
+
+
+def attention_mxfp4(be, q, q_stride, q_off, k_cache, k_scales, v_cache, v_scales, block_table, q_start, kv_len, y,
+                    tokens, batch, heads, kv_heads, head_dim, page_size, num_pages, max_pages, scale, causal=True,
+                    window=0):
+    """Attention of new tokens (q f16) over an MXFP4 cache, y f16 [tokens, heads, head_dim]."""
+    check(load().dw_hip_attention_mxfp4(be.handle, _h(q), q_stride, q_off, _h(k_cache), _h(k_scales), _h(v_cache),
+                                        _h(v_scales), _h(block_table), _h(q_start), _h(kv_len), _h(y), tokens, batch,
+                                        heads, kv_heads, head_dim, page_size, num_pages, max_pages, float(scale),
+                                        int(causal), window))
 
 
 # --- layout and BN fold on the device -----------------------------------------

@@ -250,6 +250,7 @@ int dw_hip_lut_u8(dw_hip_backend* be, const dw_hip_buffer* x, dw_hip_buffer* y, 
 #define DW_DTYPE_I8 2
 #define DW_DTYPE_U8 3
 #define DW_DTYPE_I32 4
+#define DW_DTYPE_MXFP4 5 /* an operand of dw_hip_gemm_mxfp4 only */
 
 /* maxpool2d_f32_nhwc (ops.rs:1513-1552), extended with padding: padded
  * positions never win (ONNX MaxPool; the reference ignores pads,
@@ -331,6 +332,96 @@ int dw_hip_qgemm_u8s8(dw_hip_backend* be, const dw_hip_buffer* a, const dw_hip_b
 int dw_hip_qlinear_global_avg_pool_u8(dw_hip_backend* be, const dw_hip_buffer* x, dw_hip_buffer* y, size_t n,
                                       size_t h, size_t w, size_t c, float x_scale, int x_zp, float y_scale,
                                       int y_zp);
+
+/* ------------------------------------------------------------------------ */
+/* Layers in 4 bits (no counterpart in the reference)                        */
+/* ------------------------------------------------------------------------ */
+
+/* MXFP4 rows: the microscaled 4-bit floating-point format (OCP Microscaling
+ * Formats v1.0).  A row of k elements is ceil(k / 32) blocks; a block is 16
+ * bytes, two elements a byte, the first in the low half, and has a scale byte
+ * s that stands for 2^(s - 127), 255 for NaN.  An element is a sign, two
+ * exponent bits and a mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4 or 6.  q is
+ * [rows][ceil(k/32) * 16] bytes, scales [rows][ceil(k/32)].
+ *
+ * Quantize: s = max(floor(log2 max|x|) - 2 + 127, 0) and each element
+ * x / 2^(s - 127) to the nearest, ties to even, 6 at most; 255 for a block
+ * that holds an infinity or a NaN; elements behind a row's end are 0.
+ * dtype: of x or y, F32 or F16 (f16 subnormals at their IEEE value).
+ * Dequantize to F16 rounds to nearest even, and to F32 is exact. */
+int dw_hip_quantize_mxfp4(dw_hip_backend* be, int dtype, const dw_hip_buffer* x, dw_hip_buffer* q,
+                          dw_hip_buffer* scales, size_t rows, size_t k);
+int dw_hip_dequantize_mxfp4(dw_hip_backend* be, int dtype, const dw_hip_buffer* q, const dw_hip_buffer* scales,
+                            dw_hip_buffer* y, size_t rows, size_t k);
+
+/* C [m][n] = act(A [m][k] W [n][k]^T + bias [n]), W in MXFP4 rows.  A is f16
+ * (a_dtype F16, a_scales NULL) or MXFP4 rows with their scales (MXFP4).
+ * c_dtype: of C and of the bias (may be NULL), F32 or F16.  Products are
+ * exact and summed in f32 in an order of the library's own; bias and
+ * activation (DW_ACT_*) are f32, and C is rounded once.  Elements of W and A
+ * behind a row's k must be 0, as quantize writes them.  Each size at most 2^24. */
+int dw_hip_gemm_mxfp4(dw_hip_backend* be, int a_dtype, const dw_hip_buffer* a, const dw_hip_buffer* a_scales,
+                      const dw_hip_buffer* w, const dw_hip_buffer* w_scales, const dw_hip_buffer* bias, int c_dtype,
+                      dw_hip_buffer* c, size_t m, size_t n, size_t k, int act);
+
+/* Rotary positions over several axes (time, height, width): heads of
+ * head_dim elements from column x_off of rows of x_stride elements, to those
+ * of y; dtype F32 or F16.  x and y may be one buffer (in place with equal
+ * columns, or disjoint ones).  Of each head the first rotary_dim elements
+ * turn and the others are copied: pair i < r = rotary_dim / 2 is elements
+ * (i, i + r) (pairs 0) or (2i, 2i + 1) (pairs 1), and
+ *   (a, b) -> (a cos t - b sin t, b cos t + a sin t),
+ *   t = positions[axis(i)][token] * base^-e(i).
+ * sections [axes]: how many pairs each axis has, r in all.  order 0: the
+ * axes' pairs one axis after the other; 1: in turn among the axes that have
+ * pairs left.  freq 0: e(i) = i / r; 1: e(i) = j / sections[axis(i)] with j
+ * the pair's place among those of its axis.  positions [axes][tokens] int32,
+ * any value; angles are formed in 64 bits.  rotary_dim <= 256, axes <= 8. */
+int dw_hip_rope_axes(dw_hip_backend* be, int dtype, const dw_hip_buffer* x, size_t x_stride, size_t x_off,
+                     dw_hip_buffer* y, size_t y_stride, size_t y_off, const dw_hip_buffer* positions, size_t tokens,
+                     size_t heads, size_t head_dim, size_t rotary_dim, const size_t* sections, size_t axes, int order,
+                     int pairs, int freq, double base);
+
+/* A cache of keys and values in MXFP4 pages.  k_cache and v_cache are
+ * [num_pages][kv_heads][page_size] MXFP4 rows of head_dim elements, k_scales
+ * and v_scales their scales (so dw_hip_dequantize_mxfp4 reads them as
+ * num_pages * kv_heads * page_size rows).  page_size is a power of two, 16 to
+ * 65536; head_dim 64, 128 or 256.  On the device, int32:
+ *   block_table [batch][max_pages]  page of each page_size tokens of a sequence
+ *   q_start [batch + 1]   first new token (row of q, k, v) of each sequence,
+ *                         ascending; rows from q_start[batch] on belong to none
+ *   kv_len [batch]        tokens of each sequence, the new ones included
+ * New token i of n of a sequence has position kv_len - n + i.
+ *
+ * Append writes the new tokens' keys and values (f16, kv_heads heads from
+ * column k_off / v_off of rows of k_stride / v_stride elements), quantized
+ * as dw_hip_quantize_mxfp4 does, but with scales of at least 2^-23: every
+ * value of the cache is then an f16 value.  A token whose position or page
+ * is outside the table or the cache is not written.  Two tokens on one
+ * place: either is written. */
+int dw_hip_kv_append_mxfp4(dw_hip_backend* be, const dw_hip_buffer* k, size_t k_stride, size_t k_off,
+                           const dw_hip_buffer* v, size_t v_stride, size_t v_off, dw_hip_buffer* k_cache,
+                           dw_hip_buffer* k_scales, dw_hip_buffer* v_cache, dw_hip_buffer* v_scales,
+                           const dw_hip_buffer* block_table, const dw_hip_buffer* q_start, const dw_hip_buffer* kv_len,
+                           size_t tokens, size_t batch, size_t kv_heads, size_t head_dim, size_t page_size,
+                           size_t num_pages, size_t max_pages);
+
+/* Attention of new tokens over the cache: q f16, heads heads of head_dim from
+ * column q_off of rows of q_stride; y f16 [tokens][heads][head_dim].  Head h
+ * reads kv head h / (heads / kv_heads).
+ *   y = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q.k_j - max)
+ * over the keys j < kv_len; with causal, those up to the token's position,
+ * and with a window > 0 the last `window` of them.  A row that sees no key,
+ * or only scores of -inf, is 0.  Keys that a row does not see do not reach
+ * it, whatever they hold; keys on pages outside the cache are seen by none.
+ * Scores and sums are f32; p is rounded to f16 before it meets the values.
+ * Rows of y that belong to no sequence are left as they were. */
+int dw_hip_attention_mxfp4(dw_hip_backend* be, const dw_hip_buffer* q, size_t q_stride, size_t q_off,
+                           const dw_hip_buffer* k_cache, const dw_hip_buffer* k_scales, const dw_hip_buffer* v_cache,
+                           const dw_hip_buffer* v_scales, const dw_hip_buffer* block_table,
+                           const dw_hip_buffer* q_start, const dw_hip_buffer* kv_len, dw_hip_buffer* y, size_t tokens,
+                           size_t batch, size_t heads, size_t kv_heads, size_t head_dim, size_t page_size,
+                           size_t num_pages, size_t max_pages, float scale, int causal, size_t window);
 
 /* YOLOv8 detect tail: the exported graph's ops after the head convs
  * (ultralytics Detect: DFL softmax over each side's reg_max bins and the 1x1
