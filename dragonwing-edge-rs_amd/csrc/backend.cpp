@@ -1227,7 +1227,7 @@ void check_kv(size_t tokens, size_t batch, size_t kv_heads, size_t d, size_t pag
   if (page < 16 || page > 65536 || (page & (page - 1)))
     dw::fail(DW_ERR_UNSUPPORTED, w + ": page_size must be a power of two from 16 to 65536");
   if (tokens >= kMostMx || batch > 65535 || kv_heads > 1024 || num_pages > INT32_MAX || max_pages > kMostMx ||
-      max_pages * page > INT32_MAX)
+      max_pages * page > (size_t)1 << 30)
     dw::fail(DW_ERR_UNSUPPORTED, w + ": size");
 }
 
@@ -1458,8 +1458,11 @@ int dw_hip_attention_mxfp4(dw_hip_backend* be, const dw_hip_buffer* q, size_t q_
   g.heads = (int)heads;
   g.causal = causal;
   g.window = window > (size_t)INT32_MAX ? 0 : (long long)window;
-  g.scale = scale;
-  dw::launch_attention(b->stream, a, g);
+  g.scale = fabsf(scale) * 1.44269504f;
+  g.negate = scale < 0;
+  dw::SplitArgs p{};
+  void* space = b->workspace(Backend::WS_ATTN, dw::attention_space(a, g, &p));
+  dw::launch_attention(b->stream, a, g, p, space);
   API_END
 }
 

@@ -490,12 +490,25 @@ struct AttnArgs {
   const uint16_t* q;
   size_t q_stride, q_off;
   uint16_t* y;  // [tokens][heads][d]
-  int heads, causal;
+  int heads, causal, negate;  // negate: the scale is below zero
   long long window;
-  float scale;
+  float scale;  // |scale| log2(e): p = 2^(scale (s - max))
 };
+// How single tokens' attention is split over keys, and what the splits leave:
+// set by attention_space, which gives the bytes of workspace.
+struct SplitArgs {
+  int group, head_tiles;   // heads of a kv head, tiles of 16 of them
+  int tile_tokens;         // new tokens of a tile of 16 rows
+  int waves, least;        // splits wanted, a split's fewest steps of 64 keys
+  int splits;              // of the grid
+  float* sums;             // [splits][d / 16][64][4]
+  float2* stats;           // [splits][16]: reference, sum
+  int2* items;             // [tokens][kv heads x head tiles]: first split, splits
+  size_t stats_at, items_at;  // bytes into the workspace
+};
+size_t attention_space(const KvArgs& a, const AttnArgs& g, SplitArgs* p);
 void launch_kv_append(hipStream_t st, const KvArgs& a, const void* k, size_t k_stride, size_t k_off, const void* v,
                       size_t v_stride, size_t v_off);
-void launch_attention(hipStream_t st, const KvArgs& a, const AttnArgs& g);
+void launch_attention(hipStream_t st, const KvArgs& a, const AttnArgs& g, SplitArgs p, void* space);
 
 }  // namespace dw

@@ -4,6 +4,8 @@
 // A page holds page_size rows of each kv head, [page][head][slot][d / 2]
 // bytes and [page][head][slot][d / 32] scales: the rows are MXFP4 rows of d
 // elements (mxfp4.h), so the cache's values can be read back as such rows.
+#include <algorithm>
+
 #include "dw_common.h"
 #include "mxfp4.h"
 
@@ -66,68 +68,395 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a, const uint16_t
   }
 }
 
-// The plain kernel: a wave for each new token and head, 64 keys a step.
-__global__ __launch_bounds__(64) void attention_plain_kernel(KvArgs a, AttnArgs g) {
+// A wave's share of the work: keys [begin, end) of a tile of up to 16 rows
+// (new tokens of one sequence x heads of one kv head).
+constexpr int kChunk = 64;  // keys a step
+
+struct Split {
+  int seq, token, count;  // the tile's first token and how many it has
+  int kv_head, head;      // head: the tile's first
+  int index, of;          // this split of the item's
+  int first, chunks;      // steps before this split, and its own
+  long long pos, len;     // position of the tile's first token, keys of the sequence
+};
+
+__device__ __forceinline__ unsigned long long sum_of_wave(unsigned long long v) {
+  for (int i = 1; i < 64; i *= 2) v += __shfl_xor(v, i);
+  return v;
+}
+
+// Which split this wave has.  Every item (tile, kv head) of a sequence has
+// the same number of steps; all steps over the waves wanted is a split's
+// length, so that long and short sequences share the waves evenly whatever
+// their lengths, which only the device knows.  One load a 64 sequences.
+__device__ __forceinline__ bool plan(const KvArgs& a, const AttnArgs& g, const SplitArgs& p, long long mine, Split* s) {
+  const int lane = threadIdx.x & 63;
+  const long long most = (long long)a.max_pages << a.page_shift;
+  auto of = [&](int b, int* first, int* tiles, int* steps, long long* len, long long* raw, int* count) {
+    *tiles = 0;
+    *steps = 1;
+    *len = *raw = 0;
+    *first = *count = 0;
+    if (b >= a.batch) return;
+    const int t0 = max(a.start[b], 0), t1 = min(a.start[b + 1], a.tokens);
+    *raw = a.len[b];
+    *len = min(max(*raw, 0ll), most);
+    *first = t0;
+    *count = max(t1 - t0, 0);
+    *tiles = (*count + p.tile_tokens - 1) / p.tile_tokens;
+    long long span = *len;
+    if (g.window > 0) span = min(span, g.window + p.tile_tokens + 14);
+    *steps = (int)max(1ll, (span + kChunk - 1) / kChunk);
+  };
+  int first, tiles, steps, count;
+  long long len, raw;
+  unsigned long long all = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    of(b0 + lane, &first, &tiles, &steps, &len, &raw, &count);
+    all += sum_of_wave((unsigned long long)tiles * p.head_tiles * a.kv_heads * steps);
+  }
+  const long long length = max((long long)p.least, (long long)((all + p.waves - 1) / p.waves));
+  long long before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    if (a.batch > 64) of(b0 + lane, &first, &tiles, &steps, &len, &raw, &count);
+    const int n = (int)((steps + length - 1) / length);
+    const long long here = (long long)tiles * p.head_tiles * a.kv_heads * n;
+    long long upto = here;
+    for (int i = 1; i < 64; i *= 2) {
+      const long long v = __shfl_up(upto, i);
+      if (lane >= i) upto += v;
+    }
+    const unsigned long long hit = __ballot(mine >= before + upto - here && mine < before + upto);
+    if (hit) {
+      const int src = __ffsll(hit) - 1;
+      const int at = (int)(mine - before - __shfl(upto - here, src));
+      s->of = __builtin_amdgcn_readfirstlane(__shfl(n, src));
+      const int item = __builtin_amdgcn_readfirstlane(at / s->of), heads = p.head_tiles * a.kv_heads;
+      s->index = __builtin_amdgcn_readfirstlane(at - item * s->of);
+      const int tile = item / heads, hh = item - tile * heads;
+      s->seq = b0 + src;
+      s->kv_head = hh / p.head_tiles;
+      s->head = s->kv_head * p.group + (hh - s->kv_head * p.head_tiles) * 16;
+      const int skip = tile * p.tile_tokens;
+      s->token = __builtin_amdgcn_readfirstlane(__shfl(first, src)) + skip;
+      const int whole = __builtin_amdgcn_readfirstlane(__shfl(count, src));
+      s->count = min(whole - skip, p.tile_tokens);
+      s->len = __shfl(len, src);
+      // the raw length places the tokens, whatever the table holds
+      s->pos = __shfl(raw, src) - whole + skip;
+      s->first = (int)(s->index * length);
+      s->chunks = (int)min(length, (long long)__builtin_amdgcn_readfirstlane(__shfl(steps, src)) - s->first);
+      return true;
+    }
+    before += __shfl(upto, 63);
+  }
+  return false;
+}
+
+__device__ __forceinline__ float max_of_rows(float v) {  // over the four lanes of a column
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float sum_of_rows(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <int J>
+__device__ __forceinline__ h16x2 mx_pair(uint32_t w, float scale) {
+  return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, J);
+}
+__device__ __forceinline__ f16x8 mx_eight(uint32_t w, float scale) {
+  const h16x2 a = mx_pair<0>(w, scale), b = mx_pair<1>(w, scale), c = mx_pair<2>(w, scale), d = mx_pair<3>(w, scale);
+  return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// A lane's quarter of a row: D / 4 elements, their words and scale bytes.
+template <int D>
+struct Piece {
+  uint32_t w[D / 32];
+  uint32_t s;  // D / 128 bytes, or the one the piece is half of
+  __device__ __forceinline__ void load(const uint32_t* words, const uint8_t* scales, size_t row, int quarter) {
+    const uint32_t* p = words + row * (D / 8) + quarter * (D / 32);
+    if constexpr (D == 64) {
+      const uint2 v = *(const uint2*)p;
+      w[0] = v.x, w[1] = v.y;
+      s = scales[row * 2 + (quarter >> 1)];
+    } else if constexpr (D == 128) {
+      const uint4 v = *(const uint4*)p;
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+      s = scales[row * 4 + quarter];
+    } else {
+      const uint4 v = *(const uint4*)p, u = *(const uint4*)(p + 4);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+      w[4] = u.x, w[5] = u.y, w[6] = u.z, w[7] = u.w;
+      s = *(const uint16_t*)(scales + row * 8 + quarter * 2);
+    }
+  }
+  __device__ __forceinline__ float scale(int word) const { return mx_scale(D == 256 && word >= 4 ? s >> 8 : D == 256 ? s & 255u : s); }
+  __device__ __forceinline__ f16x8 eight(int word) const { return mx_eight(w[word], scale(word)); }
+  // The four pieces' blocks that are NaN, as bits of the row's blocks.
+  __device__ __forceinline__ uint32_t nan_bits(int quarter) const {
+    if constexpr (D == 64) return s == 255u ? 1u << (quarter >> 1) : 0u;
+    if constexpr (D == 128) return s == 255u ? 1u << quarter : 0u;
+    return ((s & 255u) == 255u ? 1u << (2 * quarter) : 0u) | ((s >> 8) == 255u ? 2u << (2 * quarter) : 0u);
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) w[i] = 0;
+    s = D == 256 ? 0x7F7Fu : 127u;
+  }
+  __device__ __forceinline__ void clear_nan() {
+    if constexpr (D == 256) {
+      if ((s & 255u) == 255u) w[0] = w[1] = w[2] = w[3] = 0, s = (s & 0xFF00u) | 127u;
+      if ((s >> 8) == 255u) w[4] = w[5] = w[6] = w[7] = 0, s = (s & 255u) | 0x7F00u;
+    } else if (s == 255u) {
+      clear();
+    }
+  }
+};
+
+// Attention of one tile over one split of its keys, by one wave.
+//
+// S^T = K Q^T on 16 x 16 x 32 matrix instructions: a lane's A operand is a
+// quarter of one key's row (a whole MXFP4 block at d = 128, one scale), its B
+// operand the same quarter of a query's; the order in which the products
+// take the row's elements is the lanes', the same on both sides.  The
+// result leaves a lane four keys of one query, and two such tiles are the B
+// operand of O^T += V^T P^T as they stand, if the A operand takes the keys
+// in that order: values go through LDS as f16 rows and come back transposed,
+// four keys a read.  The running maximum moves only when a score passes it by
+// 2^8, so that most steps leave the sums as they are.
+template <int D>
+__global__ __launch_bounds__(64) void attention_split_kernel(KvArgs a, AttnArgs g, SplitArgs p) {
+  constexpr int kRow = D * 2 + 32;  // bytes of a row in LDS: four rows side by side meet no bank twice
+  __shared__ __align__(16) uint8_t vt[32 * kRow];
+  const int lane = threadIdx.x, col = lane & 15, quad = lane >> 4;
+  Split s;
+  if (!plan(a, g, p, blockIdx.x, &s)) return;
+  // this lane's query
+  const int within = p.tile_tokens > 1 ? col / p.group : 0;
+  const int head = s.head + (p.tile_tokens > 1 ? col - within * p.group : col);
+  const bool real = within < s.count && (p.tile_tokens > 1 ? col < p.tile_tokens * p.group
+                                                           : head < (s.kv_head + 1) * p.group);
+  const long long pos = s.pos + within;
+  const int hi = !real ? 0 : (int)(g.causal ? max(0ll, min(s.len, pos + 1)) : s.len);
+  const int lo = !real || g.window <= 0 ? 0 : (int)max(0ll, pos - g.window + 1);
+  const long long last = s.pos + s.count - 1;
+  const int most = (int)(g.causal ? max(0ll, min(s.len, last + 1)) : s.len);  // keys that some row sees: [from, most)
+  const int from = g.window > 0 ? (int)min((long long)most, max(0ll, s.pos - g.window + 1)) : 0;
+  const int every = (int)(g.causal ? max(0ll, min(s.len, s.pos + 1)) : s.len);  // that all rows see, up to here
+  const int all_from = g.window > 0 ? (int)max(0ll, last - g.window + 1) : 0;
+  f16x8 q[D / 32];
+  {
+    const uint16_t* src = g.q + (size_t)(s.token + within) * g.q_stride + g.q_off + (size_t)head * D + quad * (D / 4);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      if (real) {
+        const Loose<uint16_t, 8> v = load_loose<uint16_t, 8>(src + i * 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          q[i][e] = __builtin_bit_cast(_Float16, (uint16_t)(g.negate ? v.v[e] ^ 0x8000u : v.v[e]));
+      } else {
+        q[i] = f16x8{};
+      }
+    }
+  }
+  f32x4 o[D / 16] = {};
+  float m = -INFINITY, l = 0.0f;  // the scores' reference (unscaled), the sum over this lane's keys
+  uint32_t nan_blocks = 0;
+  const int j0 = (from & ~15) + s.first * kChunk;
+  const int steps = min(s.chunks, (most - j0 + kChunk - 1) / kChunk);
+  const int32_t* table = a.table + (size_t)s.seq * a.max_pages;
+  const int mask = (1 << a.page_shift) - 1;
+  int pages = -1;
+  Piece<D> k[4], v[4];
+  uint32_t have = 0;  // tiles of 16 keys that lie on a page of the cache
+  auto load = [&](int step, Piece<D>* kk, Piece<D>* vv) {
+    uint32_t ok = 0;
+    if ((step & 15) == 0) {  // the pages of 64 tiles, one a lane
+      const long long j = (long long)j0 + (step * 4 + lane) * 16;
+      pages = j < most ? table[j >> a.page_shift] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = j0 + step * kChunk + u * 16;
+      int page = __builtin_amdgcn_readlane(pages, (step * 4 + u) & 63);
+      if (page >= 0 && page < a.num_pages)
+        ok |= 1u << u;
+      else
+        page = 0;
+      const size_t row = (((size_t)page * a.kv_heads + s.kv_head) << a.page_shift) + (j & mask);
+      kk[u].load(a.kc, a.ks, row + col, quad);
+      vv[u].load(a.vc, a.vs, row + (lane >> 2), lane & 3);
+    }
+    return ok;
+  };
+  if (steps > 0) have = load(0, k, v);
+  for (int step = 0; step < steps; ++step) {
+    Piece<D> kn[4], vn[4];
+    uint32_t next = 0;
+    if (step + 1 < steps) next = load(step + 1, kn, vn);
+    const int j = j0 + step * kChunk;
+    f32x4 t[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      t[u] = f32x4{};
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) t[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[u].eight(i), q[i], t[u], 0, 0, 0);
+    }
+    uint32_t see = 0xFFFFu;
+    if (have != 15u || j + kChunk > every || j < all_from) {  // the same for the whole wave
+      see = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const bool there = have >> u & 1;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = j + u * 16 + quad * 4 + r;
+          const bool yes = there && key < hi && key >= lo;
+          see |= (uint32_t)yes << (u * 4 + r);
+          t[u][r] = yes ? t[u][r] : -INFINITY;
+        }
+        // values that no row sees must not reach the sums, whatever they hold
+        const int key = j + u * 16 + (lane >> 2);
+        if (!there || key >= most || key < from) v[u].clear();
+        // nor those that only some see, if they are NaN
+        if (s.count > 1) {
+          const uint32_t own = v[u].nan_bits(lane & 3);
+          if (__ballot(own != 0)) {
+            uint32_t row = own | __shfl_xor(own, 1);
+            row |= __shfl_xor(row, 2);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const uint32_t of = __shfl(row, (quad * 4 + r) * 4);
+              if (see >> (u * 4 + r) & 1) nan_blocks |= of;
+            }
+            if (own) v[u].clear_nan();
+          }
+        }
+      }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) top = fmaxf(top, fmaxf(fmaxf(t[u][0], t[u][1]), fmaxf(t[u][2], t[u][3])));
+    if (__ballot(m == -INFINITY ? top > m : (top - m) * g.scale > 8.0f)) {
+      const float now = fmaxf(m, max_of_rows(top));
+      const float f = now == m ? 1.0f : m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - now) * g.scale);
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) o[i] *= f;
+      m = now;
+    }
+    const float ref = m == -INFINITY ? 0.0f : m * g.scale;
+    f16x8 pr[2];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float e = __builtin_amdgcn_exp2f(fmaf(t[u][r], g.scale, -ref));
+        e = see >> (u * 4 + r) & 1 ? e : 0.0f;
+        l += e;
+        pr[u >> 1][(u & 1) * 4 + r] = (_Float16)e;
+      }
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        f16x8* dst = (f16x8*)(vt + (u * 16 + (lane >> 2)) * kRow + (lane & 3) * (D / 2));
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) dst[i] = v[half * 2 + u].eight(i);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        // a group of 16 lanes reads 4 keys x 16 elements; lane e of it gets element e of the four
+        typedef __attribute__((address_space(3))) s16x4* Lds;
+        const uint8_t* src = vt + (quad * 4 + (col >> 2)) * kRow + i * 32 + (col & 3) * 8;
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)src);
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(src + 16 * kRow));
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        const s16x8 xy = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, xy), pr[half], o[i], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) k[u] = kn[u], v[u] = vn[u];
+    have = next;
+  }
+  l = sum_of_rows(l);
+  nan_blocks |= __shfl_xor(nan_blocks, 16);
+  nan_blocks |= __shfl_xor(nan_blocks, 32);
+  if (__ballot(nan_blocks != 0)) {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+      if (nan_blocks >> (i / 2) & 1) o[i] = f32x4{NAN, NAN, NAN, NAN};
+  }
+  if (s.index == 0 && lane == 0)
+    p.items[(size_t)s.token * a.kv_heads * p.head_tiles + s.kv_head * p.head_tiles +
+            (s.head - s.kv_head * p.group) / 16] = make_int2((int)blockIdx.x, s.of);
+  if (s.of == 1) {
+    if (!real) return;
+    uint16_t* y = g.y + ((size_t)(s.token + within) * g.heads + head) * D + quad * 4;
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      ushort4 h;
+      h.x = narrow<uint16_t>(o[i][0] * f), h.y = narrow<uint16_t>(o[i][1] * f);
+      h.z = narrow<uint16_t>(o[i][2] * f), h.w = narrow<uint16_t>(o[i][3] * f);
+      *(ushort4*)(y + i * 16) = h;
+    }
+    return;
+  }
+  f32x4* out = (f32x4*)p.sums + (size_t)blockIdx.x * (D / 16) * 64 + lane;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) out[i * 64] = o[i];
+  if (quad == 0) p.stats[(size_t)blockIdx.x * 16 + col] = make_float2(m == -INFINITY ? -INFINITY : m * g.scale, l);
+}
+
+// Joins the splits of an item, where it has several: a wave for each 16
+// elements of the head, the splits' sums in f32 over their largest reference.
+template <int D>
+__global__ __launch_bounds__(D * 4) void attention_join_kernel(KvArgs a, AttnArgs g, SplitArgs p) {
   __shared__ int found;
-  __shared__ float qs[256], ps[64];
-  __shared__ size_t rows[64];
-  const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, kh = h / (g.heads / a.kv_heads);
+  const int t = blockIdx.x, hh = blockIdx.y;
   const int seq = sequence_of(a.start, a.batch, t, &found);
   if (seq >= a.batch || t < a.start[seq]) return;
-  for (int d = lane; d < a.d; d += 64) qs[d] = h2f_ieee(g.q[(size_t)t * g.q_stride + g.q_off + (size_t)h * a.d + d]);
-  __syncthreads();
-  const long long most = (long long)a.max_pages << a.page_shift;
-  const long long len = a.len[seq] < 0 ? 0 : min((long long)a.len[seq], most);
-  const long long pos = (long long)a.len[seq] - a.start[seq + 1] + t;
-  const long long end = g.causal ? min(len, pos + 1) : len;
-  const long long begin = g.window > 0 ? max(0ll, pos - g.window + 1) : 0;
-  float m = -INFINITY, l = 0.0f, o[4] = {};
-  for (long long j0 = begin; j0 < end; j0 += 64) {
-    const long long j = j0 + lane;
-    float s = -INFINITY;
-    size_t row = ~(size_t)0;
-    if (j < end) {
-      const int page = a.table[(size_t)seq * a.max_pages + (j >> a.page_shift)];
-      if (page >= 0 && page < a.num_pages) {
-        row = (((size_t)page * a.kv_heads + kh) << a.page_shift) + (j & ((1 << a.page_shift) - 1));
-        s = 0.0f;
-        for (int u = 0; u < a.d / 8; ++u) {
-          float v[8];
-          mx_decode8(a.kc[row * (a.d / 8) + u], mx_scale(a.ks[row * (a.d / 32) + u / 4]), v);
-          for (int e = 0; e < 8; ++e) s = fmaf(qs[u * 8 + e], v[e], s);
-        }
-        s *= g.scale;
-      }
-    }
-    float mx = s;
-    for (int i = 1; i < 64; i *= 2) mx = fmaxf(mx, __shfl_xor(mx, i));
-    const float now = fmaxf(m, mx);
-    const float ref = now == -INFINITY ? 0.0f : now;
-    const float p = row == ~(size_t)0 ? 0.0f : expf(s - ref);
-    float sum = p;
-    for (int i = 1; i < 64; i *= 2) sum += __shfl_xor(sum, i);
-    const float f = expf(m - ref);
-    l = l * f + sum;
-    m = now;
-    ps[lane] = p;
-    rows[lane] = row;
-    __syncthreads();
-    for (int i = 0; i < 4; ++i) o[i] *= f;
-    for (int e = 0; e < 64; ++e) {
-      if (rows[e] == ~(size_t)0) continue;
-      for (int i = 0; i * 64 + lane < a.d; ++i) {
-        const int d = i * 64 + lane;
-        float v[8];
-        mx_decode8(a.vc[rows[e] * (a.d / 8) + d / 8], mx_scale(a.vs[rows[e] * (a.d / 32) + d / 32]), v);
-        float x = v[0];
-        for (int b = 1; b < 8; ++b) x = (d & 7) == b ? v[b] : x;
-        o[i] = fmaf(ps[e], x, o[i]);
-      }
-    }
-    __syncthreads();
+  const int first = max(a.start[seq], 0);
+  if ((t - first) % p.tile_tokens) return;
+  const int2 item = p.items[(size_t)t * a.kv_heads * p.head_tiles + hh];
+  if (item.y <= 1 || item.x < 0 || item.x >= p.splits || item.y > p.splits - item.x) return;
+  const int lane = threadIdx.x & 63, part = threadIdx.x >> 6, col = lane & 15;
+  const float2* stats = p.stats + (size_t)item.x * 16 + col;
+  float m = -INFINITY;
+#pragma unroll 8
+  for (int i = 0; i < item.y; ++i) m = fmaxf(m, stats[i * 16].x);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  const f32x4* sums = (const f32x4*)p.sums + ((size_t)item.x * (D / 16) + part) * 64 + lane;
+  f32x4 o = {};
+  float l = 0.0f;
+#pragma unroll 8
+  for (int i = 0; i < item.y; ++i) {
+    const float2 st = stats[i * 16];
+    const float w = __builtin_amdgcn_exp2f(st.x - ref);
+    o += w * sums[(size_t)i * (D / 16) * 64];
+    l = fmaf(w, st.y, l);
   }
-  for (int i = 0; i * 64 + lane < a.d; ++i)
-    g.y[((size_t)t * g.heads + h) * a.d + i * 64 + lane] = narrow<uint16_t>(l == 0.0f ? 0.0f : o[i] / l);
+  const int kv_head = hh / p.head_tiles, head0 = kv_head * p.group + (hh - kv_head * p.head_tiles) * 16;
+  const int within = p.tile_tokens > 1 ? col / p.group : 0;
+  const int head = head0 + (p.tile_tokens > 1 ? col - within * p.group : col);
+  if (p.tile_tokens > 1 ? col >= p.tile_tokens * p.group : head >= (kv_head + 1) * p.group) return;
+  if (t + within >= min(a.start[seq + 1], a.tokens)) return;
+  const float f = l == 0.0f ? 0.0f : 1.0f / l;
+  ushort4 h;
+  h.x = narrow<uint16_t>(o[0] * f), h.y = narrow<uint16_t>(o[1] * f);
+  h.z = narrow<uint16_t>(o[2] * f), h.w = narrow<uint16_t>(o[3] * f);
+  *(ushort4*)(g.y + ((size_t)(t + within) * g.heads + head) * D + part * 16 + (lane >> 4) * 4) = h;
 }
 
 }  // namespace
@@ -139,8 +468,35 @@ void launch_kv_append(hipStream_t st, const KvArgs& a, const void* k, size_t k_s
   DW_HIP(hipGetLastError());
 }
 
-void launch_attention(hipStream_t st, const KvArgs& a, const AttnArgs& g) {
-  hipLaunchKernelGGL(attention_plain_kernel, dim3((unsigned)a.tokens, (unsigned)g.heads), dim3(64), 0, st, a, g);
+size_t attention_space(const KvArgs& a, const AttnArgs& g, SplitArgs* p) {
+  p->group = g.heads / a.kv_heads;
+  p->head_tiles = (p->group + 15) / 16;
+  p->tile_tokens = std::max(1, 16 / p->group);
+  const long long tiles = std::min<long long>(a.tokens, a.tokens / p->tile_tokens + (long long)a.batch);
+  const long long heads = (long long)a.kv_heads * p->head_tiles;
+  p->waves = 2048;
+  p->least = 2;
+  p->splits = (int)std::min<long long>(tiles * heads + p->waves, 1ll << 25);
+  p->stats_at = (size_t)p->splits * a.d * 64;
+  p->items_at = p->stats_at + (size_t)p->splits * 128;
+  return p->items_at + (size_t)a.tokens * heads * 8;
+}
+
+void launch_attention(hipStream_t st, const KvArgs& a, const AttnArgs& g, SplitArgs p, void* space) {
+  p.sums = (float*)space;
+  p.stats = (float2*)((char*)space + p.stats_at);
+  p.items = (int2*)((char*)space + p.items_at);
+  auto go = [&](auto* split, auto* join) {
+    hipLaunchKernelGGL(split, dim3((unsigned)p.splits), dim3(64), 0, st, a, g, p);
+    hipLaunchKernelGGL(join, dim3((unsigned)a.tokens, (unsigned)(a.kv_heads * p.head_tiles)), dim3(a.d * 4), 0, st, a,
+                       g, p);
+  };
+  if (a.d == 64)
+    go(attention_split_kernel<64>, attention_join_kernel<64>);
+  else if (a.d == 128)
+    go(attention_split_kernel<128>, attention_join_kernel<128>);
+  else
+    go(attention_split_kernel<256>, attention_join_kernel<256>);
   DW_HIP(hipGetLastError());
 }
 
