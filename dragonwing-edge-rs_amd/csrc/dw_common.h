@@ -498,11 +498,11 @@ struct AttnArgs {
 // set by attention_space, which gives the bytes of workspace.
 struct SplitArgs {
   int group, head_tiles;   // heads of a kv head, tiles of 16 of them
-  int tile_tokens;         // new tokens of a tile of 16 rows
+  int tile_tokens, rows;   // new tokens of a tile, its rows (16 at most)
   int waves, least;        // splits wanted, a split's fewest steps of 64 keys
   int splits;              // of the grid
-  float* sums;             // [splits][d / 16][64][4]
-  float2* stats;           // [splits][16]: reference, sum
+  float* sums;             // [splits][rows][d]
+  float2* stats;           // [splits][rows]: reference, sum
   int2* items;             // [tokens][kv heads x head tiles]: first split, splits
   size_t stats_at, items_at;  // bytes into the workspace
 };

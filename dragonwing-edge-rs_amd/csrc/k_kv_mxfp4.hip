@@ -413,50 +413,76 @@ __global__ __launch_bounds__(64) void attention_split_kernel(KvArgs a, AttnArgs 
     }
     return;
   }
-  f32x4* out = (f32x4*)p.sums + (size_t)blockIdx.x * (D / 16) * 64 + lane;
+  if (!real) return;
+  float* out = p.sums + ((size_t)blockIdx.x * p.rows + col) * D + quad * 4;
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) out[i * 64] = o[i];
-  if (quad == 0) p.stats[(size_t)blockIdx.x * 16 + col] = make_float2(m == -INFINITY ? -INFINITY : m * g.scale, l);
+  for (int i = 0; i < D / 16; ++i) *(f32x4*)(out + i * 16) = o[i];
+  if (quad == 0)
+    p.stats[(size_t)blockIdx.x * p.rows + col] = make_float2(m == -INFINITY ? -INFINITY : m * g.scale, l);
 }
 
-// Joins the splits of an item, where it has several: a wave for each 16
-// elements of the head, the splits' sums in f32 over their largest reference.
-template <int D>
-__global__ __launch_bounds__(D * 4) void attention_join_kernel(KvArgs a, AttnArgs g, SplitArgs p) {
+constexpr int kJoinSplits = 1024;
+
+// Joins the splits of an item, where it has several: a workgroup for each of
+// its rows, D / 4 threads a split, so that J = 512 reads 8 to 32 splits at a time;
+// the threads' sums meet in LDS in a fixed order.
+template <int D, int J>
+__global__ __launch_bounds__(J) void attention_join_kernel(KvArgs a, AttnArgs g, SplitArgs p) {
+  constexpr int kWide = J / (D / 4);  // splits at a time
   __shared__ int found;
-  const int t = blockIdx.x, hh = blockIdx.y;
+  __shared__ float weight[kJoinSplits], part[J / 64];
+  __shared__ f32x4 sums[J];
+  const int tid = threadIdx.x, t = blockIdx.x, hh = blockIdx.y, col = blockIdx.z;
   const int seq = sequence_of(a.start, a.batch, t, &found);
   if (seq >= a.batch || t < a.start[seq]) return;
-  const int first = max(a.start[seq], 0);
-  if ((t - first) % p.tile_tokens) return;
-  const int2 item = p.items[(size_t)t * a.kv_heads * p.head_tiles + hh];
+  if ((t - max(a.start[seq], 0)) % p.tile_tokens) return;
+  const int within = p.tile_tokens > 1 ? col / p.group : 0, kv_head = hh / p.head_tiles;
+  const int head = kv_head * p.group + (hh - kv_head * p.head_tiles) * 16 + col - within * p.group;
+  if (head >= (kv_head + 1) * p.group || t + within >= min(a.start[seq + 1], a.tokens)) return;
+  const int2 item = p.items[((size_t)t * a.kv_heads) * p.head_tiles + hh];
   if (item.y <= 1 || item.x < 0 || item.x >= p.splits || item.y > p.splits - item.x) return;
-  const int lane = threadIdx.x & 63, part = threadIdx.x >> 6, col = lane & 15;
-  const float2* stats = p.stats + (size_t)item.x * 16 + col;
+  const float2* stats = p.stats + (size_t)item.x * p.rows + col;
   float m = -INFINITY;
-#pragma unroll 8
-  for (int i = 0; i < item.y; ++i) m = fmaxf(m, stats[i * 16].x);
+  for (int i = tid; i < item.y; i += J) m = fmaxf(m, stats[(size_t)i * p.rows].x);
+  for (int i = 1; i < 64; i *= 2) m = fmaxf(m, __shfl_xor(m, i));
+  if ((tid & 63) == 0) part[tid >> 6] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < J / 64; ++i) m = fmaxf(m, part[i]);
   const float ref = m == -INFINITY ? 0.0f : m;
-  const f32x4* sums = (const f32x4*)p.sums + ((size_t)item.x * (D / 16) + part) * 64 + lane;
+  const int at = tid % (D / 4), lane = tid / (D / 4);
+  const float* src = p.sums + ((size_t)item.x * p.rows + col) * D + at * 4;
   f32x4 o = {};
   float l = 0.0f;
-#pragma unroll 8
-  for (int i = 0; i < item.y; ++i) {
-    const float2 st = stats[i * 16];
-    const float w = __builtin_amdgcn_exp2f(st.x - ref);
-    o += w * sums[(size_t)i * (D / 16) * 64];
-    l = fmaf(w, st.y, l);
+  for (int i0 = 0; i0 < item.y; i0 += kJoinSplits) {
+    const int n = min(kJoinSplits, item.y - i0);
+    __syncthreads();
+    for (int i = tid; i < n; i += J) {
+      const float2 st = stats[(size_t)(i0 + i) * p.rows];
+      const float w = __builtin_amdgcn_exp2f(st.x - ref);
+      weight[i] = w;
+      l = fmaf(w, st.y, l);
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int i = lane; i < n; i += kWide) o += weight[i] * *(const f32x4*)(src + (size_t)(i0 + i) * p.rows * D);
   }
-  const int kv_head = hh / p.head_tiles, head0 = kv_head * p.group + (hh - kv_head * p.head_tiles) * 16;
-  const int within = p.tile_tokens > 1 ? col / p.group : 0;
-  const int head = head0 + (p.tile_tokens > 1 ? col - within * p.group : col);
-  if (p.tile_tokens > 1 ? col >= p.tile_tokens * p.group : head >= (kv_head + 1) * p.group) return;
-  if (t + within >= min(a.start[seq + 1], a.tokens)) return;
+  for (int i = 1; i < 64; i *= 2) l += __shfl_xor(l, i);
+  __syncthreads();
+  if ((tid & 63) == 0) part[tid >> 6] = l;
+  sums[tid] = o;
+  __syncthreads();
+  if (tid >= D / 4) return;
+  l = part[0];
+#pragma unroll
+  for (int i = 1; i < J / 64; ++i) l += part[i];
+#pragma unroll
+  for (int i = 1; i < kWide; ++i) o += sums[i * (D / 4) + tid];
   const float f = l == 0.0f ? 0.0f : 1.0f / l;
   ushort4 h;
   h.x = narrow<uint16_t>(o[0] * f), h.y = narrow<uint16_t>(o[1] * f);
   h.z = narrow<uint16_t>(o[2] * f), h.w = narrow<uint16_t>(o[3] * f);
-  *(ushort4*)(g.y + ((size_t)(t + within) * g.heads + head) * D + part * 16 + (lane >> 4) * 4) = h;
+  *(ushort4*)(g.y + ((size_t)(t + within) * g.heads + head) * D + tid * 4) = h;
 }
 
 }  // namespace
@@ -477,8 +503,9 @@ size_t attention_space(const KvArgs& a, const AttnArgs& g, SplitArgs* p) {
   p->waves = 2048;
   p->least = 2;
   p->splits = (int)std::min<long long>(tiles * heads + p->waves, 1ll << 25);
-  p->stats_at = (size_t)p->splits * a.d * 64;
-  p->items_at = p->stats_at + (size_t)p->splits * 128;
+  p->rows = std::min(16, p->group * p->tile_tokens);
+  p->stats_at = (size_t)p->splits * p->rows * a.d * 4;
+  p->items_at = p->stats_at + (size_t)p->splits * p->rows * 8;
   return p->items_at + (size_t)a.tokens * heads * 8;
 }
 
@@ -486,17 +513,20 @@ void launch_attention(hipStream_t st, const KvArgs& a, const AttnArgs& g, SplitA
   p.sums = (float*)space;
   p.stats = (float2*)((char*)space + p.stats_at);
   p.items = (int2*)((char*)space + p.items_at);
-  auto go = [&](auto* split, auto* join) {
+  // Rows of few splits are many: a wave each then (64 sequences of up to 512
+  // keys, 8 kv heads: see the figures below).
+  const dim3 rows((unsigned)a.tokens, (unsigned)(a.kv_heads * p.head_tiles), (unsigned)p.rows);
+  const bool few = (long long)a.tokens * g.heads <= 1024;
+  auto go = [&](auto* split, auto* wide, auto* wave) {
     hipLaunchKernelGGL(split, dim3((unsigned)p.splits), dim3(64), 0, st, a, g, p);
-    hipLaunchKernelGGL(join, dim3((unsigned)a.tokens, (unsigned)(a.kv_heads * p.head_tiles)), dim3(a.d * 4), 0, st, a,
-                       g, p);
+    hipLaunchKernelGGL(few ? wide : wave, rows, dim3(few ? 512 : 64), 0, st, a, g, p);
   };
   if (a.d == 64)
-    go(attention_split_kernel<64>, attention_join_kernel<64>);
+    go(attention_split_kernel<64>, attention_join_kernel<64, 512>, attention_join_kernel<64, 64>);
   else if (a.d == 128)
-    go(attention_split_kernel<128>, attention_join_kernel<128>);
+    go(attention_split_kernel<128>, attention_join_kernel<128, 512>, attention_join_kernel<128, 64>);
   else
-    go(attention_split_kernel<256>, attention_join_kernel<256>);
+    go(attention_split_kernel<256>, attention_join_kernel<256, 512>, attention_join_kernel<256, 64>);
   DW_HIP(hipGetLastError());
 }
 
