@@ -1327,7 +1327,8 @@ int dw_hip_gemm_mxfp4(dw_hip_backend* be, int a_dtype, const dw_hip_buffer* a, c
   g.k = (int)k;
   g.act = act;
   g.c_half = c_dtype == DW_DTYPE_F16;
-  dw::launch_gemm_mx(b->stream, g);
+  const size_t bytes = dw::gemm_mx_space(g);
+  dw::launch_gemm_mx(b->stream, g, bytes ? b->workspace(Backend::WS_GEMM4, bytes) : nullptr);
   API_END
 }
 

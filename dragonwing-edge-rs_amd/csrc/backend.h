@@ -42,7 +42,7 @@ struct ScratchUse {
 // (the reference's backends are Send + Sync, backend.rs:42-48).  Work from
 // different threads is queued in the order the lock is taken.
 struct Backend {
-  enum { WS_WPACK = 0, WS_SCALE = 1, WS_BIAS = 2, WS_LUT = 3, WS_POST = 4, WS_ATTN = 5, kWsSlots = 6 };
+  enum { WS_WPACK = 0, WS_SCALE = 1, WS_BIAS = 2, WS_LUT = 3, WS_POST = 4, WS_ATTN = 5, WS_GEMM4 = 6, kWsSlots = 7 };
   struct Ws {
     void* ptr = nullptr;
     size_t bytes = 0;

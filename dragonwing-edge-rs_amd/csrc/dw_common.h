@@ -457,8 +457,11 @@ struct GemmMxArgs {
   const void* bias;
   void* c;
   int m, n, k, act, c_half;
+  int lda;  // f16 rows' stride, a multiple of 8: set by the launcher
 };
-void launch_gemm_mx(hipStream_t st, const GemmMxArgs& a);
+// Bytes of workspace that the product wants.
+size_t gemm_mx_space(const GemmMxArgs& a);
+void launch_gemm_mx(hipStream_t st, GemmMxArgs a, void* space);
 
 // Rotary positions: heads of x [tokens][x_stride] from column x_off, to y.
 struct RopeTable {
