@@ -457,7 +457,10 @@ struct GemmMxArgs {
   const void* bias;
   void* c;
   int m, n, k, act, c_half;
-  int lda;  // f16 rows' stride, a multiple of 8: set by the launcher
+  // set by the launcher: f16 rows' stride (a multiple of 8), scale rows' (of
+  // 4), the sums of K's shares [shares][m][ldp]
+  int lda, pitch, ldp;
+  float* parts;
 };
 // Bytes of workspace that the product wants.
 size_t gemm_mx_space(const GemmMxArgs& a);

@@ -62,6 +62,8 @@ __device__ __forceinline__ void store4(const GemmMxArgs& a, size_t row, int n, f
     }
 }
 
+constexpr int kFewRows = 64;
+
 // --- a few rows -----------------------------------------------------------------
 
 // Sixteen scale bytes from block b of a row of `blocks`: four steps of four
@@ -299,56 +301,335 @@ void rows(hipStream_t st, const GemmMxArgs& a) {
     launch_rows<MX, 4, 2>(st, a);
 }
 
-// --- the others -----------------------------------------------------------------
+// --- many rows --------------------------------------------------------------------
 
-template <bool MX>
-__global__ __launch_bounds__(256) void gemm_mx_plain_kernel(GemmMxArgs a) {
-  const size_t blocks = (a.k + 31) / 32, total = (size_t)a.m * a.n;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
-    const size_t row = i / a.n, col = i - row * a.n;
-    const uint32_t* w = (const uint32_t*)a.w + col * blocks * 4;
-    float sum = 0.0f;
-    for (size_t b = 0; b < blocks; ++b) {
-      const float sw = mx_scale(a.ws[col * blocks + b]);
+// Waits until at most N of the wave's loads, and none of its LDS reads, are in
+// flight.
+template <int N>
+__device__ __forceinline__ void loads_left() {
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);
+}
+__device__ __forceinline__ void meet() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+__device__ __align__(16) const uint32_t kZeros[4] = {0, 0, 0, 0};
+
+typedef __attribute__((address_space(3))) void* LdsPtr;
+
+// A tile of WM x TM x 16 rows of A and WN x TN x 16 of W by WM x WN waves, in
+// steps of 128 elements of K that a ring of S stages in LDS holds.
+template <bool MX, int WM, int WN, int TM, int TN, int S>
+struct Tile {
+  static constexpr int kWaves = WM * WN, kRowsA = WM * TM * 16, kRowsW = WN * TN * 16;
+  static constexpr int kA = kRowsA * (MX ? 64 : 256), kW = kRowsW * 64, kSa = MX ? kRowsA * 4 : 0, kSw = kRowsW * 4;
+  static constexpr int kStage = kA + kW + kSa + kSw, kLds = kStage * S;
+  // a wave's loads of a stage, 64 pieces of 16 bytes (or scale words of 4)
+  // each: groups of 16 rows of A and of W, and scales
+  static constexpr int kGroupsA = kRowsA / 16 / kWaves, kGroupsW = kRowsW / 16 / kWaves, kPieces = MX ? 1 : 4;
+  static constexpr int kScales = (kSa + kSw) / 256;
+  static constexpr int kEach = kGroupsA * kPieces + kGroupsW + (kScales + kWaves - 1) / kWaves;
+  static_assert(kRowsA / 16 % kWaves == 0 && kRowsW / 16 % kWaves == 0, "every wave counts the same loads");
+  static_assert(kScales % kWaves == 0 || kWaves % kScales == 0, "and so for the scales");
+  static_assert(kEach * (S - 2) < 64, "the counter of loads");
+
+  // Where a lane's pieces of the first step are, and the step from which on
+  // they lie behind the end of K.  In LDS the pieces follow one another in the
+  // order in which the matrix instruction's lanes take them, so that no read
+  // meets a bank twice.
+  struct Source {
+    const uint8_t *a[kGroupsA], *w[kGroupsW], *s[(kScales + kWaves - 1) / kWaves];
+  };
+  static __device__ __forceinline__ Source source(const GemmMxArgs& g, int m0, int n0, int wave) {
+    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+    const size_t blocks = (g.k + 31) / 32;
+    Source r;
+#pragma unroll
+    for (int i = 0; i < kGroupsA; ++i) {
+      const size_t m = min(m0 + (wave * kGroupsA + i) * 16 + col, g.m - 1);  // rows behind the end are not stored
+      r.a[i] = (const uint8_t*)g.a + (MX ? (m * blocks + quad) * 16 : (m * g.lda + quad * 8) * 2);
+    }
+#pragma unroll
+    for (int i = 0; i < kGroupsW; ++i) {
+      const size_t n = min(n0 + (wave * kGroupsW + i) * 16 + col, g.n - 1);
+      r.w[i] = g.w + (n * blocks + quad) * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < (kScales + kWaves - 1) / kWaves; ++i) {
+      const int row = (wave + i * kWaves) % kScales * 64 + lane;
+      r.s[i] = MX && row < kRowsA ? g.as + (size_t)min(m0 + row, g.m - 1) * g.pitch
+                                  : g.ws + (size_t)min(n0 + row - (MX ? kRowsA : 0), g.n - 1) * g.pitch;
+    }
+    return r;
+  }
+  // TAIL: some of the step's pieces may lie behind the end of K.
+  template <bool TAIL>
+  static __device__ __forceinline__ void load(const GemmMxArgs& g, const Source& r, uint8_t* stage, int step, int wave) {
+    const int quad = (threadIdx.x & 63) >> 4;
+    const bool in = !TAIL || step * 4 + quad < (g.k + 31) / 32;
+    const uint8_t* zeros = (const uint8_t*)kZeros;
+#pragma unroll
+    for (int i = 0; i < kGroupsA; ++i)
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j) {
+        const uint8_t* p = r.a[i] + (size_t)step * (MX ? 64 : 256) + j * 64;
+        if (TAIL && !(MX ? in : step * 128 + j * 32 + quad * 8 < g.lda)) p = zeros;
+        __builtin_amdgcn_global_load_lds((const void*)p, (LdsPtr)(stage + ((wave * kGroupsA + i) * kPieces + j) * 1024),
+                                         16, 0, 0);
+      }
+#pragma unroll
+    for (int i = 0; i < kGroupsW; ++i)
+      __builtin_amdgcn_global_load_lds((const void*)(in ? r.w[i] + (size_t)step * 64 : zeros),
+                                       (LdsPtr)(stage + kA + (wave * kGroupsW + i) * 1024), 16, 0, 0);
+#pragma unroll
+    for (int i = 0; i < (kScales + kWaves - 1) / kWaves; ++i)
+      __builtin_amdgcn_global_load_lds((const void*)(r.s[i] + (size_t)step * 4),
+                                       (LdsPtr)(stage + kA + kW + (wave + i * kWaves) % kScales * 256), 4, 0, 0);
+  }
+
+  // One step: the loads of a later one into `next`, the products of the one in
+  // `p`.  The two never are one stage; that they cannot be is what lets the
+  // reads go ahead of the loads in flight (else each would wait for them).
+  template <bool EXACT>
+  static __device__ __forceinline__ uint32_t step(const GemmMxArgs& a, const Source& src, const uint8_t* __restrict__ p,
+                                                  uint8_t* __restrict__ next, int at, bool tail, int wave,
+                                                  f32x4 (&acc)[TN][TM]) {
+    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4, wm = wave % WM, wn = wave / WM;
+    if (tail)
+      load<true>(a, src, next, at, wave);
+    else
+      load<false>(a, src, next, at, wave);
+    const uint8_t *pa = p + wm * TM * (MX ? 1024 : 4096), *pw = p + kA + wn * TN * 1024;
+    const uint8_t *sw = p + kA + kW + kSa + wn * TN * 64, *sa = p + kA + kW + wm * TM * 64;
+    uint32_t odd = 0;
+    if constexpr (MX) {
+      uint4 x[TM];
+      int fx[TM];
+#pragma unroll
+      for (int u = 0; u < TM; ++u) {
+        x[u] = *(const uint4*)(pa + u * 1024 + lane * 16);
+        fx[u] = sa[u * 64 + col * 4 + quad];
+      }
+#pragma unroll
+      for (int t = 0; t < TN; ++t) {
+        const uint4 y = *(const uint4*)(pw + t * 1024 + lane * 16);
+        const int fw = sw[t * 64 + col * 4 + quad];
+        const i32x8 q = {(int)y.x, (int)y.y, (int)y.z, (int)y.w, 0, 0, 0, 0};
+#pragma unroll
+        for (int u = 0; u < TM; ++u) {
+          const i32x8 v = {(int)x[u].x, (int)x[u].y, (int)x[u].z, (int)x[u].w, 0, 0, 0, 0};
+          acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(q, v, acc[t][u], 4, 4, 0, fw, 0, fx[u]);
+        }
+      }
+    } else {
+#pragma unroll
       for (int j = 0; j < 4; ++j) {
-        float v[8], u[8];
-        mx_decode8(w[b * 4 + j], sw, v);
-        if (MX) mx_decode8(((const uint32_t*)a.a)[(row * blocks + b) * 4 + j], mx_scale(a.as[row * blocks + b]), u);
-        for (int e = 0; e < 8; ++e) {
-          const size_t at = b * 32 + j * 8 + e;
-          if (at < (size_t)a.k) sum = fmaf(MX ? u[e] : h2f_ieee(((const uint16_t*)a.a)[row * a.lda + at]), v[e], sum);
+        f16x8 x[TM];
+#pragma unroll
+        for (int u = 0; u < TM; ++u) x[u] = *(const f16x8*)(pa + (u * 4 + j) * 1024 + lane * 16);
+#pragma unroll
+        for (int t = 0; t < TN; ++t) {
+          const uint32_t y = *(const uint32_t*)(pw + t * 1024 + j * 256 + col * 16 + quad * 4);
+          const uint32_t fb = (uint32_t)sw[t * 64 + col * 4 + j] << 23;
+          const float f = __builtin_bit_cast(float, fb);
+          if constexpr (EXACT) {
+#pragma unroll
+            for (int u = 0; u < TM; ++u) acc[t][u] = times_exact(y, f, x[u], acc[t][u]);
+          } else {
+            odd |= fb - (104u << 23) > (36u << 23) ? y & 0x77777777u : 0u;
+            const f16x8 v = eight_f16(y, f);
+#pragma unroll
+            for (int u = 0; u < TM; ++u)
+              acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, x[u], acc[t][u], 0, 0, 0);
+          }
         }
       }
     }
-    sum = finish(a, (int)col, sum);
-    if (a.c_half)
-      ((uint16_t*)a.c)[i] = narrow<uint16_t>(sum);
-    else
-      ((float*)a.c)[i] = sum;
+    return odd;
+  }
+
+  template <bool EXACT>
+  static __device__ __forceinline__ uint32_t sum(const GemmMxArgs& a, uint8_t* lds, int m0, int n0, int from, int to,
+                                                 f32x4 (&acc)[TN][TM]) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint32_t odd = 0;
+#pragma unroll
+    for (int t = 0; t < TN; ++t)
+#pragma unroll
+      for (int u = 0; u < TM; ++u) acc[t][u] = f32x4{};
+    const Source src = source(a, m0, n0, wave);
+    // the step some of whose pieces may lie behind the end of K
+    const int last = (a.k + 127) / 128 - 1;
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) load<true>(a, src, lds + i * kStage, min(from + i, to - 1), wave);
+    int at = 0;
+    for (int s = from; s < to; ++s) {
+      loads_left<kEach*(S - 2)>();
+      meet();  // the step's operands are there, and the step before is read by all
+      const int later = min(s + S - 1, to - 1);  // behind the share's end: its last step again
+      odd |= step<EXACT>(a, src, lds + at * kStage, lds + (at == 0 ? S - 1 : at - 1) * kStage, later, later == last,
+                         wave, acc);
+      at = at == S - 1 ? 0 : at + 1;
+    }
+    loads_left<0>();
+    meet();
+    return odd;
+  }
+};
+
+template <bool MX, int WM, int WN, int TM, int TN, int S>
+__global__ __launch_bounds__(WM* WN * 64) void gemm_mx_tile_kernel(GemmMxArgs a, int tiles_m, int tiles_n) {
+  using T = Tile<MX, WM, WN, TM, TN, S>;
+  extern __shared__ __align__(16) uint8_t lds[];
+  // Neighbouring workgroups go to the 8 XCDs in turn: each takes a run of
+  // tiles, eight rows of tiles wide, that share operands in its L2.
+  const int total = tiles_m * tiles_n, id = blockIdx.x;
+  const int per = total / 8, rest = total % 8, xcd = id % 8;
+  const int tile = xcd * per + min(xcd, rest) + id / 8;
+  constexpr int kBand = 8;
+  const int band = tile / (kBand * tiles_n), high = min(kBand, tiles_m - band * kBand);
+  const int in = tile - band * kBand * tiles_n;
+  const int m0 = (band * kBand + in % high) * T::kRowsA, n0 = in / high * T::kRowsW;
+  const int steps = ((a.k + 31) / 32 + 3) / 4;
+  const int from = (int)((long long)steps * blockIdx.y / gridDim.y), to = (int)((long long)steps * (blockIdx.y + 1) / gridDim.y);
+  f32x4 acc[TN][TM];
+  const uint32_t odd = T::template sum<false>(a, lds, m0, n0, from, to, acc);
+  if constexpr (!MX) {
+    if (__syncthreads_or(odd != 0)) T::template sum<true>(a, lds, m0, n0, from, to, acc);
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int m1 = m0 + wave % WM * TM * 16 + (lane & 15), n1 = n0 + wave / WM * TN * 16 + (lane >> 4) * 4;
+  if (gridDim.y == 1) {
+#pragma unroll
+    for (int u = 0; u < TM; ++u) {
+      if (m1 + u * 16 >= a.m) continue;
+#pragma unroll
+      for (int t = 0; t < TN; ++t) store4(a, m1 + u * 16, n1 + t * 16, acc[t][u]);
+    }
+    return;
+  }
+  // a share of K: f32 sums, to be joined
+  float* out = a.parts + (size_t)blockIdx.y * a.m * a.ldp;
+#pragma unroll
+  for (int u = 0; u < TM; ++u) {
+    if (m1 + u * 16 >= a.m) continue;
+#pragma unroll
+    for (int t = 0; t < TN; ++t)
+      if (n1 + t * 16 < a.ldp) *(f32x4*)(out + (size_t)(m1 + u * 16) * a.ldp + n1 + t * 16) = acc[t][u];
+  }
+}
+
+// The shares' sums, in order, then bias, activation and rounding.
+__global__ __launch_bounds__(256) void gemm_mx_join_kernel(GemmMxArgs a, int shares) {
+  const int n = (blockIdx.x * 256 + threadIdx.x) * 4;
+  if (n >= a.n) return;
+  for (int m = blockIdx.y; m < a.m; m += gridDim.y) {
+    const float* p = a.parts + (size_t)m * a.ldp + n;
+    f32x4 s = *(const f32x4*)p;
+    for (int i = 1; i < shares; ++i) s += *(const f32x4*)(p + (size_t)i * a.m * a.ldp);
+    store4(a, m, n, s);
+  }
+}
+
+// Scale bytes with each row at a stride of whole words, 127 behind its end.
+__global__ __launch_bounds__(256) void pad_scales_kernel(const uint8_t* __restrict__ s, uint32_t* __restrict__ y,
+                                                         size_t rows, int blocks, int words) {
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < rows * words; i += (size_t)gridDim.x * 256) {
+    const size_t r = i / words;
+    const int b = (int)(i - r * words) * 4;
+    uint32_t v = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v |= (b + j < blocks ? (uint32_t)s[r * blocks + b + j] : 127u) << (8 * j);
+    y[i] = v;
   }
 }
 
 }  // namespace
 
-size_t gemm_mx_space(const GemmMxArgs& a) {
-  return a.as || a.k % 8 == 0 ? 0 : (size_t)a.m * ((a.k + 7) / 8 * 8) * 2;
+namespace {
+
+// How a product of more than 64 rows is cut, and where its workspace lies.
+struct Plan {
+  bool big;      // tiles of 256 columns, else 128
+  int shares;    // of K
+  size_t rows, scales_a, scales_w, parts, bytes;
+};
+Plan plan(const GemmMxArgs& a) {
+  Plan p{};
+  auto take = [&](size_t bytes) {
+    const size_t at = p.bytes;
+    p.bytes += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  const size_t blocks = (a.k + 31) / 32, words = (blocks + 3) / 4;
+  if (!a.as && a.k % 8) p.rows = take((size_t)a.m * ((a.k + 7) / 8 * 8) * 2);
+  if (a.m <= kFewRows) return p;
+  if (blocks % 4) {
+    if (a.as) p.scales_a = take(a.m * words * 4);
+    p.scales_w = take(a.n * words * 4);
+  }
+  auto tiles = [&](int rm, int rn) { return (size_t)((a.m + rm - 1) / rm) * ((a.n + rn - 1) / rn); };
+  p.big = a.as ? tiles(256, 256) >= 192 : tiles(128, 256) >= 192;
+  p.shares = 1;
+  const size_t t = p.big ? 1000 : tiles(128, 128);
+  while (p.shares < 16 && t * p.shares * 2 <= 384 && words / (p.shares * 2) >= 6) p.shares *= 2;
+  if (p.shares > 1) p.parts = take((size_t)p.shares * a.m * ((a.n + 3) / 4 * 4) * 4);
+  return p;
 }
 
+template <bool MX, int WM, int WN, int TM, int TN, int S>
+void launch_tiles(hipStream_t st, const GemmMxArgs& a, int shares) {
+  using T = Tile<MX, WM, WN, TM, TN, S>;
+  const int tm = (a.m + T::kRowsA - 1) / T::kRowsA, tn = (a.n + T::kRowsW - 1) / T::kRowsW;
+  auto* k = gemm_mx_tile_kernel<MX, WM, WN, TM, TN, S>;
+  static const hipError_t sized = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds);
+  DW_HIP(sized);
+  hipLaunchKernelGGL(k, dim3((unsigned)((size_t)tm * tn), (unsigned)shares), dim3(WM * WN * 64), T::kLds, st, a, tm, tn);
+}
+
+}  // namespace
+
+size_t gemm_mx_space(const GemmMxArgs& a) { return plan(a).bytes; }
+
 void launch_gemm_mx(hipStream_t st, GemmMxArgs a, void* space) {
+  const Plan p = plan(a);
+  char* base = (char*)space;
   a.lda = a.k;
   if (!a.as && a.k % 8) {
     a.lda = (a.k + 7) / 8 * 8;
+    void* y = base + p.rows;
     hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)((a.lda + 2047) / 2048), (unsigned)std::min(a.m, 65535)),
-                       dim3(256), 0, st, (const uint16_t*)a.a, (uint16_t*)space, a.m, a.k, a.lda);
-    a.a = space;
+                       dim3(256), 0, st, (const uint16_t*)a.a, (uint16_t*)y, a.m, a.k, a.lda);
+    a.a = y;
   }
-  if (a.m <= 64) {
+  if (a.m <= kFewRows) {
     a.as ? rows<true>(st, a) : rows<false>(st, a);
-  } else {
-    const size_t total = (size_t)a.m * a.n;
-    const dim3 grid((unsigned)std::min<size_t>((total + 255) / 256, 1u << 20));
-    hipLaunchKernelGGL(a.as ? gemm_mx_plain_kernel<true> : gemm_mx_plain_kernel<false>, grid, dim3(256), 0, st, a);
+    DW_HIP(hipGetLastError());
+    return;
   }
+  const int blocks = (a.k + 31) / 32, words = (blocks + 3) / 4;
+  a.pitch = words * 4;
+  if (blocks % 4) {
+    auto pad = [&](const uint8_t*& s, size_t rows, size_t at) {
+      uint32_t* y = (uint32_t*)(base + at);
+      hipLaunchKernelGGL(pad_scales_kernel, dim3((unsigned)std::min<size_t>((rows * words + 255) / 256, 4096)), dim3(256),
+                         0, st, s, y, rows, blocks, words);
+      s = (const uint8_t*)y;
+    };
+    if (a.as) pad(a.as, a.m, p.scales_a);
+    pad(a.ws, a.n, p.scales_w);
+  }
+  a.parts = (float*)(base + p.parts);
+  a.ldp = (a.n + 3) / 4 * 4;
+  if (a.as)
+    p.big ? launch_tiles<true, 2, 4, 8, 4, 4>(st, a, 1) : launch_tiles<true, 2, 2, 4, 4, 4>(st, a, p.shares);
+  else
+    p.big ? launch_tiles<false, 2, 2, 4, 8, 3>(st, a, 1) : launch_tiles<false, 2, 2, 4, 4, 3>(st, a, p.shares);
+  if (p.shares > 1)
+    hipLaunchKernelGGL(gemm_mx_join_kernel, dim3((unsigned)((a.n + 1023) / 1024), (unsigned)std::min(a.m, 65535)),
+                       dim3(256), 0, st, a, p.shares);
   DW_HIP(hipGetLastError());
 }
 

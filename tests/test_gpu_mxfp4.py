@@ -142,6 +142,23 @@ def test_product(backend, m, n, k, kind):
 
 
 @pytest.mark.parametrize("kind", ["f16", "mxfp4"])
+@pytest.mark.parametrize("m,n,k", [(3303, 4001, 100), (1900, 7300, 288), (6500, 2050, 129), (70, 2050, 8200),
+                                   (130, 1030, 14000)])
+def test_large_product(backend, m, n, k, kind):
+    # many tiles, and few with a long K that is shared
+    rng = np.random.default_rng(m)
+    q, s = weights(rng, n, k)
+    a = rng.normal(0, 1, (m, k)).astype(np.float16)
+    wide = a.astype(np.float64)
+    if kind == "mxfp4":
+        a = ref.encode(wide)
+        wide = ref.decode(*a, k)
+    b = rng.normal(0, 1, n).astype(np.float16)
+    want, off = ref.product(wide, ref.decode(q, s, k), b.astype(np.float64), 2)
+    check_product(run_product(backend, a, q, s, m, n, k, b, 2, np.float16), want, off)
+
+
+@pytest.mark.parametrize("kind", ["f16", "mxfp4"])
 @pytest.mark.parametrize("m", [1, 20, 150, 400])
 def test_product_of_far_apart_scales(backend, m, kind):
     # factors of one row from 2^-60 to 2^60, and activations that make every
