@@ -1185,7 +1185,7 @@ int dw_hip_yolo_postprocess(dw_hip_backend* be, const dw_hip_buffer* raw, size_t
 // options) is checked before the handles.
 namespace {
 
-constexpr size_t kMostMx = (size_t)1 << 24;  // of each of a product's sizes, and of a cache's tokens and pages
+constexpr size_t kMostMx = (size_t)1 << 24;  // of a product's rows and columns, and of a cache's tokens and pages
 
 // A buffer of exactly `bytes` on the backend's device.
 void need_on(const Backend* b, const dw_hip_buffer* x, size_t bytes, const char* what) {
@@ -1301,7 +1301,8 @@ int dw_hip_gemm_mxfp4(dw_hip_backend* be, int a_dtype, const dw_hip_buffer* a, c
   const size_t es = float_bytes(c_dtype, "gemm_mxfp4: C");
   check_act(act, "gemm_mxfp4");
   if (!m || !n || !k) dw::fail(DW_ERR_INVALID, "gemm_mxfp4: zero size");
-  if (m > kMostMx || n > kMostMx || k > kMostMx) dw::fail(DW_ERR_UNSUPPORTED, "gemm_mxfp4: a size above 2^24");
+  if (m > kMostMx || n > kMostMx || k > kMostMx / 4)
+    dw::fail(DW_ERR_UNSUPPORTED, "gemm_mxfp4: m or n above 2^24, or k above 2^22");
   const bool mx = a_dtype == DW_DTYPE_MXFP4;
   if (mx != (a_scales != nullptr)) dw::fail(DW_ERR_INVALID, "gemm_mxfp4: scales of A for MXFP4 rows, and only for them");
   Backend* b = B(be);

@@ -303,13 +303,9 @@ void rows(hipStream_t st, const GemmMxArgs& a) {
 
 // --- many rows --------------------------------------------------------------------
 
-// Waits until at most N of the wave's loads, and none of its LDS reads, are in
-// flight.
-template <int N>
-__device__ __forceinline__ void loads_left() {
-  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);
-}
-__device__ __forceinline__ void meet() {
+// All of the wave's loads and LDS reads done, then all waves here.
+__device__ __forceinline__ void settle() {
+  __builtin_amdgcn_s_waitcnt(7 << 4);
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
@@ -319,169 +315,232 @@ __device__ __align__(16) const uint32_t kZeros[4] = {0, 0, 0, 0};
 
 typedef __attribute__((address_space(3))) void* LdsPtr;
 
-// A tile of WM x TM x 16 rows of A and WN x TN x 16 of W by WM x WN waves, in
-// steps of 128 elements of K that a ring of S stages in LDS holds.
-template <bool MX, int WM, int WN, int TM, int TN, int S>
+// A tile of WM x TM x 16 rows of A and WN x TN x 16 of W by WM x WN waves.
+//
+// K goes by in stages of whole cache lines: 256 elements of MXFP4 rows (128
+// bytes), 128 of f16 rows (256 bytes); of W 64 bytes a row there.  Loads write
+// to LDS directly, a stage ahead, into the half of LDS that the last stage
+// left; a stage's products come in parts of one matrix instruction's depth,
+// each part's operands read ahead of the products of the part before, also
+// over the end of a stage.  Scales come four bytes an operand row and 128
+// elements: 16 bytes a row at a time, which last for 512 elements, because
+// each such load touches a line for every row.
+template <bool MX, int WM, int WN, int TM, int TN>
 struct Tile {
   static constexpr int kWaves = WM * WN, kRowsA = WM * TM * 16, kRowsW = WN * TN * 16;
-  static constexpr int kA = kRowsA * (MX ? 64 : 256), kW = kRowsW * 64, kSa = MX ? kRowsA * 4 : 0, kSw = kRowsW * 4;
-  static constexpr int kStage = kA + kW + kSa + kSw, kLds = kStage * S;
-  // a wave's loads of a stage, 64 pieces of 16 bytes (or scale words of 4)
-  // each: groups of 16 rows of A and of W, and scales
-  static constexpr int kGroupsA = kRowsA / 16 / kWaves, kGroupsW = kRowsW / 16 / kWaves, kPieces = MX ? 1 : 4;
-  static constexpr int kScales = (kSa + kSw) / 256;
-  static constexpr int kEach = kGroupsA * kPieces + kGroupsW + (kScales + kWaves - 1) / kWaves;
-  static_assert(kRowsA / 16 % kWaves == 0 && kRowsW / 16 % kWaves == 0, "every wave counts the same loads");
-  static_assert(kScales % kWaves == 0 || kWaves % kScales == 0, "and so for the scales");
-  static_assert(kEach * (S - 2) < 64, "the counter of loads");
+  static constexpr int kDepth = MX ? 256 : 128, kParts = MX ? 2 : 4, kSpan = 512 / kDepth;
+  static constexpr int kLineA = MX ? 128 : 256, kLineW = MX ? 128 : 64;  // bytes of a row and stage
+  static constexpr int kA = kRowsA * kLineA, kW = kRowsW * kLineW, kStage = kA + kW;
+  static constexpr int kScaleRows = (MX ? kRowsA : 0) + kRowsW, kScales = kScaleRows * 16;
+  static constexpr int kLds = 2 * (kStage + kScales);
+  // a wave's loads of a stage, 64 pieces of 16 bytes each, and of scales
+  static constexpr int kLoadsA = kA / 1024 / kWaves, kLoadsW = kW / 1024 / kWaves, kLoadsS = (kScaleRows / 64 + kWaves - 1) / kWaves;
+  static_assert(kLoadsA * kWaves * 1024 == kA && kLoadsW * kWaves * 1024 == kW, "whole loads");
 
-  // Where a lane's pieces of the first step are, and the step from which on
-  // they lie behind the end of K.  In LDS the pieces follow one another in the
-  // order in which the matrix instruction's lanes take them, so that no read
-  // meets a bank twice.
-  struct Source {
-    const uint8_t *a[kGroupsA], *w[kGroupsW], *s[(kScales + kWaves - 1) / kWaves];
-  };
-  static __device__ __forceinline__ Source source(const GemmMxArgs& g, int m0, int n0, int wave) {
-    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+  const GemmMxArgs& g;
+  uint8_t* lds;
+  int m0, n0, wave, lane, col, quad, wm, wn;
+  uint32_t at_a[kLoadsA], at_w[kLoadsW], at_s[kLoadsS];  // a lane's pieces of the first stage, from the tile's rows
+  const uint8_t *base_a, *base_w;
+
+  // LDS keeps rows of A (and, for MXFP4 rows, of W) as they are, but the pieces
+  // of row r stand at their index xor r: eight lanes that read one piece of
+  // eight rows meet all banks.  Rows of W of 64 bytes stand 16 together, piece
+  // by piece.
+  __device__ __forceinline__ Tile(const GemmMxArgs& args, uint8_t* shared, int row0, int col0)
+      : g(args), lds(shared), m0(row0), n0(col0) {
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4, wm = wave % WM, wn = wave / WM;
     const size_t blocks = (g.k + 31) / 32;
-    Source r;
+    const size_t row_a = MX ? blocks * 16 : (size_t)g.lda * 2, row_w = blocks * 16;
+    base_a = (const uint8_t*)g.a + m0 * row_a;
+    base_w = g.w + n0 * row_w;
 #pragma unroll
-    for (int i = 0; i < kGroupsA; ++i) {
-      const size_t m = min(m0 + (wave * kGroupsA + i) * 16 + col, g.m - 1);  // rows behind the end are not stored
-      r.a[i] = (const uint8_t*)g.a + (MX ? (m * blocks + quad) * 16 : (m * g.lda + quad * 8) * 2);
+    for (int i = 0; i < kLoadsA; ++i) {
+      const int r = (wave * kLoadsA + i) * (1024 / kLineA) + lane / (kLineA / 16);
+      at_a[i] = (uint32_t)(min(r, g.m - 1 - m0) * row_a) + piece_a(i) * 16;  // rows behind the end are not stored
     }
 #pragma unroll
-    for (int i = 0; i < kGroupsW; ++i) {
-      const size_t n = min(n0 + (wave * kGroupsW + i) * 16 + col, g.n - 1);
-      r.w[i] = g.w + (n * blocks + quad) * 16;
+    for (int i = 0; i < kLoadsW; ++i) {
+      const int r = MX ? (wave * kLoadsW + i) * 8 + lane / 8 : (wave * kLoadsW + i) * 16 + col;
+      at_w[i] = (uint32_t)(min(r, g.n - 1 - n0) * row_w) + piece_w() * 16;
     }
 #pragma unroll
-    for (int i = 0; i < (kScales + kWaves - 1) / kWaves; ++i) {
-      const int row = (wave + i * kWaves) % kScales * 64 + lane;
-      r.s[i] = MX && row < kRowsA ? g.as + (size_t)min(m0 + row, g.m - 1) * g.pitch
-                                  : g.ws + (size_t)min(n0 + row - (MX ? kRowsA : 0), g.n - 1) * g.pitch;
+    for (int i = 0; i < kLoadsS; ++i) {
+      const int r = scale_row(i);
+      at_s[i] = (uint32_t)((MX && r < kRowsA ? min(r, g.m - 1 - m0) : min(r - (MX ? kRowsA : 0), g.n - 1 - n0)) * g.pitch);
     }
-    return r;
   }
-  // TAIL: some of the step's pieces may lie behind the end of K.
-  template <bool TAIL>
-  static __device__ __forceinline__ void load(const GemmMxArgs& g, const Source& r, uint8_t* stage, int step, int wave) {
-    const int quad = (threadIdx.x & 63) >> 4;
-    const bool in = !TAIL || step * 4 + quad < (g.k + 31) / 32;
-    const uint8_t* zeros = (const uint8_t*)kZeros;
+  __device__ __forceinline__ int piece_a(int i) const {
+    const int r = i * (1024 / kLineA) + lane / (kLineA / 16);  // of the row's last three bits
+    return lane % (kLineA / 16) ^ (r & 7);
+  }
+  __device__ __forceinline__ int piece_w() const { return MX ? lane % 8 ^ lane / 8 : quad; }
+  __device__ __forceinline__ int scale_row(int i) const { return (wave + i * kWaves) % (kScaleRows / 64) * 64 + lane; }
+
+  // LAST: some of the stage's pieces may lie behind the end of K.
+  template <bool LAST>
+  __device__ __forceinline__ void load(uint8_t* __restrict__ slot, int stage) const {
+    const uint8_t* pa = base_a + (size_t)stage * kLineA;
+    const uint8_t* pw = base_w + (size_t)stage * kLineW;
+    const int pieces = LAST ? (MX ? (g.k + 31) / 32 - stage * 8 : (g.lda - stage * 128) / 8) : 0;
+    const int pieces_w = LAST ? (g.k + 31) / 32 - stage * (MX ? 8 : 4) : 0;
 #pragma unroll
-    for (int i = 0; i < kGroupsA; ++i)
+    for (int i = 0; i < kLoadsA; ++i) {
+      const uint8_t* p = pa + at_a[i];
+      if (LAST && piece_a(i) >= pieces) p = (const uint8_t*)kZeros;
+      __builtin_amdgcn_global_load_lds((const void*)p, (LdsPtr)(slot + (wave * kLoadsA + i) * 1024), 16, 0, 0);
+    }
 #pragma unroll
-      for (int j = 0; j < kPieces; ++j) {
-        const uint8_t* p = r.a[i] + (size_t)step * (MX ? 64 : 256) + j * 64;
-        if (TAIL && !(MX ? in : step * 128 + j * 32 + quad * 8 < g.lda)) p = zeros;
-        __builtin_amdgcn_global_load_lds((const void*)p, (LdsPtr)(stage + ((wave * kGroupsA + i) * kPieces + j) * 1024),
-                                         16, 0, 0);
-      }
+    for (int i = 0; i < kLoadsW; ++i) {
+      const uint8_t* p = pw + at_w[i];
+      if (LAST && piece_w() >= pieces_w) p = (const uint8_t*)kZeros;
+      __builtin_amdgcn_global_load_lds((const void*)p, (LdsPtr)(slot + kA + (wave * kLoadsW + i) * 1024), 16, 0, 0);
+    }
+  }
+  // The scales of 512 elements.
+  __device__ __forceinline__ void load_scales(uint8_t* __restrict__ slot, int span) const {
+    const int at = min(span, g.pitch / 16 - 1) * 16;
 #pragma unroll
-    for (int i = 0; i < kGroupsW; ++i)
-      __builtin_amdgcn_global_load_lds((const void*)(in ? r.w[i] + (size_t)step * 64 : zeros),
-                                       (LdsPtr)(stage + kA + (wave * kGroupsW + i) * 1024), 16, 0, 0);
-#pragma unroll
-    for (int i = 0; i < (kScales + kWaves - 1) / kWaves; ++i)
-      __builtin_amdgcn_global_load_lds((const void*)(r.s[i] + (size_t)step * 4),
-                                       (LdsPtr)(stage + kA + kW + (wave + i * kWaves) % kScales * 256), 4, 0, 0);
+    for (int i = 0; i < kLoadsS; ++i) {
+      const bool of_a = MX && scale_row(i) < kRowsA;  // the same for the wave
+      const uint8_t* p = (of_a ? g.as + (size_t)m0 * g.pitch : g.ws + (size_t)n0 * g.pitch) + at + at_s[i];
+      __builtin_amdgcn_global_load_lds((const void*)p, (LdsPtr)(slot + (wave + i * kWaves) % (kScaleRows / 64) * 1024), 16,
+                                       0, 0);
+    }
   }
 
-  // One step: the loads of a later one into `next`, the products of the one in
-  // `p`.  The two never are one stage; that they cannot be is what lets the
-  // reads go ahead of the loads in flight (else each would wait for them).
-  template <bool EXACT>
-  static __device__ __forceinline__ uint32_t step(const GemmMxArgs& a, const Source& src, const uint8_t* __restrict__ p,
-                                                  uint8_t* __restrict__ next, int at, bool tail, int wave,
-                                                  f32x4 (&acc)[TN][TM]) {
-    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4, wm = wave % WM, wn = wave / WM;
-    if (tail)
-      load<true>(a, src, next, at, wave);
-    else
-      load<false>(a, src, next, at, wave);
-    const uint8_t *pa = p + wm * TM * (MX ? 1024 : 4096), *pw = p + kA + wn * TN * 1024;
-    const uint8_t *sw = p + kA + kW + kSa + wn * TN * 64, *sa = p + kA + kW + wm * TM * 64;
-    uint32_t odd = 0;
+  // A wave's operands of a part.
+  struct Operands {
+    uint4 x[TM];
+    uint32_t fx[MX ? TM : 1];
+    uint4 y[MX ? TN : 1];
+    uint32_t word[MX ? 1 : TN], fw[TN];
+  };
+  __device__ __forceinline__ void read(const uint8_t* __restrict__ p, const uint8_t* __restrict__ scales, int stage,
+                                       int part, Operands& r) const {
+    const uint8_t* pa = p + wm * TM * 16 * kLineA + col * kLineA + (((quad ^ (col & 7)) ^ part * 4) * 16);
+#pragma unroll
+    for (int u = 0; u < TM; ++u) r.x[u] = *(const uint4*)(pa + u * 16 * kLineA);
     if constexpr (MX) {
-      uint4 x[TM];
-      int fx[TM];
+      const uint8_t* sa = scales + (wm * TM * 16 + col) * 16 + (stage & 1) * 8 + part * 4 + quad;
+      const uint8_t* sw = scales + (kRowsA + wn * TN * 16 + col) * 16 + (stage & 1) * 8 + part * 4 + quad;
+      const uint8_t* pw = p + kA + wn * TN * 2048 + col * 128 + (((quad ^ (col & 7)) ^ part * 4) * 16);
 #pragma unroll
-      for (int u = 0; u < TM; ++u) {
-        x[u] = *(const uint4*)(pa + u * 1024 + lane * 16);
-        fx[u] = sa[u * 64 + col * 4 + quad];
-      }
+      for (int u = 0; u < TM; ++u) r.fx[u] = sa[u * 256];
 #pragma unroll
-      for (int t = 0; t < TN; ++t) {
-        const uint4 y = *(const uint4*)(pw + t * 1024 + lane * 16);
-        const int fw = sw[t * 64 + col * 4 + quad];
-        const i32x8 q = {(int)y.x, (int)y.y, (int)y.z, (int)y.w, 0, 0, 0, 0};
+      for (int t = 0; t < TN; ++t) r.y[t] = *(const uint4*)(pw + t * 2048);
+#pragma unroll
+      for (int t = 0; t < TN; ++t) r.fw[t] = sw[t * 256];
+    } else {
+      const uint8_t* sw = scales + (wn * TN * 16 + col) * 16 + (stage & 3) * 4;
+      const uint8_t* pw = p + kA + wn * TN * 1024 + part * 256 + col * 16 + quad * 4;
+#pragma unroll
+      for (int t = 0; t < TN; ++t) r.word[t] = *(const uint32_t*)(pw + t * 1024);
+#pragma unroll
+      for (int t = 0; t < TN; ++t) r.fw[t] = *(const uint32_t*)(sw + t * 256);
+    }
+  }
+  template <bool EXACT>
+  static __device__ __forceinline__ void multiply(const Operands& r, int part, uint32_t* far, f32x4 (&acc)[TN][TM]) {
+#pragma unroll
+    for (int t = 0; t < TN; ++t) {
+      if constexpr (MX) {
+        const i32x8 q = {(int)r.y[t].x, (int)r.y[t].y, (int)r.y[t].z, (int)r.y[t].w, 0, 0, 0, 0};
 #pragma unroll
         for (int u = 0; u < TM; ++u) {
-          const i32x8 v = {(int)x[u].x, (int)x[u].y, (int)x[u].z, (int)x[u].w, 0, 0, 0, 0};
-          acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(q, v, acc[t][u], 4, 4, 0, fw, 0, fx[u]);
+          const i32x8 v = {(int)r.x[u].x, (int)r.x[u].y, (int)r.x[u].z, (int)r.x[u].w, 0, 0, 0, 0};
+          acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(q, v, acc[t][u], 4, 4, 0, (int)r.fw[t], 0,
+                                                                      (int)r.fx[u]);
         }
-      }
-    } else {
+      } else {
+        const float f = __builtin_bit_cast(float, part == 3 ? r.fw[t] >> 1 : r.fw[t] << (23 - 8 * part));
+        if constexpr (EXACT) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        f16x8 x[TM];
+          for (int u = 0; u < TM; ++u) acc[t][u] = times_exact(r.word[t], f, __builtin_bit_cast(f16x8, r.x[u]), acc[t][u]);
+        } else {
+          // factors of 2^-15 to 1, as weights have them, four at a time
+          if (part == 0) *far |= (r.fw[t] ^ 0x70707070u) & 0xF0F0F0F0u;
+          const f16x8 v = eight_f16(r.word[t], f);
 #pragma unroll
-        for (int u = 0; u < TM; ++u) x[u] = *(const f16x8*)(pa + (u * 4 + j) * 1024 + lane * 16);
-#pragma unroll
-        for (int t = 0; t < TN; ++t) {
-          const uint32_t y = *(const uint32_t*)(pw + t * 1024 + j * 256 + col * 16 + quad * 4);
-          const uint32_t fb = (uint32_t)sw[t * 64 + col * 4 + j] << 23;
-          const float f = __builtin_bit_cast(float, fb);
-          if constexpr (EXACT) {
-#pragma unroll
-            for (int u = 0; u < TM; ++u) acc[t][u] = times_exact(y, f, x[u], acc[t][u]);
-          } else {
-            odd |= fb - (104u << 23) > (36u << 23) ? y & 0x77777777u : 0u;
-            const f16x8 v = eight_f16(y, f);
-#pragma unroll
-            for (int u = 0; u < TM; ++u)
-              acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, x[u], acc[t][u], 0, 0, 0);
-          }
+          for (int u = 0; u < TM; ++u)
+            acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, __builtin_bit_cast(f16x8, r.x[u]), acc[t][u], 0, 0, 0);
         }
       }
     }
-    return odd;
   }
 
+  // Stages [from, to), from a multiple of kSpan.  A stage reads from `cur` and
+  // loads into `next`: that the two are apart is what lets reads go ahead of
+  // loads in flight (else each would wait for them).
+  template <bool EXACT, int MORE>  // MORE: 0 no stage follows, 1 the last may, 2 any
+  __device__ __forceinline__ void stage(const uint8_t* __restrict__ cur, const uint8_t* __restrict__ scales,
+                                        uint8_t* __restrict__ next, uint8_t* __restrict__ next_scales, int s,
+                                        Operands& one, Operands& two, uint32_t* far, f32x4 (&acc)[TN][TM]) const {
+    if constexpr (MORE != 0) {
+      load<MORE == 1>(next, s + 1);
+      if ((s + 1) % kSpan == kSpan - 1) load_scales(next_scales, (s + 1) / kSpan + 1);
+    }
+    read(cur, scales, s, 0, one);
+    multiply<EXACT>(two, kParts - 1, far, acc);  // of the stage before
+#pragma unroll
+    for (int i = 1; i < kParts; ++i) {
+      Operands& now = i % 2 ? one : two;
+      Operands& then = i % 2 ? two : one;
+      read(cur, scales, s, i, then);
+      multiply<EXACT>(now, i - 1, far, acc);
+    }
+  }
   template <bool EXACT>
-  static __device__ __forceinline__ uint32_t sum(const GemmMxArgs& a, uint8_t* lds, int m0, int n0, int from, int to,
-                                                 f32x4 (&acc)[TN][TM]) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    uint32_t odd = 0;
+  __device__ __forceinline__ uint32_t sum(int from, int to, f32x4 (&acc)[TN][TM]) const {
+    uint32_t far = 0;
 #pragma unroll
     for (int t = 0; t < TN; ++t)
 #pragma unroll
       for (int u = 0; u < TM; ++u) acc[t][u] = f32x4{};
-    const Source src = source(a, m0, n0, wave);
-    // the step some of whose pieces may lie behind the end of K
-    const int last = (a.k + 127) / 128 - 1;
+    Operands one, two = {};  // zeros times zeros come before the first stage
+    if constexpr (!MX) {
 #pragma unroll
-    for (int i = 0; i < S - 1; ++i) load<true>(a, src, lds + i * kStage, min(from + i, to - 1), wave);
-    int at = 0;
-    for (int s = from; s < to; ++s) {
-      loads_left<kEach*(S - 2)>();
-      meet();  // the step's operands are there, and the step before is read by all
-      const int later = min(s + S - 1, to - 1);  // behind the share's end: its last step again
-      odd |= step<EXACT>(a, src, lds + at * kStage, lds + (at == 0 ? S - 1 : at - 1) * kStage, later, later == last,
-                         wave, acc);
-      at = at == S - 1 ? 0 : at + 1;
+      for (int t = 0; t < TN; ++t) two.fw[t] = 0x70707070u;
     }
-    loads_left<0>();
-    meet();
+    load<true>(lds, from);
+    load_scales(lds + 2 * kStage, from / kSpan);
+    auto slot = [&](int s) { return lds + ((s - from) & 1) * kStage; };
+    auto scales = [&](int span) { return lds + 2 * kStage + ((span - from / kSpan) & 1) * kScales; };
+    int s = from;
+    for (; s < to - 2; ++s) {
+      settle();
+      stage<EXACT, 2>(slot(s), scales(s / kSpan), slot(s + 1), scales((s + 1) / kSpan + 1), s, one, two, &far, acc);
+    }
+    if (s < to - 1) {
+      settle();
+      stage<EXACT, 1>(slot(s), scales(s / kSpan), slot(s + 1), scales((s + 1) / kSpan + 1), s, one, two, &far, acc);
+      ++s;
+    }
+    settle();
+    stage<EXACT, 0>(slot(s), scales(s / kSpan), slot(s + 1), scales(s / kSpan + 1), s, one, two, &far, acc);
+    multiply<EXACT>(two, kParts - 1, &far, acc);
+    settle();
+    return far;
+  }
+  // Whether f16 does not hold a weight of the tile: factors one by one.
+  __device__ __forceinline__ bool outside(int from, int to) const {
+    const int blocks = (g.k + 31) / 32, b0 = from * (kDepth / 32), b1 = min(to * (kDepth / 32), blocks);
+    bool odd = false;
+    for (int i = threadIdx.x; i < (b1 - b0) * kRowsW; i += kWaves * 64) {
+      const size_t r = min(n0 + i / (b1 - b0), g.n - 1), b = b0 + i % (b1 - b0);
+      if (g.ws[r * g.pitch + b] - 104u > 36u) {
+        const uint4 q = *(const uint4*)(g.w + (r * blocks + b) * 16);
+        odd |= ((q.x | q.y | q.z | q.w) & 0x77777777u) != 0;
+      }
+    }
     return odd;
   }
 };
 
-template <bool MX, int WM, int WN, int TM, int TN, int S>
+template <bool MX, int WM, int WN, int TM, int TN>
 __global__ __launch_bounds__(WM* WN * 64) void gemm_mx_tile_kernel(GemmMxArgs a, int tiles_m, int tiles_n) {
-  using T = Tile<MX, WM, WN, TM, TN, S>;
+  using T = Tile<MX, WM, WN, TM, TN>;
   extern __shared__ __align__(16) uint8_t lds[];
   // Neighbouring workgroups go to the 8 XCDs in turn: each takes a run of
   // tiles, eight rows of tiles wide, that share operands in its L2.
@@ -492,12 +551,14 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_mx_tile_kernel(GemmMxArgs a,
   const int band = tile / (kBand * tiles_n), high = min(kBand, tiles_m - band * kBand);
   const int in = tile - band * kBand * tiles_n;
   const int m0 = (band * kBand + in % high) * T::kRowsA, n0 = in / high * T::kRowsW;
-  const int steps = ((a.k + 31) / 32 + 3) / 4;
-  const int from = (int)((long long)steps * blockIdx.y / gridDim.y), to = (int)((long long)steps * (blockIdx.y + 1) / gridDim.y);
+  const int stages = (a.k + T::kDepth - 1) / T::kDepth, spans = (stages + T::kSpan - 1) / T::kSpan;
+  const int from = (int)((long long)spans * blockIdx.y / gridDim.y) * T::kSpan;
+  const int to = min(stages, (int)((long long)spans * (blockIdx.y + 1) / gridDim.y) * T::kSpan);
   f32x4 acc[TN][TM];
-  const uint32_t odd = T::template sum<false>(a, lds, m0, n0, from, to, acc);
+  const T t(a, lds, m0, n0);
+  const uint32_t far = t.template sum<false>(from, to, acc);
   if constexpr (!MX) {
-    if (__syncthreads_or(odd != 0)) T::template sum<true>(a, lds, m0, n0, from, to, acc);
+    if (__syncthreads_or(far != 0) && __syncthreads_or(t.outside(from, to))) t.template sum<true>(from, to, acc);
   }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int m1 = m0 + wave % WM * TM * 16 + (lane & 15), n1 = n0 + wave / WM * TN * 16 + (lane >> 4) * 4;
@@ -506,7 +567,7 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_mx_tile_kernel(GemmMxArgs a,
     for (int u = 0; u < TM; ++u) {
       if (m1 + u * 16 >= a.m) continue;
 #pragma unroll
-      for (int t = 0; t < TN; ++t) store4(a, m1 + u * 16, n1 + t * 16, acc[t][u]);
+      for (int i = 0; i < TN; ++i) store4(a, m1 + u * 16, n1 + i * 16, acc[i][u]);
     }
     return;
   }
@@ -516,8 +577,8 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_mx_tile_kernel(GemmMxArgs a,
   for (int u = 0; u < TM; ++u) {
     if (m1 + u * 16 >= a.m) continue;
 #pragma unroll
-    for (int t = 0; t < TN; ++t)
-      if (n1 + t * 16 < a.ldp) *(f32x4*)(out + (size_t)(m1 + u * 16) * a.ldp + n1 + t * 16) = acc[t][u];
+    for (int i = 0; i < TN; ++i)
+      if (n1 + i * 16 < a.ldp) *(f32x4*)(out + (size_t)(m1 + u * 16) * a.ldp + n1 + i * 16) = acc[i][u];
   }
 }
 
@@ -533,7 +594,7 @@ __global__ __launch_bounds__(256) void gemm_mx_join_kernel(GemmMxArgs a, int sha
   }
 }
 
-// Scale bytes with each row at a stride of whole words, 127 behind its end.
+// Scale bytes with each row at a stride of 16 bytes or more, 127 behind its end.
 __global__ __launch_bounds__(256) void pad_scales_kernel(const uint8_t* __restrict__ s, uint32_t* __restrict__ y,
                                                          size_t rows, int blocks, int words) {
   for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < rows * words; i += (size_t)gridDim.x * 256) {
@@ -563,27 +624,27 @@ Plan plan(const GemmMxArgs& a) {
     p.bytes += (bytes + 255) / 256 * 256;
     return at;
   };
-  const size_t blocks = (a.k + 31) / 32, words = (blocks + 3) / 4;
+  const size_t blocks = (a.k + 31) / 32, pitch = (blocks + 15) / 16 * 16;
   if (!a.as && a.k % 8) p.rows = take((size_t)a.m * ((a.k + 7) / 8 * 8) * 2);
   if (a.m <= kFewRows) return p;
-  if (blocks % 4) {
-    if (a.as) p.scales_a = take(a.m * words * 4);
-    p.scales_w = take(a.n * words * 4);
+  if (blocks % 16) {
+    if (a.as) p.scales_a = take(a.m * pitch);
+    p.scales_w = take(a.n * pitch);
   }
   auto tiles = [&](int rm, int rn) { return (size_t)((a.m + rm - 1) / rm) * ((a.n + rn - 1) / rn); };
   p.big = a.as ? tiles(256, 256) >= 192 : tiles(128, 256) >= 192;
   p.shares = 1;
   const size_t t = p.big ? 1000 : tiles(128, 128);
-  while (p.shares < 16 && t * p.shares * 2 <= 384 && words / (p.shares * 2) >= 6) p.shares *= 2;
+  while (p.shares < 16 && t * p.shares * 2 <= 384 && pitch / 16 / (p.shares * 2) >= 2) p.shares *= 2;
   if (p.shares > 1) p.parts = take((size_t)p.shares * a.m * ((a.n + 3) / 4 * 4) * 4);
   return p;
 }
 
-template <bool MX, int WM, int WN, int TM, int TN, int S>
+template <bool MX, int WM, int WN, int TM, int TN>
 void launch_tiles(hipStream_t st, const GemmMxArgs& a, int shares) {
-  using T = Tile<MX, WM, WN, TM, TN, S>;
+  using T = Tile<MX, WM, WN, TM, TN>;
   const int tm = (a.m + T::kRowsA - 1) / T::kRowsA, tn = (a.n + T::kRowsW - 1) / T::kRowsW;
-  auto* k = gemm_mx_tile_kernel<MX, WM, WN, TM, TN, S>;
+  auto* k = gemm_mx_tile_kernel<MX, WM, WN, TM, TN>;
   static const hipError_t sized = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds);
   DW_HIP(sized);
   hipLaunchKernelGGL(k, dim3((unsigned)((size_t)tm * tn), (unsigned)shares), dim3(WM * WN * 64), T::kLds, st, a, tm, tn);
@@ -609,9 +670,9 @@ void launch_gemm_mx(hipStream_t st, GemmMxArgs a, void* space) {
     DW_HIP(hipGetLastError());
     return;
   }
-  const int blocks = (a.k + 31) / 32, words = (blocks + 3) / 4;
+  const int blocks = (a.k + 31) / 32, words = (blocks + 15) / 16 * 4;
   a.pitch = words * 4;
-  if (blocks % 4) {
+  if (blocks % 16) {
     auto pad = [&](const uint8_t*& s, size_t rows, size_t at) {
       uint32_t* y = (uint32_t*)(base + at);
       hipLaunchKernelGGL(pad_scales_kernel, dim3((unsigned)std::min<size_t>((rows * words + 255) / 256, 4096)), dim3(256),
@@ -624,9 +685,9 @@ void launch_gemm_mx(hipStream_t st, GemmMxArgs a, void* space) {
   a.parts = (float*)(base + p.parts);
   a.ldp = (a.n + 3) / 4 * 4;
   if (a.as)
-    p.big ? launch_tiles<true, 2, 4, 8, 4, 4>(st, a, 1) : launch_tiles<true, 2, 2, 4, 4, 4>(st, a, p.shares);
+    p.big ? launch_tiles<true, 2, 2, 8, 8>(st, a, 1) : launch_tiles<true, 2, 2, 4, 4>(st, a, p.shares);
   else
-    p.big ? launch_tiles<false, 2, 2, 4, 8, 3>(st, a, 1) : launch_tiles<false, 2, 2, 4, 4, 3>(st, a, p.shares);
+    p.big ? launch_tiles<false, 2, 2, 4, 8>(st, a, 1) : launch_tiles<false, 2, 2, 4, 4>(st, a, p.shares);
   if (p.shares > 1)
     hipLaunchKernelGGL(gemm_mx_join_kernel, dim3((unsigned)((a.n + 1023) / 1024), (unsigned)std::min(a.m, 65535)),
                        dim3(256), 0, st, a, p.shares);

@@ -359,7 +359,8 @@ int dw_hip_dequantize_mxfp4(dw_hip_backend* be, int dtype, const dw_hip_buffer* 
  * c_dtype: of C and of the bias (may be NULL), F32 or F16.  Products are
  * exact and summed in f32 in an order of the library's own; bias and
  * activation (DW_ACT_*) are f32, and C is rounded once.  Elements of W and A
- * behind a row's k must be 0, as quantize writes them.  Each size at most 2^24. */
+ * behind a row's k must be 0, as quantize writes them.  m and n at most 2^24,
+ * k at most 2^22. */
 int dw_hip_gemm_mxfp4(dw_hip_backend* be, int a_dtype, const dw_hip_buffer* a, const dw_hip_buffer* a_scales,
                       const dw_hip_buffer* w, const dw_hip_buffer* w_scales, const dw_hip_buffer* bias, int c_dtype,
                       dw_hip_buffer* c, size_t m, size_t n, size_t k, int act);
