@@ -333,6 +333,7 @@ struct Tile {
   static constexpr int kA = kRowsA * kLineA, kW = kRowsW * kLineW, kStage = kA + kW;
   static constexpr int kScaleRows = (MX ? kRowsA : 0) + kRowsW, kScales = kScaleRows * 16;
   static constexpr int kLds = 2 * (kStage + kScales);
+  static constexpr bool kAhead = TM * TN <= 16;  // the others' sums leave no registers for operands read ahead
   // a wave's loads of a stage, 64 pieces of 16 bytes each, and of scales
   static constexpr int kLoadsA = kA / 1024 / kWaves, kLoadsW = kW / 1024 / kWaves, kLoadsS = (kScaleRows / 64 + kWaves - 1) / kWaves;
   static_assert(kLoadsA * kWaves * 1024 == kA && kLoadsW * kWaves * 1024 == kW, "whole loads");
@@ -470,6 +471,17 @@ struct Tile {
     }
   }
 
+  // Reads stay ahead of the products, and the products of a wave that has its
+  // operands go before the other waves' reads.
+  template <bool EXACT>
+  static __device__ __forceinline__ void products(const Operands& r, int part, uint32_t* far, f32x4 (&acc)[TN][TM]) {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+    multiply<EXACT>(r, part, far, acc);
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
   // Stages [from, to), from a multiple of kSpan.  A stage reads from `cur` and
   // loads into `next`: that the two are apart is what lets reads go ahead of
   // loads in flight (else each would wait for them).
@@ -478,17 +490,25 @@ struct Tile {
                                         uint8_t* __restrict__ next, uint8_t* __restrict__ next_scales, int s,
                                         Operands& one, Operands& two, uint32_t* far, f32x4 (&acc)[TN][TM]) const {
     if constexpr (MORE != 0) {
+      if (s % kSpan == 0) load_scales(next_scales, s / kSpan + 1);
       load<MORE == 1>(next, s + 1);
-      if ((s + 1) % kSpan == kSpan - 1) load_scales(next_scales, (s + 1) / kSpan + 1);
+    }
+    if constexpr (!kAhead) {
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) {
+        read(cur, scales, s, i, one);
+        products<EXACT>(one, i, far, acc);
+      }
+      return;
     }
     read(cur, scales, s, 0, one);
-    multiply<EXACT>(two, kParts - 1, far, acc);  // of the stage before
+    products<EXACT>(two, kParts - 1, far, acc);  // of the stage before
 #pragma unroll
     for (int i = 1; i < kParts; ++i) {
       Operands& now = i % 2 ? one : two;
       Operands& then = i % 2 ? two : one;
       read(cur, scales, s, i, then);
-      multiply<EXACT>(now, i - 1, far, acc);
+      products<EXACT>(now, i - 1, far, acc);
     }
   }
   template <bool EXACT>
@@ -503,23 +523,23 @@ struct Tile {
 #pragma unroll
       for (int t = 0; t < TN; ++t) two.fw[t] = 0x70707070u;
     }
-    load<true>(lds, from);
     load_scales(lds + 2 * kStage, from / kSpan);
-    auto slot = [&](int s) { return lds + ((s - from) & 1) * kStage; };
+    load<true>(lds, from);
+    auto slot = [&](int i) { return lds + ((i - from) & 1) * kStage; };
     auto scales = [&](int span) { return lds + 2 * kStage + ((span - from / kSpan) & 1) * kScales; };
     int s = from;
     for (; s < to - 2; ++s) {
       settle();
-      stage<EXACT, 2>(slot(s), scales(s / kSpan), slot(s + 1), scales((s + 1) / kSpan + 1), s, one, two, &far, acc);
+      stage<EXACT, 2>(slot(s), scales(s / kSpan), slot(s + 1), scales(s / kSpan + 1), s, one, two, &far, acc);
     }
     if (s < to - 1) {
       settle();
-      stage<EXACT, 1>(slot(s), scales(s / kSpan), slot(s + 1), scales((s + 1) / kSpan + 1), s, one, two, &far, acc);
+      stage<EXACT, 1>(slot(s), scales(s / kSpan), slot(s + 1), scales(s / kSpan + 1), s, one, two, &far, acc);
       ++s;
     }
     settle();
     stage<EXACT, 0>(slot(s), scales(s / kSpan), slot(s + 1), scales(s / kSpan + 1), s, one, two, &far, acc);
-    multiply<EXACT>(two, kParts - 1, &far, acc);
+    if constexpr (kAhead) products<EXACT>(two, kParts - 1, &far, acc);
     settle();
     return far;
   }
@@ -613,7 +633,7 @@ namespace {
 
 // How a product of more than 64 rows is cut, and where its workspace lies.
 struct Plan {
-  bool big;      // tiles of 256 columns, else 128
+  bool big;      // tiles of 256 columns, else of 128
   int shares;    // of K
   size_t rows, scales_a, scales_w, parts, bytes;
 };
@@ -631,11 +651,25 @@ Plan plan(const GemmMxArgs& a) {
     if (a.as) p.scales_a = take(a.m * pitch);
     p.scales_w = take(a.n * pitch);
   }
-  auto tiles = [&](int rm, int rn) { return (size_t)((a.m + rm - 1) / rm) * ((a.n + rn - 1) / rn); };
-  p.big = a.as ? tiles(256, 256) >= 192 : tiles(128, 256) >= 192;
-  p.shares = 1;
-  const size_t t = p.big ? 1000 : tiles(128, 128);
-  while (p.shares < 16 && t * p.shares * 2 <= 384 && pitch / 16 / (p.shares * 2) >= 2) p.shares *= 2;
+  // The expected time of each tile and number of shares: rounds of workgroups
+  // over the chip, each its stages and a start, and the joining of the shares
+  // at 4 bytes a sum and share.  Measured stages: f16 rows 1.9 us (128 x 256,
+  // a workgroup a CU) and 1.3 us (128 x 128); MXFP4 rows 2.7 us (256 x 256),
+  // and 128 x 128 1.7 us for two workgroups a CU, 1.1 us for one.
+  const int depth = a.as ? 256 : 128, spans = (a.k + 511) / 512;
+  double best = 1e30;
+  for (int big = 0; big < 2; ++big) {
+    const int rows = a.as && big ? 256 : 128, cols = big ? 256 : 128, slots = a.as && !big ? 512 : 256;
+    const size_t tiles = (size_t)((a.m + rows - 1) / rows) * ((a.n + cols - 1) / cols);
+    for (int shares = 1; shares <= 16 && shares <= spans; shares *= 2) {
+      const double rounds = (double)((tiles * shares + slots - 1) / slots);
+      const double two = std::min(std::max(tiles * shares / 256.0 - 1.0, 0.0), 1.0);  // share of CUs that have two
+      const double stage = a.as ? (big ? 2.7 : 1.1 + 0.6 * two) : (big ? 1.9 : 1.3);
+      double t = rounds * (3.0 + stage * ((spans + shares - 1) / shares * (512 / depth)));
+      if (shares > 1) t += 2.0 + (double)a.m * a.n * 4 * (2 * shares + 1) / 8e6;
+      if (t < best) best = t, p.big = big, p.shares = shares;
+    }
+  }
   if (p.shares > 1) p.parts = take((size_t)p.shares * a.m * ((a.n + 3) / 4 * 4) * 4);
   return p;
 }
@@ -685,9 +719,9 @@ void launch_gemm_mx(hipStream_t st, GemmMxArgs a, void* space) {
   a.parts = (float*)(base + p.parts);
   a.ldp = (a.n + 3) / 4 * 4;
   if (a.as)
-    p.big ? launch_tiles<true, 2, 2, 8, 8>(st, a, 1) : launch_tiles<true, 2, 2, 4, 4>(st, a, p.shares);
+    p.big ? launch_tiles<true, 2, 4, 8, 4>(st, a, p.shares) : launch_tiles<true, 2, 2, 4, 4>(st, a, p.shares);
   else
-    p.big ? launch_tiles<false, 2, 2, 4, 8>(st, a, 1) : launch_tiles<false, 2, 2, 4, 4>(st, a, p.shares);
+    p.big ? launch_tiles<false, 2, 4, 4, 4>(st, a, p.shares) : launch_tiles<false, 2, 2, 4, 4>(st, a, p.shares);
   if (p.shares > 1)
     hipLaunchKernelGGL(gemm_mx_join_kernel, dim3((unsigned)((a.n + 1023) / 1024), (unsigned)std::min(a.m, 65535)),
                        dim3(256), 0, st, a, p.shares);
