@@ -62,7 +62,7 @@ __device__ __forceinline__ void store4(const GemmMxArgs& a, size_t row, int n, f
     }
 }
 
-constexpr int kFewRows = 64;
+constexpr int kFewRows = 32;
 
 // --- a few rows -----------------------------------------------------------------
 
@@ -136,101 +136,141 @@ __device__ __forceinline__ f32x4 times_exact(uint32_t w, float s, f16x8 x, f32x4
 // Bound by the weights' bytes: 17/32 of one an element, read once.  A lane's
 // operand is a whole block, four lanes side by side read 64 bytes of a row,
 // and four steps' loads are in flight at a time; each workgroup reads the
-// rows of A again from L2, which NT divides.
-template <bool MX, int MT, int NT, bool EXACT>
-__device__ __forceinline__ bool rows_sum(const GemmMxArgs& a, int n0, int from, int to, f32x4 (&acc)[NT][MT]) {
-  const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
-  const int blocks = (a.k + 31) / 32;
+// rows of A again from L2, which NT divides.  One f16 row x 14336 x 4096:
+// 10.3 us (3.0 TB/s); 16 MXFP4 rows x 8192 x 8192: 10.1 us (3.6 TB/s).
+// FEW: f16 rows, at most four, that a wave brings to LDS whole, an element
+// once: the matrix instruction's operand has 16 columns, and as loads of its
+// own each would cost 64 bytes a lane and step.
+template <bool MX, int MT, int NT, bool FEW>
+struct Rows {
+  const GemmMxArgs& g;
   const uint8_t *w[NT], *ws[NT], *x[MT], *xs[MT];
-  bool there[MT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const size_t n = min(n0 + t * 16 + col, a.n - 1);  // rows behind the end are not stored
-    w[t] = a.w + n * blocks * 16;
-    ws[t] = a.ws + n * blocks;
-#pragma unroll
-    for (int u = 0; u < MT; ++u) acc[t][u] = f32x4{};
-  }
-#pragma unroll
-  for (int u = 0; u < MT; ++u) {
-    there[u] = u * 16 + col < a.m;
-    const size_t m = there[u] ? u * 16 + col : 0;
-    x[u] = (const uint8_t*)a.a + (MX ? m * blocks * 16 : m * a.lda * 2);
-    xs[u] = MX ? a.as + m * blocks : nullptr;
-  }
-  const uint32_t turn = 8 * quad + 9;  // a rotation by this takes byte `quad` to bits 30:23
-  uint32_t odd = 0;                    // a factor that f16 does not hold
-  for (int s0 = from; s0 < to; s0 += 4) {
-    uint4 wv[NT][4], sw[NT], sx[MT];
+  int lane, col, quad, blocks;
+  uint8_t* few;  // this wave's rows in LDS
+  static constexpr int kFewLine = 1024 + 16;
+  __device__ __forceinline__ Rows(const GemmMxArgs& args, int n0, uint8_t* lds) : g(args), few(lds) {
+    lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4, blocks = (g.k + 31) / 32;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      sw[t] = scales16(ws[t], s0 * 4, blocks);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int b = (s0 + i) * 4 + quad;
-        wv[t][i] = b < blocks && s0 + i < to ? *(const uint4*)(w[t] + (size_t)b * 16) : make_uint4(0, 0, 0, 0);
-      }
+      const size_t n = min(n0 + t * 16 + col, g.n - 1);  // rows behind the end are not stored, on both sides
+      w[t] = g.w + (n * blocks + quad) * 16;
+      ws[t] = g.ws + n * blocks;
     }
-    if constexpr (MX) {
 #pragma unroll
-      for (int u = 0; u < MT; ++u) sx[u] = scales16(xs[u], s0 * 4, blocks);
+    for (int u = 0; u < MT; ++u) {
+      const size_t m = min(u * 16 + col, g.m - 1);
+      x[u] = (const uint8_t*)g.a + (MX ? (m * blocks + quad) * 16 : (m * g.lda + quad * 32) * 2);
+      xs[u] = MX ? g.as + m * blocks : nullptr;
+    }
+  }
+  // Four steps from s0; ALL: none of them reaches behind the end of K.
+  template <bool EXACT, bool ALL>
+  __device__ __forceinline__ void four(int s0, int to, uint32_t* odd, f32x4 (&acc)[NT][MT]) const {
+    uint4 wv[NT][4], sw[NT], sx[MT], xv[MT][MX ? 4 : 16];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        wv[t][i] = ALL || (s0 + i < to && (s0 + i) * 4 + quad < blocks) ? *(const uint4*)(w[t] + (size_t)(s0 + i) * 64)
+                                                                        : make_uint4(0, 0, 0, 0);
+      if constexpr (ALL)
+        __builtin_memcpy(&sw[t], ws[t] + s0 * 4, 16);
+      else
+        sw[t] = scales16(ws[t], s0 * 4, blocks);
+    }
+#pragma unroll
+    for (int u = 0; u < MT; ++u) {
+      if constexpr (MX) {
+        if constexpr (ALL)
+          __builtin_memcpy(&sx[u], xs[u] + s0 * 4, 16);
+        else
+          sx[u] = scales16(xs[u], s0 * 4, blocks);
+      }
+      if constexpr (FEW) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (r >= g.m) break;
+          const int k = s0 * 128 + lane * 8;
+          const uint4 v = ALL || (k < g.lda && s0 + lane / 16 < to)
+                              ? *(const uint4*)((const uint8_t*)g.a + ((size_t)r * g.lda + k) * 2)
+                              : make_uint4(0, 0, 0, 0);
+          *(uint4*)(few + r * kFewLine + lane * 16) = v;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const uint8_t* p = few + min(col, g.m - 1) * kFewLine + quad * 64;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) xv[u][i] = *(const uint4*)(p + i / 4 * 256 + i % 4 * 16);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        continue;
+      }
+#pragma unroll
+      for (int i = 0; i < (MX ? 4 : 16); ++i) {
+        if constexpr (MX)
+          xv[u][i] = ALL || (s0 + i < to && (s0 + i) * 4 + quad < blocks) ? *(const uint4*)(x[u] + (size_t)(s0 + i) * 64)
+                                                                          : make_uint4(0, 0, 0, 0);
+        else
+          xv[u][i] = ALL || (s0 + i / 4 < to && ((s0 + i / 4) * 4 + quad) * 32 + i % 4 * 8 < g.lda)
+                         ? *(const uint4*)(x[u] + (size_t)(s0 + i / 4) * 256 + i % 4 * 16)
+                         : make_uint4(0, 0, 0, 0);
+      }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (s0 + i >= to) break;
-      const int b = (s0 + i) * 4 + quad;
-      uint32_t fw[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const uint32_t v = word(sw[t], i);
         if constexpr (MX) {
-          fw[t] = v >> (8 * quad);
+          const i32x8 p = {(int)wv[t][i].x, (int)wv[t][i].y, (int)wv[t][i].z, (int)wv[t][i].w, 0, 0, 0, 0};
+#pragma unroll
+          for (int u = 0; u < MT; ++u) {
+            const i32x8 q = {(int)xv[u][i].x, (int)xv[u][i].y, (int)xv[u][i].z, (int)xv[u][i].w, 0, 0, 0, 0};
+            acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(p, q, acc[t][u], 4, 4, 0, (int)(v >> (8 * quad)),
+                                                                        0, (int)(word(sx[u], i) >> (8 * quad)));
+          }
         } else {
-          fw[t] = __builtin_amdgcn_alignbit(v, v, turn);
+          const uint32_t fb = __builtin_amdgcn_alignbit(v, v, 8 * quad + 9);  // byte `quad` to bits 30:23
+          const float f = __builtin_bit_cast(float, fb);
           if constexpr (!EXACT) {
             const uint4 q = wv[t][i];
-            const bool some = ((q.x | q.y | q.z | q.w) & 0x77777777u) != 0;
-            const bool out = (fw[t] & 0x7F800000u) - (104u << 23) > (36u << 23);
-            odd |= (uint32_t)((out && some) || (fw[t] & 0x7F800000u) == 0x7F800000u);
+            const uint32_t some = (q.x | q.y | q.z | q.w) & 0x77777777u;
+            *odd |= (fb & 0x7F800000u) - (104u << 23) > (36u << 23) ? some : 0u;
           }
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < MT; ++u) {
-        if constexpr (MX) {
-          const bool in = there[u] && b < blocks;
-          const uint4 v = in ? *(const uint4*)(x[u] + (size_t)b * 16) : make_uint4(0, 0, 0, 0);
-          const uint32_t fx = in ? word(sx[u], i) >> (8 * quad) : 127u;
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            const i32x8 p = {(int)wv[t][i].x, (int)wv[t][i].y, (int)wv[t][i].z, (int)wv[t][i].w, 0, 0, 0, 0};
-            const i32x8 q = {(int)v.x, (int)v.y, (int)v.z, (int)v.w, 0, 0, 0, 0};
-            acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(p, q, acc[t][u], 4, 4, 0, (int)fw[t], 0,
-                                                                        (int)fx);
-          }
-        } else {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int k = b * 32 + j * 8;
-            const f16x8 v = there[u] && k < a.lda ? *(const f16x8*)(x[u] + (size_t)k * 2) : f16x8{};
+            if constexpr (EXACT) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              const float f = __builtin_bit_cast(float, fw[t]);
-              if constexpr (EXACT)
-                acc[t][u] = times_exact(word(wv[t][i], j), f, v, acc[t][u]);
-              else
-                acc[t][u] =
-                    __builtin_amdgcn_mfma_f32_16x16x32_f16(eight_f16(word(wv[t][i], j), f), v, acc[t][u], 0, 0, 0);
+              for (int u = 0; u < MT; ++u)
+                acc[t][u] = times_exact(word(wv[t][i], j), f, __builtin_bit_cast(f16x8, xv[u][i * 4 + j]), acc[t][u]);
+            } else {
+              const f16x8 e = eight_f16(word(wv[t][i], j), f);
+#pragma unroll
+              for (int u = 0; u < MT; ++u)
+                acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(e, __builtin_bit_cast(f16x8, xv[u][i * 4 + j]),
+                                                                  acc[t][u], 0, 0, 0);
             }
           }
         }
       }
     }
   }
-  return odd != 0;
-}
+  template <bool EXACT>
+  __device__ __forceinline__ uint32_t sum(int from, int to, f32x4 (&acc)[NT][MT]) const {
+    uint32_t odd = 0;  // a factor that f16 does not hold
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int u = 0; u < MT; ++u) acc[t][u] = f32x4{};
+    const int whole = min(to, MX ? blocks / 4 : g.lda / 128);
+    int s = from;
+    for (; s + 4 <= whole; s += 4) four<EXACT, true>(s, to, &odd, acc);
+    for (; s < to; s += 4) four<EXACT, false>(s, to, &odd, acc);
+    return odd;
+  }
+};
 
-template <bool MX, int MT, int NT>
+template <bool MX, int MT, int NT, bool FEW>
 __global__ __launch_bounds__(MT* NT == 1 ? 1024 : 512) void gemm_mx_rows_kernel(GemmMxArgs a) {
   extern __shared__ __align__(16) f32x4 sums[];  // [waves][NT * MT][64]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
@@ -239,10 +279,12 @@ __global__ __launch_bounds__(MT* NT == 1 ? 1024 : 512) void gemm_mx_rows_kernel(
   // the waves' shares are whole groups of four steps
   const int groups = (steps + 3) / 4;
   const int from = groups * wave / waves * 4, to = min(steps, groups * (wave + 1) / waves * 4);
-  const bool odd = rows_sum<MX, MT, NT, false>(a, n0, from, to, acc);
+  const Rows<MX, MT, NT, FEW> r(a, n0, (uint8_t*)sums + wave * 4 * Rows<MX, MT, NT, FEW>::kFewLine);
+  const uint32_t odd = r.template sum<false>(from, to, acc);
   if constexpr (!MX)
-    if (__ballot(odd)) rows_sum<MX, MT, NT, true>(a, n0, from, to, acc);
+    if (__ballot(odd != 0)) r.template sum<true>(from, to, acc);
   if (waves > 1) {
+    if (FEW) __syncthreads();  // the rows' place becomes the sums'
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -282,23 +324,30 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const uint16_t* __restric
   }
 }
 
-template <bool MX, int MT, int NT>
+template <bool MX, int MT, int NT, bool FEW = false>
 void launch_rows(hipStream_t st, const GemmMxArgs& a) {
   const int tiles = (a.n + 16 * NT - 1) / (16 * NT), groups = ((a.k + 31) / 32 + 15) / 16;
   int waves = 1;
-  while (waves < (MT * NT == 1 ? 16 : 8) && waves * 2 * NT * MT <= 64 && waves < groups && tiles * waves < 4096) waves *= 2;
-  const size_t lds = waves > 1 ? (size_t)waves * NT * MT * 1024 : 0;
-  hipLaunchKernelGGL((gemm_mx_rows_kernel<MX, MT, NT>), dim3((unsigned)tiles), dim3(64u * waves), lds, st, a);
+  while (waves < (MT * NT == 1 ? 16 : 8) && waves < groups && tiles * waves < 4096) waves *= 2;
+  size_t lds = waves > 1 ? (size_t)waves * NT * MT * 1024 : 0;
+  if (FEW) lds = std::max(lds, (size_t)waves * 4 * Rows<MX, MT, NT, FEW>::kFewLine);
+  hipLaunchKernelGGL((gemm_mx_rows_kernel<MX, MT, NT, FEW>), dim3((unsigned)tiles), dim3(64u * waves), lds, st, a);
 }
 
-template <bool MX>
+// Two tiles of 16 weight rows a wave halve what is read of A, where enough
+// waves are left (16 f16 rows x 5120 x 5120: 10.9 us, 15.8 us with one tile;
+// x 4096 x 14336: 22.6 us, 19.7 us with one).  Up to four f16 rows come
+// through LDS (one row x 4096 x 14336: 8.8 us, 9.9 us without).
 void rows(hipStream_t st, const GemmMxArgs& a) {
-  if (a.m <= 16)
-    launch_rows<MX, 1, 1>(st, a);
-  else if (a.m <= 32)
-    launch_rows<MX, 2, 2>(st, a);
+  const bool wide = a.n >= 5120;
+  if (a.m > 16)
+    a.as ? launch_rows<true, 2, 2>(st, a) : launch_rows<false, 2, 2>(st, a);
+  else if (a.as)
+    wide ? launch_rows<true, 1, 2>(st, a) : launch_rows<true, 1, 1>(st, a);
+  else if (a.m <= 4)
+    launch_rows<false, 1, 1, true>(st, a);
   else
-    launch_rows<MX, 4, 2>(st, a);
+    wide ? launch_rows<false, 1, 2>(st, a) : launch_rows<false, 1, 1>(st, a);
 }
 
 // --- many rows --------------------------------------------------------------------
@@ -700,7 +749,7 @@ void launch_gemm_mx(hipStream_t st, GemmMxArgs a, void* space) {
     a.a = y;
   }
   if (a.m <= kFewRows) {
-    a.as ? rows<true>(st, a) : rows<false>(st, a);
+    rows(st, a);
     DW_HIP(hipGetLastError());
     return;
   }
