@@ -1439,6 +1439,8 @@ int dw_hip_attention_mxfp4(dw_hip_backend* be, const dw_hip_buffer* q, size_t q_
   check_kv(tokens, batch, kv_heads, head_dim, page_size, num_pages, max_pages, "attention_mxfp4");
   if (!heads || heads % kv_heads) dw::fail(DW_ERR_INVALID, "attention_mxfp4: heads must be a multiple of kv_heads");
   if (heads > 4096) dw::fail(DW_ERR_UNSUPPORTED, "attention_mxfp4: more than 4096 heads");
+  if (tokens * heads > kMostMx || batch * heads > kMostMx / 4)
+    dw::fail(DW_ERR_UNSUPPORTED, "attention_mxfp4: more than 2^24 rows, or 2^22 heads of all sequences");
   if (!std::isfinite(scale)) dw::fail(DW_ERR_INVALID, "attention_mxfp4: scale must be finite");
   if (causal != 0 && causal != 1) dw::fail(DW_ERR_INVALID, "attention_mxfp4: causal must be 0 or 1");
   if (window && !causal) dw::fail(DW_ERR_UNSUPPORTED, "attention_mxfp4: a window needs causal attention");
@@ -1463,8 +1465,8 @@ int dw_hip_attention_mxfp4(dw_hip_backend* be, const dw_hip_buffer* q, size_t q_
   g.scale = fabsf(scale) * 1.44269504f;
   g.negate = scale < 0;
   dw::SplitArgs p{};
-  void* space = b->workspace(Backend::WS_ATTN, dw::attention_space(a, g, &p));
-  dw::launch_attention(b->stream, a, g, p, space);
+  const size_t bytes = dw::attention_space(a, g, &p);
+  dw::launch_attention(b->stream, a, g, p, bytes ? b->workspace(Backend::WS_ATTN, bytes) : nullptr);
   API_END
 }
 

@@ -500,9 +500,11 @@ struct AttnArgs {
   long long window;
   float scale;  // |scale| log2(e): p = 2^(scale (s - max))
 };
-// How single tokens' attention is split over keys, and what the splits leave:
-// set by attention_space, which gives the bytes of workspace.
+// How attention is cut: whole tiles of many rows, or few rows split over keys
+// and what the splits leave.  Set by attention_space, which gives the bytes of
+// workspace.
 struct SplitArgs {
+  bool whole;
   int group, head_tiles;   // heads of a kv head, tiles of 16 of them
   int tile_tokens, rows;   // new tokens of a tile, its rows (16 at most)
   int waves, least;        // splits wanted, a split's fewest steps of 64 keys

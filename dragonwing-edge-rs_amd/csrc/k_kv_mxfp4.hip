@@ -5,6 +5,7 @@
 // bytes and [page][head][slot][d / 32] scales: the rows are MXFP4 rows of d
 // elements (mxfp4.h), so the cache's values can be read back as such rows.
 #include <algorithm>
+#include <type_traits>
 
 #include "dw_common.h"
 #include "mxfp4.h"
@@ -485,6 +486,258 @@ __global__ __launch_bounds__(J) void attention_join_kernel(KvArgs a, AttnArgs g,
   *(ushort4*)(g.y + ((size_t)(t + within) * g.heads + head) * D + tid * 4) = h;
 }
 
+// --- many new tokens ---------------------------------------------------------------
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// A tile of up to 128 rows (new tokens of a sequence x heads of a kv head) over
+// all of its keys, 32 rows a wave.
+//
+// KT keys a step: a thread widens a quarter of a key's and of a value's row to
+// f16 (their packed form was loaded a step before) and writes it to LDS, where
+// the four waves read it: the conversion, not the bytes, would bound the
+// kernel if each wave made its own.  S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16 matrix instructions:
+// the first's result leaves a lane keys of one row that are the second's B
+// operand as they stand, if V^T takes the keys in that order, which
+// transposing reads of LDS give it.  Two workgroups fit a CU up to d = 128, so
+// that one's exponentials run beside the other's products.  4,096 causal tokens
+// of 32 heads over 8 kv heads, d = 128: 193 us, 710 TFLOP/s (466 us as a wave
+// for each 16 rows); the exponentials and conversions take as long as the
+// products there.
+template <int D>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(KvArgs a, AttnArgs g, int tile_tokens, int tiles_most) {
+  constexpr int KT = D == 256 ? 32 : 64;
+  constexpr int kKeyRow = D * 2 + 16, kValueRow = D * 2 + 32;  // bytes: no bank twice for the lanes of a read
+  constexpr int kBuffer = KT * (kKeyRow + kValueRow);
+  extern __shared__ __align__(16) uint8_t lds[];
+  __shared__ uint32_t nan_lds[2][KT];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row = lane & 31, half = lane >> 5;
+  const int group = g.heads / a.kv_heads, kv_head = blockIdx.x % a.kv_heads;
+  // the tiles with the most keys, a sequence's last, go first
+  int tile = tiles_most - 1 - blockIdx.x / a.kv_heads;
+  int seq = -1, start = 0, count = 0;
+  for (int b0 = 0, before = 0; b0 < a.batch; b0 += 64) {
+    const int b = b0 + lane;
+    int t0 = 0, n = 0;
+    if (b < a.batch) {
+      t0 = max(a.start[b], 0);
+      n = max(min(a.start[b + 1], a.tokens) - t0, 0);
+    }
+    const int tiles = (n + tile_tokens - 1) / tile_tokens;
+    int upto = tiles;
+    for (int i = 1; i < 64; i *= 2) {
+      const int v = __shfl_up(upto, i);
+      if (lane >= i) upto += v;
+    }
+    const unsigned long long hit = __ballot(tile >= before + upto - tiles && tile < before + upto);
+    if (hit) {
+      const int src = __ffsll(hit) - 1;
+      seq = b0 + src;
+      tile = __builtin_amdgcn_readfirstlane(tile - before - __shfl(upto - tiles, src));
+      start = __builtin_amdgcn_readfirstlane(__shfl(t0, src));
+      count = __builtin_amdgcn_readfirstlane(__shfl(n, src));
+      break;
+    }
+    before += __shfl(upto, 63);
+  }
+  if (seq < 0) return;
+  const long long table_keys = (long long)a.max_pages << a.page_shift;
+  const long long raw = a.len[seq], len = min(max(raw, 0ll), table_keys);
+  const int skip = tile * tile_tokens, mine = min(count - skip, tile_tokens);
+  const long long pos0 = raw - count + skip, pos1 = pos0 + mine - 1;
+  // this lane's row
+  const int r = wave * 32 + row, within = r / group, head = kv_head * group + r - within * group;
+  const bool real = within < mine;
+  const int token = start + skip + within;
+  const long long pos = pos0 + within;
+  const int hi = !real ? 0 : (int)(g.causal ? max(0ll, min(len, pos + 1)) : len);
+  const int lo = !real || g.window <= 0 ? 0 : (int)max(0ll, pos - g.window + 1);
+  const int most = (int)(g.causal ? max(0ll, min(len, pos1 + 1)) : len);  // keys that some row sees: [from, most)
+  const int from = g.window > 0 ? (int)min((long long)most, max(0ll, pos0 - g.window + 1)) : 0;
+  const int every = (int)(g.causal ? max(0ll, min(len, pos0 + 1)) : len);  // that all rows see, up to here
+  const int all_from = g.window > 0 ? (int)max(0ll, pos1 - g.window + 1) : 0;
+  f16x8 q[D / 16];
+  {
+    const uint16_t* src = g.q + (size_t)(real ? token : start) * g.q_stride + g.q_off + (size_t)head * D + half * 8;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      q[i] = f16x8{};
+      if (real) {
+        const Loose<uint16_t, 8> v = load_loose<uint16_t, 8>(src + i * 16);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          q[i][e] = __builtin_bit_cast(_Float16, (uint16_t)(g.negate ? v.v[e] ^ 0x8000u : v.v[e]));
+      }
+    }
+  }
+  f32x16 o[D / 32] = {};
+  float m = -INFINITY, l = 0.0f;
+  uint32_t nan_blocks = 0;
+  const int j0 = from & ~15, steps = (most - j0 + KT - 1) / KT;
+  const int32_t* table = a.table + (size_t)seq * a.max_pages;
+  const int mask = (1 << a.page_shift) - 1;
+  // the page of key `lane` of a step, or -1
+  auto page_of = [&](int step) {
+    const long long j = (long long)j0 + (long long)step * KT + lane;
+    const int page = lane < KT && j < most ? table[j >> a.page_shift] : -1;
+    return page < a.num_pages ? page : -1;
+  };
+  // this thread's part of the widening: a quarter of one key's row
+  const bool does_k = KT == 64 || wave < 2, does_v = KT == 64 || wave >= 2;
+  const int key = (tid >> 2) % KT, quarter = tid & 3;
+  Piece<D> k, v;
+  auto fetch = [&](int step, int pages) {
+    const int j = j0 + step * KT + key;
+    const int page = max(__shfl(pages, key), 0);  // a key on no page is seen by no row: any row's bytes will do
+    const size_t at = (((size_t)page * a.kv_heads + kv_head) << a.page_shift) + (j & mask);
+    if (does_k) k.load(a.kc, a.ks, at, quarter);
+    if (does_v) v.load(a.vc, a.vs, at, quarter);
+  };
+  auto whole = [&](int step, unsigned long long there) {
+    const int j = j0 + step * KT;
+    return there == ~0ull >> (64 - KT) && j + KT <= every && j >= all_from;
+  };
+  auto widen_to = [&](int step, unsigned long long there) {
+    uint8_t* kb = lds + (step & 1) * kBuffer + key * kKeyRow + quarter * (D / 2);
+    uint8_t* vb = lds + (step & 1) * kBuffer + KT * kKeyRow + key * kValueRow + quarter * (D / 2);
+    if (does_k) {
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) *(f16x8*)(kb + i * 16) = k.eight(i);
+    }
+    if (does_v) {
+      if (!whole(step, there)) {
+        // values that no row sees must not reach the sums, whatever they hold,
+        // nor those that only some see, if they are NaN
+        const int j = j0 + step * KT + key;
+        if (!(there >> key & 1) || j >= most || j < from) v.clear();
+        const uint32_t own = v.nan_bits(quarter);
+        uint32_t bits = own | __shfl_xor(own, 1);
+        bits |= __shfl_xor(bits, 2);
+        if (own) v.clear_nan();
+        if (quarter == 0) nan_lds[step & 1][key] = bits;
+      }
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) *(f16x8*)(vb + i * 16) = v.eight(i);
+    }
+  };
+  unsigned long long there = 0, there_next = 0;
+  if (steps > 0) {
+    int pages = page_of(0);
+    there = __ballot(pages >= 0);
+    fetch(0, pages);
+    widen_to(0, there);
+    if (steps > 1) {
+      pages = page_of(1);
+      there_next = __ballot(pages >= 0);
+      fetch(1, pages);
+    }
+  }
+  int pages = steps > 2 ? page_of(2) : -1;
+  __syncthreads();
+  for (int step = 0; step < steps; ++step) {
+    unsigned long long there_after = 0;
+    if (step + 1 < steps) {
+      widen_to(step + 1, there_next);
+      if (step + 2 < steps) {
+        there_after = __ballot(pages >= 0);
+        fetch(step + 2, pages);
+        if (step + 3 < steps) pages = page_of(step + 3);
+      }
+    }
+    const uint8_t* kb = lds + (step & 1) * kBuffer;
+    const uint8_t* vb = kb + KT * kKeyRow;
+    f32x16 t[KT / 32];
+#pragma unroll
+    for (int u = 0; u < KT / 32; ++u) {
+      t[u] = f32x16{};
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const f16x8 x = *(const f16x8*)(kb + (u * 32 + row) * kKeyRow + i * 32 + half * 16);
+        t[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q[i], t[u], 0, 0, 0);
+      }
+    }
+    uint32_t see = ~0u;
+    if (!whole(step, there)) {
+      see = 0;
+#pragma unroll
+      for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int c = u * 32 + 8 * (e / 4) + 4 * half + e % 4, j = j0 + step * KT + c;
+          const bool yes = (there >> c & 1) && j < hi && j >= lo;
+          see |= (uint32_t)yes << (u * 16 + e);
+          t[u][e] = yes ? t[u][e] : -INFINITY;
+        }
+      const uint32_t any = lane < KT ? nan_lds[step & 1][lane] : 0u;
+      if (__ballot(any != 0)) {
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (see >> (u * 16 + e) & 1) nan_blocks |= nan_lds[step & 1][u * 32 + 8 * (e / 4) + 4 * half + e % 4];
+      }
+    }
+    float top = t[0][0];
+#pragma unroll
+    for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, t[u][e]);
+    if (__ballot(m == -INFINITY ? top > m : (top - m) * g.scale > 8.0f)) {
+      const float now = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
+      const float f = now == m ? 1.0f : m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - now) * g.scale);
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) o[i] *= f;
+      m = now;
+    }
+    const float ref = m == -INFINITY ? 0.0f : m * g.scale;
+    f16x8 p[KT / 16];
+#pragma unroll
+    for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float x = __builtin_amdgcn_exp2f(fmaf(t[u][e], g.scale, -ref));
+        x = see >> (u * 16 + e) & 1 ? x : 0.0f;
+        l += x;
+        p[u * 2 + e / 8][e % 8] = (_Float16)x;
+      }
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int u = 0; u < KT / 16; ++u) {
+        // four groups of 16 lanes: 4 keys x 16 elements each
+        typedef __attribute__((address_space(3))) s16x4* Lds;
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        const int e = lane & 15;
+        const uint8_t* src = vb + (u * 16 + 4 * half + (e >> 2)) * kValueRow + i * 64 + ((lane >> 4) & 1) * 32 + (e & 3) * 8;
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)src);
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(src + 8 * kValueRow));
+        const s16x8 xy = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, xy), p[u], o[i], 0, 0, 0);
+      }
+    there = there_next;
+    there_next = there_after;
+    __syncthreads();
+  }
+  l += __shfl_xor(l, 32);
+  nan_blocks |= __shfl_xor(nan_blocks, 32);
+  if (!real) return;
+  uint16_t* y = g.y + ((size_t)token * g.heads + head) * D + half * 4;
+  const float f = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    const float scale = nan_blocks >> i & 1 ? NAN : f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      ushort4 h;
+      h.x = narrow<uint16_t>(o[i][e * 4] * scale), h.y = narrow<uint16_t>(o[i][e * 4 + 1] * scale);
+      h.z = narrow<uint16_t>(o[i][e * 4 + 2] * scale), h.w = narrow<uint16_t>(o[i][e * 4 + 3] * scale);
+      *(ushort4*)(y + i * 32 + e * 8) = h;
+    }
+  }
+}
+
 }  // namespace
 
 void launch_kv_append(hipStream_t st, const KvArgs& a, const void* k, size_t k_stride, size_t k_off, const void* v,
@@ -494,15 +747,49 @@ void launch_kv_append(hipStream_t st, const KvArgs& a, const void* k, size_t k_s
   DW_HIP(hipGetLastError());
 }
 
+namespace {
+
+template <int D>
+void launch_tiles(hipStream_t st, const KvArgs& a, const AttnArgs& g) {
+  constexpr int kKeys = D == 256 ? 32 : 64, kLds = 2 * kKeys * (D * 4 + 48);
+  const int tile_tokens = 128 / (g.heads / a.kv_heads), tiles = std::min(a.tokens, a.tokens / tile_tokens + a.batch);
+  static const hipError_t sized =
+      hipFuncSetAttribute((const void*)attention_tile_kernel<D>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  DW_HIP(sized);
+  hipLaunchKernelGGL(attention_tile_kernel<D>, dim3((unsigned)(tiles * a.kv_heads)), dim3(256), kLds, st, a, g,
+                     tile_tokens, tiles);
+}
+
+template <int D>
+void launch_splits(hipStream_t st, const KvArgs& a, const AttnArgs& g, const SplitArgs& p) {
+  // Rows of few splits are many: a wave each then.
+  const dim3 rows((unsigned)a.tokens, (unsigned)(a.kv_heads * p.head_tiles), (unsigned)p.rows);
+  const bool few = (long long)a.tokens * g.heads <= 1024;
+  hipLaunchKernelGGL(attention_split_kernel<D>, dim3((unsigned)p.splits), dim3(64), 0, st, a, g, p);
+  if (few)
+    hipLaunchKernelGGL((attention_join_kernel<D, 512>), rows, dim3(512), 0, st, a, g, p);
+  else
+    hipLaunchKernelGGL((attention_join_kernel<D, 64>), rows, dim3(64), 0, st, a, g, p);
+}
+
+}  // namespace
+
 size_t attention_space(const KvArgs& a, const AttnArgs& g, SplitArgs* p) {
   p->group = g.heads / a.kv_heads;
+  // Whole tiles are faster where there are enough of them, and full: 512 new
+  // tokens of 32 heads 24 us, 53 us split; 256 of them after 8,192 keys (64
+  // tiles, 8,192 rows) 250 us, 110 us split; 8 sequences of up to 64 after
+  // 2,048 keys 68 us, 31 us split.
+  p->whole = p->group <= 128 && (long long)a.tokens * g.heads >= 12288 &&
+             (long long)a.tokens * p->group >= 128ll * a.batch;
+  if (p->whole) return 0;
   p->head_tiles = (p->group + 15) / 16;
   p->tile_tokens = std::max(1, 16 / p->group);
   const long long tiles = std::min<long long>(a.tokens, a.tokens / p->tile_tokens + (long long)a.batch);
   const long long heads = (long long)a.kv_heads * p->head_tiles;
   p->waves = 2048;
   p->least = 2;
-  p->splits = (int)std::min<long long>(tiles * heads + p->waves, 1ll << 25);
+  p->splits = (int)(tiles * heads + p->waves);
   p->rows = std::min(16, p->group * p->tile_tokens);
   p->stats_at = (size_t)p->splits * p->rows * a.d * 4;
   p->items_at = p->stats_at + (size_t)p->splits * p->rows * 8;
@@ -510,23 +797,21 @@ size_t attention_space(const KvArgs& a, const AttnArgs& g, SplitArgs* p) {
 }
 
 void launch_attention(hipStream_t st, const KvArgs& a, const AttnArgs& g, SplitArgs p, void* space) {
-  p.sums = (float*)space;
-  p.stats = (float2*)((char*)space + p.stats_at);
-  p.items = (int2*)((char*)space + p.items_at);
-  // Rows of few splits are many: a wave each then (64 sequences of up to 512
-  // keys, 8 kv heads: see the figures below).
-  const dim3 rows((unsigned)a.tokens, (unsigned)(a.kv_heads * p.head_tiles), (unsigned)p.rows);
-  const bool few = (long long)a.tokens * g.heads <= 1024;
-  auto go = [&](auto* split, auto* wide, auto* wave) {
-    hipLaunchKernelGGL(split, dim3((unsigned)p.splits), dim3(64), 0, st, a, g, p);
-    hipLaunchKernelGGL(few ? wide : wave, rows, dim3(few ? 512 : 64), 0, st, a, g, p);
+  auto run = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    p.whole ? launch_tiles<D>(st, a, g) : launch_splits<D>(st, a, g, p);
   };
+  if (!p.whole) {
+    p.sums = (float*)space;
+    p.stats = (float2*)((char*)space + p.stats_at);
+    p.items = (int2*)((char*)space + p.items_at);
+  }
   if (a.d == 64)
-    go(attention_split_kernel<64>, attention_join_kernel<64, 512>, attention_join_kernel<64, 64>);
+    run(std::integral_constant<int, 64>{});
   else if (a.d == 128)
-    go(attention_split_kernel<128>, attention_join_kernel<128, 512>, attention_join_kernel<128, 64>);
+    run(std::integral_constant<int, 128>{});
   else
-    go(attention_split_kernel<256>, attention_join_kernel<256, 512>, attention_join_kernel<256, 64>);
+    run(std::integral_constant<int, 256>{});
   DW_HIP(hipGetLastError());
 }
 
