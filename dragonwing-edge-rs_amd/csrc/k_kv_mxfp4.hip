@@ -81,8 +81,15 @@ struct Split {
   long long pos, len;     // position of the tile's first token, keys of the sequence
 };
 
-__device__ __forceinline__ unsigned long long sum_of_wave(unsigned long long v) {
-  for (int i = 1; i < 64; i *= 2) v += __shfl_xor(v, i);
+// Sums up to and with each lane, in the lanes' registers (six steps of data
+// parallel primitives; each shuffle through LDS would cost several times one).
+__device__ __forceinline__ int sums_upto(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // the lane one to the left in its row of 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);   // two
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);   // four
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);   // eight
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // the last of row 0 to row 1, of 2 to 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // the last of row 1 to rows 2 and 3
   return v;
 }
 
@@ -90,66 +97,59 @@ __device__ __forceinline__ unsigned long long sum_of_wave(unsigned long long v) 
 // the same number of steps; all steps over the waves wanted is a split's
 // length, so that long and short sequences share the waves evenly whatever
 // their lengths, which only the device knows.  One load a 64 sequences.
-__device__ __forceinline__ bool plan(const KvArgs& a, const AttnArgs& g, const SplitArgs& p, long long mine, Split* s) {
-  const int lane = threadIdx.x & 63;
-  const long long most = (long long)a.max_pages << a.page_shift;
-  auto of = [&](int b, int* first, int* tiles, int* steps, long long* len, long long* raw, int* count) {
-    *tiles = 0;
-    *steps = 1;
-    *len = *raw = 0;
-    *first = *count = 0;
+__device__ __forceinline__ bool plan(const KvArgs& a, const AttnArgs& g, const SplitArgs& p, int mine, Split* s) {
+  const int lane = threadIdx.x & 63, heads = p.head_tiles * a.kv_heads;
+  const int most = a.max_pages << a.page_shift;
+  int first, items, steps, count, len, raw;
+  auto of = [&](int b) {
+    first = count = items = len = raw = 0;
+    steps = 1;
     if (b >= a.batch) return;
-    const int t0 = max(a.start[b], 0), t1 = min(a.start[b + 1], a.tokens);
-    *raw = a.len[b];
-    *len = min(max(*raw, 0ll), most);
-    *first = t0;
-    *count = max(t1 - t0, 0);
-    *tiles = (*count + p.tile_tokens - 1) / p.tile_tokens;
-    long long span = *len;
-    if (g.window > 0) span = min(span, g.window + p.tile_tokens + 14);
-    *steps = (int)max(1ll, (span + kChunk - 1) / kChunk);
+    const int t0 = a.start[b], t1 = a.start[b + 1];
+    raw = a.len[b];
+    first = max(t0, 0);
+    count = max(min(t1, a.tokens) - first, 0);
+    len = min(max(raw, 0), most);
+    items = (count + p.tile_tokens - 1) / p.tile_tokens * heads;
+    const int span = g.window > 0 ? (int)min((long long)len, g.window + p.tile_tokens + 14) : len;
+    steps = max(1, (span + kChunk - 1) / kChunk);
   };
-  int first, tiles, steps, count;
-  long long len, raw;
-  unsigned long long all = 0;
+  // the total, in f32: it only has to be the same for all waves
+  float all = 0.0f;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    of(b0 + lane, &first, &tiles, &steps, &len, &raw, &count);
-    all += sum_of_wave((unsigned long long)tiles * p.head_tiles * a.kv_heads * steps);
+    of(b0 + lane);
+    float v = (float)items * (float)steps;
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) v += __shfl_xor(v, i);
+    all += v;
   }
-  const long long length = max((long long)p.least, (long long)((all + p.waves - 1) / p.waves));
-  long long before = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    if (a.batch > 64) of(b0 + lane, &first, &tiles, &steps, &len, &raw, &count);
-    const int n = (int)((steps + length - 1) / length);
-    const long long here = (long long)tiles * p.head_tiles * a.kv_heads * n;
-    long long upto = here;
-    for (int i = 1; i < 64; i *= 2) {
-      const long long v = __shfl_up(upto, i);
-      if (lane >= i) upto += v;
-    }
+  const int length = max(p.least, (int)fminf(ceilf(all / (float)p.waves), 1e9f));
+  int before = 0;
+  for (int b0 = 0; b0 < a.batch && before <= mine; b0 += 64) {
+    if (a.batch > 64) of(b0 + lane);
+    const int n = (steps - 1) / length + 1;
+    const int upto = sums_upto(items * n), here = items * n;
     const unsigned long long hit = __ballot(mine >= before + upto - here && mine < before + upto);
     if (hit) {
       const int src = __ffsll(hit) - 1;
-      const int at = (int)(mine - before - __shfl(upto - here, src));
-      s->of = __builtin_amdgcn_readfirstlane(__shfl(n, src));
-      const int item = __builtin_amdgcn_readfirstlane(at / s->of), heads = p.head_tiles * a.kv_heads;
-      s->index = __builtin_amdgcn_readfirstlane(at - item * s->of);
-      const int tile = item / heads, hh = item - tile * heads;
+      s->of = __builtin_amdgcn_readlane(n, src);
+      const int at = mine - before - __builtin_amdgcn_readlane(upto - here, src);
+      const int item = at / s->of, tile = item / heads, hh = item - tile * heads;
+      s->index = at - item * s->of;
       s->seq = b0 + src;
       s->kv_head = hh / p.head_tiles;
       s->head = s->kv_head * p.group + (hh - s->kv_head * p.head_tiles) * 16;
-      const int skip = tile * p.tile_tokens;
-      s->token = __builtin_amdgcn_readfirstlane(__shfl(first, src)) + skip;
-      const int whole = __builtin_amdgcn_readfirstlane(__shfl(count, src));
+      const int skip = tile * p.tile_tokens, whole = __builtin_amdgcn_readlane(count, src);
+      s->token = __builtin_amdgcn_readlane(first, src) + skip;
       s->count = min(whole - skip, p.tile_tokens);
-      s->len = __shfl(len, src);
+      s->len = __builtin_amdgcn_readlane(len, src);
       // the raw length places the tokens, whatever the table holds
-      s->pos = __shfl(raw, src) - whole + skip;
-      s->first = (int)(s->index * length);
-      s->chunks = (int)min(length, (long long)__builtin_amdgcn_readfirstlane(__shfl(steps, src)) - s->first);
+      s->pos = (long long)__builtin_amdgcn_readlane(raw, src) - whole + skip;
+      s->first = s->index * length;
+      s->chunks = min(length, __builtin_amdgcn_readlane(steps, src) - s->first);
       return true;
     }
-    before += __shfl(upto, 63);
+    before += __builtin_amdgcn_readlane(upto, 63);
   }
   return false;
 }
@@ -352,7 +352,8 @@ __global__ __launch_bounds__(64) void attention_split_kernel(KvArgs a, AttnArgs 
       for (int i = 0; i < D / 16; ++i) o[i] *= f;
       m = now;
     }
-    const float ref = m == -INFINITY ? 0.0f : m * g.scale;
+    // 2^6 times: a p of 2^-20 of the largest is still a normal f16 number
+    const float ref = (m == -INFINITY ? 0.0f : m * g.scale) - 6.0f;
     f16x8 pr[2];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -691,7 +692,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(K
       for (int i = 0; i < D / 32; ++i) o[i] *= f;
       m = now;
     }
-    const float ref = m == -INFINITY ? 0.0f : m * g.scale;
+    // 2^6 times: a p of 2^-20 of the largest is still a normal f16 number
+    const float ref = (m == -INFINITY ? 0.0f : m * g.scale) - 6.0f;
     f16x8 p[KT / 16];
 #pragma unroll
     for (int u = 0; u < KT / 32; ++u)
@@ -764,7 +766,7 @@ template <int D>
 void launch_splits(hipStream_t st, const KvArgs& a, const AttnArgs& g, const SplitArgs& p) {
   // Rows of few splits are many: a wave each then.
   const dim3 rows((unsigned)a.tokens, (unsigned)(a.kv_heads * p.head_tiles), (unsigned)p.rows);
-  const bool few = (long long)a.tokens * g.heads <= 1024;
+  const bool few = (long long)a.tokens * g.heads <= 512;
   hipLaunchKernelGGL(attention_split_kernel<D>, dim3((unsigned)p.splits), dim3(64), 0, st, a, g, p);
   if (few)
     hipLaunchKernelGGL((attention_join_kernel<D, 512>), rows, dim3(512), 0, st, a, g, p);
