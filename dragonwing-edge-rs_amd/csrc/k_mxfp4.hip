@@ -41,26 +41,28 @@ __global__ __launch_bounds__(256) void quantize_mxfp4_kernel(const T* __restrict
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void dequantize_mxfp4_kernel(const uint32_t* __restrict__ q,
+// E elements a thread: 16 bytes of y, so that a wave's stores are one piece.
+template <typename T, int E>
+__global__ __launch_bounds__(256) void dequantize_mxfp4_kernel(const uint8_t* __restrict__ q,
                                                                const uint8_t* __restrict__ scales,
                                                                T* __restrict__ y, size_t rows, size_t k) {
-  const size_t units = (k + 31) / 32 * 4;
+  const size_t blocks = (k + 31) / 32;
   const size_t u = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (u * 8 >= k) return;
+  if (u * E >= k) return;
   for (size_t r = (size_t)blockIdx.y * blockDim.y + threadIdx.y; r < rows; r += (size_t)gridDim.y * blockDim.y) {
+    const uint8_t* at = q + r * blocks * 16 + u * (E / 2);
     float v[8];
-    mx_decode8(q[r * units + u], mx_scale(scales[r * (units / 4) + u / 4]), v);
-    T* p = y + r * k + u * 8;
-    Loose<T, 8> l;
+    mx_decode8(E == 8 ? *(const uint32_t*)at : *(const uint16_t*)at, mx_scale(scales[r * blocks + u / (32 / E)]), v);
+    T* p = y + r * k + u * E;
+    Loose<T, E> l;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) l.v[i] = narrow<T>(v[i]);
-    if (u * 8 + 8 <= k) {
-      store_loose<T, 8>(p, l);
+    for (int i = 0; i < E; ++i) l.v[i] = narrow<T>(v[i]);
+    if (u * E + E <= k) {
+      store_loose<T, E>(p, l);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (u * 8 + i < k) p[i] = l.v[i];
+      for (int i = 0; i < E; ++i)
+        if (u * E + i < k) p[i] = l.v[i];
     }
   }
 }
@@ -69,13 +71,13 @@ struct Shape {
   size_t rows, k;
   dim3 grid, block;
 };
-Shape shape_of(size_t rows, size_t k) {
+Shape shape_of(size_t rows, size_t k, int each) {  // each: elements of a thread
   Shape s{rows, k, {}, {}};
-  if (k % 32 == 0 && rows * k <= (size_t)1 << 34) {  // a grid has under 2^32 threads
+  if (k % 32 == 0 && rows * k <= (size_t)1 << 33) {  // a grid has under 2^32 threads
     s.k = rows * k;
     s.rows = 1;
   }
-  const size_t units = (s.k + 31) / 32 * 4;
+  const size_t units = (s.k + 31) / 32 * (32 / each);
   unsigned tx = 4;
   while (tx < 256 && tx < units) tx *= 2;
   const unsigned ty = 256 / tx;
@@ -87,7 +89,7 @@ Shape shape_of(size_t rows, size_t k) {
 }  // namespace
 
 void launch_quantize_mxfp4(hipStream_t st, int dtype, const void* x, void* q, void* scales, size_t rows, size_t k) {
-  const Shape s = shape_of(rows, k);
+  const Shape s = shape_of(rows, k, 8);
   if (dtype == F16)
     hipLaunchKernelGGL(quantize_mxfp4_kernel<uint16_t>, s.grid, s.block, 0, st, (const uint16_t*)x, (uint32_t*)q,
                        (uint8_t*)scales, s.rows, s.k);
@@ -99,12 +101,12 @@ void launch_quantize_mxfp4(hipStream_t st, int dtype, const void* x, void* q, vo
 
 void launch_dequantize_mxfp4(hipStream_t st, int dtype, const void* q, const void* scales, void* y, size_t rows,
                              size_t k) {
-  const Shape s = shape_of(rows, k);
+  const Shape s = shape_of(rows, k, dtype == F16 ? 8 : 4);
   if (dtype == F16)
-    hipLaunchKernelGGL(dequantize_mxfp4_kernel<uint16_t>, s.grid, s.block, 0, st, (const uint32_t*)q,
+    hipLaunchKernelGGL((dequantize_mxfp4_kernel<uint16_t, 8>), s.grid, s.block, 0, st, (const uint8_t*)q,
                        (const uint8_t*)scales, (uint16_t*)y, s.rows, s.k);
   else
-    hipLaunchKernelGGL(dequantize_mxfp4_kernel<float>, s.grid, s.block, 0, st, (const uint32_t*)q,
+    hipLaunchKernelGGL((dequantize_mxfp4_kernel<float, 4>), s.grid, s.block, 0, st, (const uint8_t*)q,
                        (const uint8_t*)scales, (float*)y, s.rows, s.k);
   DW_HIP(hipGetLastError());
 }
