@@ -504,7 +504,7 @@ struct AttnArgs {
 // and what the splits leave.  Set by attention_space, which gives the bytes of
 // workspace.
 struct SplitArgs {
-  bool whole;
+  bool whole, join;        // join: an item may have several splits
   int group, head_tiles;   // heads of a kv head, tiles of 16 of them
   int tile_tokens, rows;   // new tokens of a tile, its rows (16 at most)
   int waves, least;        // splits wanted, a split's fewest steps of 64 keys

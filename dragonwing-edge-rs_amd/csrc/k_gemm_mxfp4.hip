@@ -366,8 +366,8 @@ typedef __attribute__((address_space(3))) void* LdsPtr;
 
 // A tile of WM x TM x 16 rows of A and WN x TN x 16 of W by WM x WN waves.
 //
-// K goes by in stages of whole cache lines: 256 elements of MXFP4 rows (128
-// bytes), 128 of f16 rows (256 bytes); of W 64 bytes a row there.  Loads write
+// K goes by in stages of whole cache lines: 256 elements of MXFP4 rows, 64 of
+// f16 rows (128 bytes); of W 32 bytes a row there.  Loads write
 // to LDS directly, a stage ahead, into the half of LDS that the last stage
 // left; a stage's products come in parts of one matrix instruction's depth,
 // each part's operands read ahead of the products of the part before, also
@@ -377,8 +377,8 @@ typedef __attribute__((address_space(3))) void* LdsPtr;
 template <bool MX, int WM, int WN, int TM, int TN>
 struct Tile {
   static constexpr int kWaves = WM * WN, kRowsA = WM * TM * 16, kRowsW = WN * TN * 16;
-  static constexpr int kDepth = MX ? 256 : 128, kParts = MX ? 2 : 4, kSpan = 512 / kDepth;
-  static constexpr int kLineA = MX ? 128 : 256, kLineW = MX ? 128 : 64;  // bytes of a row and stage
+  static constexpr int kDepth = MX ? 256 : 64, kParts = 2, kSpan = 512 / kDepth;
+  static constexpr int kLineA = 128, kLineW = MX ? 128 : 32;  // bytes of a row and stage
   static constexpr int kA = kRowsA * kLineA, kW = kRowsW * kLineW, kStage = kA + kW;
   static constexpr int kScaleRows = (MX ? kRowsA : 0) + kRowsW, kScales = kScaleRows * 16;
   static constexpr int kLds = 2 * (kStage + kScales);
@@ -395,7 +395,7 @@ struct Tile {
 
   // LDS keeps rows of A (and, for MXFP4 rows, of W) as they are, but the pieces
   // of row r stand at their index xor r: eight lanes that read one piece of
-  // eight rows meet all banks.  Rows of W of 64 bytes stand 16 together, piece
+  // eight rows meet all banks.  Rows of W of 32 bytes stand 32 together, piece
   // by piece.
   __device__ __forceinline__ Tile(const GemmMxArgs& args, uint8_t* shared, int row0, int col0)
       : g(args), lds(shared), m0(row0), n0(col0) {
@@ -412,7 +412,7 @@ struct Tile {
     }
 #pragma unroll
     for (int i = 0; i < kLoadsW; ++i) {
-      const int r = MX ? (wave * kLoadsW + i) * 8 + lane / 8 : (wave * kLoadsW + i) * 16 + col;
+      const int r = MX ? (wave * kLoadsW + i) * 8 + lane / 8 : (wave * kLoadsW + i) * 32 + lane % 32;
       at_w[i] = (uint32_t)(min(r, g.n - 1 - n0) * row_w) + piece_w() * 16;
     }
 #pragma unroll
@@ -425,7 +425,7 @@ struct Tile {
     const int r = i * (1024 / kLineA) + lane / (kLineA / 16);  // of the row's last three bits
     return lane % (kLineA / 16) ^ (r & 7);
   }
-  __device__ __forceinline__ int piece_w() const { return MX ? lane % 8 ^ lane / 8 : quad; }
+  __device__ __forceinline__ int piece_w() const { return MX ? lane % 8 ^ lane / 8 : lane / 32; }
   __device__ __forceinline__ int scale_row(int i) const { return (wave + i * kWaves) % (kScaleRows / 64) * 64 + lane; }
 
   // LAST: some of the stage's pieces may lie behind the end of K.
@@ -433,8 +433,8 @@ struct Tile {
   __device__ __forceinline__ void load(uint8_t* __restrict__ slot, int stage) const {
     const uint8_t* pa = base_a + (size_t)stage * kLineA;
     const uint8_t* pw = base_w + (size_t)stage * kLineW;
-    const int pieces = LAST ? (MX ? (g.k + 31) / 32 - stage * 8 : (g.lda - stage * 128) / 8) : 0;
-    const int pieces_w = LAST ? (g.k + 31) / 32 - stage * (MX ? 8 : 4) : 0;
+    const int pieces = LAST ? (MX ? (g.k + 31) / 32 : g.lda / 8) - stage * 8 : 0;
+    const int pieces_w = LAST ? (g.k + 31) / 32 - stage * (kDepth / 32) : 0;
 #pragma unroll
     for (int i = 0; i < kLoadsA; ++i) {
       const uint8_t* p = pa + at_a[i];
@@ -483,12 +483,12 @@ struct Tile {
 #pragma unroll
       for (int t = 0; t < TN; ++t) r.fw[t] = sw[t * 256];
     } else {
-      const uint8_t* sw = scales + (wn * TN * 16 + col) * 16 + (stage & 3) * 4;
-      const uint8_t* pw = p + kA + wn * TN * 1024 + part * 256 + col * 16 + quad * 4;
+      const uint8_t* sw = scales + (wn * TN * 16 + col) * 16 + (stage & 7) * 2;
+      const uint8_t* pw = p + kA + wn * TN * 512 + part * 512 + col * 16 + quad * 4;
 #pragma unroll
-      for (int t = 0; t < TN; ++t) r.word[t] = *(const uint32_t*)(pw + t * 1024);
+      for (int t = 0; t < TN; ++t) r.word[t] = *(const uint32_t*)(pw + t / 2 * 1024 + t % 2 * 256);
 #pragma unroll
-      for (int t = 0; t < TN; ++t) r.fw[t] = *(const uint32_t*)(sw + t * 256);
+      for (int t = 0; t < TN; ++t) r.fw[t] = *(const uint16_t*)(sw + t * 256);
     }
   }
   template <bool EXACT>
@@ -504,13 +504,13 @@ struct Tile {
                                                                       (int)r.fx[u]);
         }
       } else {
-        const float f = __builtin_bit_cast(float, part == 3 ? r.fw[t] >> 1 : r.fw[t] << (23 - 8 * part));
+        const float f = __builtin_bit_cast(float, r.fw[t] << (23 - 8 * part));
         if constexpr (EXACT) {
 #pragma unroll
           for (int u = 0; u < TM; ++u) acc[t][u] = times_exact(r.word[t], f, __builtin_bit_cast(f16x8, r.x[u]), acc[t][u]);
         } else {
-          // factors of 2^-15 to 1, as weights have them, four at a time
-          if (part == 0) *far |= (r.fw[t] ^ 0x70707070u) & 0xF0F0F0F0u;
+          // factors of 2^-15 to 1, as weights have them, both parts' at a time
+          if (part == 0) *far |= (r.fw[t] ^ 0x7070u) & 0xF0F0u;
           const f16x8 v = eight_f16(r.word[t], f);
 #pragma unroll
           for (int u = 0; u < TM; ++u)
@@ -570,7 +570,7 @@ struct Tile {
     Operands one, two = {};  // zeros times zeros come before the first stage
     if constexpr (!MX) {
 #pragma unroll
-      for (int t = 0; t < TN; ++t) two.fw[t] = 0x70707070u;
+      for (int t = 0; t < TN; ++t) two.fw[t] = 0x7070u;
     }
     load_scales(lds + 2 * kStage, from / kSpan);
     load<true>(lds, from);
@@ -702,18 +702,20 @@ Plan plan(const GemmMxArgs& a) {
   }
   // The expected time of each tile and number of shares: rounds of workgroups
   // over the chip, each its stages and a start, and the joining of the shares
-  // at 4 bytes a sum and share.  Measured stages: f16 rows 1.9 us (128 x 256,
-  // a workgroup a CU) and 1.3 us (128 x 128); MXFP4 rows 2.7 us (256 x 256),
-  // and 128 x 128 1.7 us for two workgroups a CU, 1.1 us for one.
-  const int depth = a.as ? 256 : 128, spans = (a.k + 511) / 512;
+  // at 4 bytes a sum and share.  Measured stages of 256 x 256: f16 rows 1.45 us
+  // on a few CUs, 1.83 us on all, MXFP4 rows 2.7 us; of 128 x 128, with one
+  // workgroup a CU and with two: f16 rows 0.62 and 1.10 us, MXFP4 rows 1.0 and
+  // 1.55 us.
+  const int depth = a.as ? 256 : 64, spans = (a.k + 511) / 512;
   double best = 1e30;
   for (int big = 0; big < 2; ++big) {
-    const int rows = a.as && big ? 256 : 128, cols = big ? 256 : 128, slots = a.as && !big ? 512 : 256;
+    const int rows = big ? 256 : 128, cols = rows, slots = big ? 256 : 512;
     const size_t tiles = (size_t)((a.m + rows - 1) / rows) * ((a.n + cols - 1) / cols);
     for (int shares = 1; shares <= 16 && shares <= spans; shares *= 2) {
       const double rounds = (double)((tiles * shares + slots - 1) / slots);
-      const double two = std::min(std::max(tiles * shares / 256.0 - 1.0, 0.0), 1.0);  // share of CUs that have two
-      const double stage = a.as ? (big ? 2.7 : 1.1 + 0.6 * two) : (big ? 1.9 : 1.3);
+      const double one = std::min(tiles * shares / 256.0, 1.0);                         // share of CUs that have one
+      const double two = std::min(std::max(tiles * shares / 256.0 - 1.0, 0.0), 1.0);  // and that have two
+      const double stage = a.as ? (big ? 2.7 : 1.0 + 0.55 * two) : (big ? 1.45 + 0.38 * one : 0.62 + 0.48 * two);
       double t = rounds * (3.0 + stage * ((spans + shares - 1) / shares * (512 / depth)));
       if (shares > 1) t += 2.0 + (double)a.m * a.n * 4 * (2 * shares + 1) / 8e6;
       if (t < best) best = t, p.big = big, p.shares = shares;
@@ -728,8 +730,6 @@ void launch_tiles(hipStream_t st, const GemmMxArgs& a, int shares) {
   using T = Tile<MX, WM, WN, TM, TN>;
   const int tm = (a.m + T::kRowsA - 1) / T::kRowsA, tn = (a.n + T::kRowsW - 1) / T::kRowsW;
   auto* k = gemm_mx_tile_kernel<MX, WM, WN, TM, TN>;
-  static const hipError_t sized = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds);
-  DW_HIP(sized);
   hipLaunchKernelGGL(k, dim3((unsigned)((size_t)tm * tn), (unsigned)shares), dim3(WM * WN * 64), T::kLds, st, a, tm, tn);
 }
 
@@ -770,7 +770,7 @@ void launch_gemm_mx(hipStream_t st, GemmMxArgs a, void* space) {
   if (a.as)
     p.big ? launch_tiles<true, 2, 4, 8, 4>(st, a, p.shares) : launch_tiles<true, 2, 2, 4, 4>(st, a, p.shares);
   else
-    p.big ? launch_tiles<false, 2, 4, 4, 4>(st, a, p.shares) : launch_tiles<false, 2, 2, 4, 4>(st, a, p.shares);
+    p.big ? launch_tiles<false, 2, 4, 8, 4>(st, a, p.shares) : launch_tiles<false, 2, 2, 4, 4>(st, a, p.shares);
   if (p.shares > 1)
     hipLaunchKernelGGL(gemm_mx_join_kernel, dim3((unsigned)((a.n + 1023) / 1024), (unsigned)std::min(a.m, 65535)),
                        dim3(256), 0, st, a, p.shares);

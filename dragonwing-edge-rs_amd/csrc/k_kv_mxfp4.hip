@@ -755,9 +755,6 @@ template <int D>
 void launch_tiles(hipStream_t st, const KvArgs& a, const AttnArgs& g) {
   constexpr int kKeys = D == 256 ? 32 : 64, kLds = 2 * kKeys * (D * 4 + 48);
   const int tile_tokens = 128 / (g.heads / a.kv_heads), tiles = std::min(a.tokens, a.tokens / tile_tokens + a.batch);
-  static const hipError_t sized =
-      hipFuncSetAttribute((const void*)attention_tile_kernel<D>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-  DW_HIP(sized);
   hipLaunchKernelGGL(attention_tile_kernel<D>, dim3((unsigned)(tiles * a.kv_heads)), dim3(256), kLds, st, a, g,
                      tile_tokens, tiles);
 }
@@ -768,6 +765,7 @@ void launch_splits(hipStream_t st, const KvArgs& a, const AttnArgs& g, const Spl
   const dim3 rows((unsigned)a.tokens, (unsigned)(a.kv_heads * p.head_tiles), (unsigned)p.rows);
   const bool few = (long long)a.tokens * g.heads <= 512;
   hipLaunchKernelGGL(attention_split_kernel<D>, dim3((unsigned)p.splits), dim3(64), 0, st, a, g, p);
+  if (!p.join) return;  // a split takes all keys that the table has room for
   if (few)
     hipLaunchKernelGGL((attention_join_kernel<D, 512>), rows, dim3(512), 0, st, a, g, p);
   else
@@ -790,8 +788,14 @@ size_t attention_space(const KvArgs& a, const AttnArgs& g, SplitArgs* p) {
   const long long tiles = std::min<long long>(a.tokens, a.tokens / p->tile_tokens + (long long)a.batch);
   const long long heads = (long long)a.kv_heads * p->head_tiles;
   p->waves = 2048;
-  p->least = 2;
-  p->splits = (int)(tiles * heads + p->waves);
+  p->waves = a.d == 256 ? 1024 : 2048;  // that the chip holds at a time
+  // A split takes two steps of 64 keys or more, or all of them where joining
+  // would take longer: one sequence of 1,024 keys 12.2 us in splits of two, 20.9
+  // us in splits of eight; 64 of up to 512 17.5 us split, 14.1 us whole.
+  const int steps = ((a.max_pages << a.page_shift) + kChunk - 1) / kChunk;  // of the longest sequence
+  p->join = steps > (tiles * heads >= 256 ? 8 : 4);
+  p->least = p->join ? 2 : 8;
+  p->splits = (int)(tiles * heads + p->waves + 1);
   p->rows = std::min(16, p->group * p->tile_tokens);
   p->stats_at = (size_t)p->splits * p->rows * a.d * 4;
   p->items_at = p->stats_at + (size_t)p->splits * p->rows * 8;
