@@ -199,11 +199,13 @@ struct Piece {
   }
   __device__ __forceinline__ float scale(int word) const { return mx_scale(D == 256 && word >= 4 ? s >> 8 : D == 256 ? s & 255u : s); }
   __device__ __forceinline__ f16x8 eight(int word) const { return mx_eight(w[word], scale(word)); }
-  // The four pieces' blocks that are NaN, as bits of the row's blocks.
+  // The piece's blocks that are NaN, or whose factor passes f16, as bits of the
+  // row's blocks.
+  static __device__ __forceinline__ bool bad(uint32_t byte) { return byte > 127u + 13u; }
   __device__ __forceinline__ uint32_t nan_bits(int quarter) const {
-    if constexpr (D == 64) return s == 255u ? 1u << (quarter >> 1) : 0u;
-    if constexpr (D == 128) return s == 255u ? 1u << quarter : 0u;
-    return ((s & 255u) == 255u ? 1u << (2 * quarter) : 0u) | ((s >> 8) == 255u ? 2u << (2 * quarter) : 0u);
+    if constexpr (D == 64) return bad(s) ? 1u << (quarter >> 1) : 0u;
+    if constexpr (D == 128) return bad(s) ? 1u << quarter : 0u;
+    return (bad(s & 255u) ? 1u << (2 * quarter) : 0u) | (bad(s >> 8) ? 2u << (2 * quarter) : 0u);
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -212,9 +214,9 @@ struct Piece {
   }
   __device__ __forceinline__ void clear_nan() {
     if constexpr (D == 256) {
-      if ((s & 255u) == 255u) w[0] = w[1] = w[2] = w[3] = 0, s = (s & 0xFF00u) | 127u;
-      if ((s >> 8) == 255u) w[4] = w[5] = w[6] = w[7] = 0, s = (s & 255u) | 0x7F00u;
-    } else if (s == 255u) {
+      if (bad(s & 255u)) w[0] = w[1] = w[2] = w[3] = 0, s = (s & 0xFF00u) | 127u;
+      if (bad(s >> 8)) w[4] = w[5] = w[6] = w[7] = 0, s = (s & 255u) | 0x7F00u;
+    } else if (bad(s)) {
       clear();
     }
   }

@@ -399,7 +399,7 @@ int dw_hip_rope_axes(dw_hip_backend* be, int dtype, const dw_hip_buffer* x, size
  * as dw_hip_quantize_mxfp4 does, but with scales of at least 2^-23: every
  * value of the cache is then an f16 value.  A token whose position or page
  * is outside the table or the cache is not written.  Two tokens on one
- * place: either is written. */
+ * place: what the row then holds is unspecified. */
 int dw_hip_kv_append_mxfp4(dw_hip_backend* be, const dw_hip_buffer* k, size_t k_stride, size_t k_off,
                            const dw_hip_buffer* v, size_t v_stride, size_t v_off, dw_hip_buffer* k_cache,
                            dw_hip_buffer* k_scales, dw_hip_buffer* v_cache, dw_hip_buffer* v_scales,
@@ -415,6 +415,8 @@ int dw_hip_kv_append_mxfp4(dw_hip_backend* be, const dw_hip_buffer* k, size_t k_
  * and with a window > 0 the last `window` of them.  A row that sees no key,
  * or only scores of -inf, is 0.  Keys that a row does not see do not reach
  * it, whatever they hold; keys on pages outside the cache are seen by none.
+ * Values of the cache are read as f16: scales above 2^13, which append never
+ * writes, may give infinities or NaN in the rows that see them.
  * Scores and sums are f32; p is rounded to f16 before it meets the values.
  * Rows of y that belong to no sequence are left as they were. */
 int dw_hip_attention_mxfp4(dw_hip_backend* be, const dw_hip_buffer* q, size_t q_stride, size_t q_off,

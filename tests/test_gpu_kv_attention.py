@@ -193,6 +193,149 @@ def test_growing_scores(backend):
     check(attend(backend, c, q, 1.0), *ref.attention(q.astype(np.float64), c, 1.0))
 
 
+@pytest.mark.parametrize("most", [1, 9])
+def test_many_sequences(backend, most):
+    # more than a wave has lanes, some without keys or new tokens
+    rng = np.random.default_rng(most)
+    nq = [int(x) for x in rng.integers(0, most + 1, 150)]
+    kv = [n + int(x) for n, x in zip(nq, rng.integers(0, 90, 150))]
+    kv[3] = kv[70] = 0
+    kv[140] = 400
+    c = ref.Cache(rng, nq, kv, 1, 64, 16, extra=1)
+    q = rng.normal(0, 1, (c.tokens, 3, 64)).astype(np.float16)
+    check(attend(backend, c, q, 0.125), *ref.attention(q.astype(np.float64), c, 0.125))
+
+
+def test_many_sequences_of_many_new_tokens(backend):
+    rng = np.random.default_rng(31)
+    nq = [int(x) for x in rng.integers(0, 40, 80)]
+    nq[5], nq[77] = 150, 140
+    kv = [n + int(x) for n, x in zip(nq, rng.integers(0, 60, 80))]
+    c = ref.Cache(rng, nq, kv, 2, 64, 16)
+    q = rng.normal(0, 1, (c.tokens, 16, 64)).astype(np.float16)
+    assert c.tokens * 16 >= 12288
+    check(attend(backend, c, q, 0.125), *ref.attention(q.astype(np.float64), c, 0.125))
+
+
+@pytest.mark.parametrize("nq", [[1, 2], [120, 9]])
+@pytest.mark.parametrize("heads,kv_heads", [(160, 1), (256, 2), (34, 2)])
+def test_many_heads_of_a_kv_head(backend, heads, kv_heads, nq):
+    rng = np.random.default_rng(heads)
+    c = ref.Cache(rng, nq, [150, 77], kv_heads, 64, 32)
+    q = rng.normal(0, 1, (c.tokens, heads, 64)).astype(np.float16)
+    check(attend(backend, c, q, 0.125), *ref.attention(q.astype(np.float64), c, 0.125))
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 100)])
+def test_prompts_of_whole_tiles(backend, d, causal, window):
+    rng = np.random.default_rng(d + window)
+    c = ref.Cache(rng, [260, 0, 131], [300, 20, 500], 2, d, 64, extra=2)
+    q = rng.normal(0, 1, (c.tokens, 32, d)).astype(np.float16)
+    assert c.tokens * 32 >= 12288
+    check(attend(backend, c, q, d ** -0.5, causal, window), *ref.attention(q.astype(np.float64), c, d ** -0.5, causal,
+                                                                        window))
+
+
+def test_whole_tiles_with_bad_pages_nan_and_empty_rows(backend):
+    rng = np.random.default_rng(77)
+    c = ref.Cache(rng, [300, 200], [280, 333], 1, 128, 16)
+    for name, b, j, blk in (("v", 0, 250, 3), ("k", 0, 270, 1), ("v", 1, 300, 0)):
+        c.s[name][c.table[b, j // 16], 0, j % 16, blk] = 255
+    q = rng.normal(0, 1, (c.tokens, 32, 128)).astype(np.float16)
+    want, off = ref.attention(q.astype(np.float64), c, 0.1)
+    got = attend(backend, c, q, 0.1)
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+    check(got, want, np.where(np.isnan(off), 0, off))
+    assert (got[:20] == 0).all()  # the first 20 of 300 new tokens have no key among 280
+    # pages outside the cache: as if their keys were masked
+    bufs = put(backend, c)
+    table = c.table.copy()
+    table[1, 2], table[1, 20] = c.num_pages, -3
+    bufs[4] = backend.from_numpy(table)
+    got = attend(backend, c, q, 0.1, bufs=bufs)
+    r, h = 300 + 150, 5
+    pos = 333 - 200 + 150
+    j = np.array([x for x in range(pos + 1) if x // 16 not in (2, 20)])
+    k, v = c.rows("k", 1, 0)[j], c.rows("v", 1, 0)[j]
+    e = k @ q[r, h].astype(np.float64) * 0.1
+    e = np.exp(e - e.max())
+    np.testing.assert_allclose(got[r, h], e @ v / e.sum(), rtol=2.0 ** -10, atol=8 * 2.0 ** -11)
+
+
+def test_long_splits(backend):
+    # so many steps that a split takes more than its first 1,024 keys' pages; some heads against the oracle
+    rng = np.random.default_rng(15)
+    batch, hk, d, page, keys = 64, 8, 64, 64, 4700
+    pages = -(-keys // page)
+    n = batch * pages
+    table = rng.permutation(n).astype(np.int32).reshape(batch, pages)
+    q8 = {x: rng.integers(0, 256, (n, hk, page, d // 2), dtype=np.uint8) for x in "kv"}
+    s8 = {x: rng.integers(121, 127, (n, hk, page, d // 32), dtype=np.uint8) for x in "kv"}
+    bufs = [backend.from_numpy(x) for x in (q8["k"], s8["k"], q8["v"], s8["v"], table,
+                                            np.arange(batch + 1, dtype=np.int32), np.full(batch, keys, np.int32))]
+    q = rng.normal(0, 1, (batch, hk, d)).astype(np.float16)
+    y = backend.alloc(q.nbytes)
+    ops.attention_mxfp4(backend, backend.from_numpy(q), hk * d, 0, *bufs, y, batch, batch, hk, hk, d, page, n, pages,
+                        0.125)
+    got = backend.to_numpy(y, np.float16, q.shape).astype(np.float64)
+    for b, h in ((0, 0), (7, 3), (31, 7), (63, 1)):
+        k, v = (ref.decode(q8[x][table[b], h], s8[x][table[b], h], d).reshape(-1, d)[:keys] for x in "kv")
+        s = k @ q[b, h].astype(np.float64) * 0.125
+        e = np.exp(s - s.max())
+        want, mean = e @ v / e.sum(), e @ np.abs(v) / e.sum()
+        off = mean * (2.0 ** -11 + 2 * (d + 3) * 2.0 ** -23 * (np.abs(k) @ np.abs(q[b, h].astype(np.float64))).max() / 8
+                      + 2.0 ** -20 + keys * 2.0 ** -23) + keys * 2.0 ** -25 * np.abs(v).max() / e.sum()
+        assert (np.abs(got[b, h] - want) <= off + 2.0 ** -11 * np.abs(want) + 2.0 ** -25).all()
+
+
+def test_a_cache_past_32_bit_offsets(backend):
+    # pages of 256 KiB, the last ones past 2^32 bytes: appended to, then attended over
+    rng = np.random.default_rng(9)
+    hk, d, page, n = 8, 256, 256, 17000
+    rows = n * hk * page
+    bufs = [backend.alloc(rows * x) for x in (d // 2, d // 32, d // 2, d // 32)]
+    table = np.array([[n - 1, 3, n - 2]], np.int32)
+    t = 600
+    lists = [backend.from_numpy(x) for x in (table, np.array([0, t], np.int32), np.array([t], np.int32))]
+    kv = rng.normal(0, 1, (t, 2, hk, d)).astype(np.float16)
+    bkv = backend.from_numpy(kv)
+    ops.kv_append_mxfp4(backend, bkv, 2 * hk * d, 0, bkv, 2 * hk * d, hk * d, *bufs, *lists, t, 1, hk, d, page, n, 3)
+    q = rng.normal(0, 1, (1, hk, d)).astype(np.float16)
+    y = backend.alloc(q.nbytes)
+    lists[1] = backend.from_numpy(np.array([0, 1], np.int32))
+    ops.attention_mxfp4(backend, backend.from_numpy(q), hk * d, 0, *bufs, *lists, y, 1, 1, hk, hk, d, page, n, 3, 0.06)
+    got = backend.to_numpy(y, np.float16, q.shape).astype(np.float64)
+    for b in bufs:
+        b.free()
+    for h in range(hk):
+        k, v = (ref.decode(*ref.encode(kv[:, i, h].astype(np.float64), -23), d) for i in (0, 1))
+        s = k @ q[0, h].astype(np.float64) * 0.06
+        e = np.exp(s - s.max())
+        want, mean = e @ v / e.sum(), e @ np.abs(v) / e.sum()
+        assert (np.abs(got[0, h] - want) <= 1.5 * 2.0 ** -11 * mean + t * 2.0 ** -25 * 8 + 2.0 ** -11 * np.abs(want)).all()
+
+
+def test_two_backends_at_once(backend):
+    import dragonwing_edge_rs_amd as dw
+    rng = np.random.default_rng(44)
+    other = dw.Backend(0)
+    c = ref.Cache(rng, [1, 1, 3], [900, 40, 77], 2, 128, 16)
+    q = rng.normal(0, 1, (c.tokens, 8, 128)).astype(np.float16)
+    want = attend(backend, c, q, 0.1)
+    state = []
+    for be in (backend, other):
+        y = be.alloc(c.tokens * 8 * 128 * 2)
+        state.append((be, be.from_numpy(q), put(be, c), y))
+    for _ in range(20):
+        for be, bq, bufs, y in state:
+            ops.attention_mxfp4(be, bq, 1024, 0, *bufs, y, c.tokens, c.batch, 8, *sizes(c), 0.1)
+    for be, _, _, y in state:
+        np.testing.assert_array_equal(be.to_numpy(y, np.float16, q.shape).astype(np.float64), want)
+    del state, y
+    other.close()
+
+
 def test_attention_is_the_same_every_time(backend):
     rng = np.random.default_rng(12)
     for nq, kv in (([1, 1], [5000, 77]), ([100, 30], [700, 30])):
