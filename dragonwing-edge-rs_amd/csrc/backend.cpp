@@ -1273,6 +1273,7 @@ int dw_hip_quantize_mxfp4(dw_hip_backend* be, int dtype, const dw_hip_buffer* x,
   need_on(b, x, rows * k * es, "quantize_mxfp4: input");
   need_on(b, q, rows * blocks * 16, "quantize_mxfp4: packed rows");
   need_on(b, scales, rows * blocks, "quantize_mxfp4: scales");
+  if (x == q || x == scales || q == scales) dw::fail(DW_ERR_INVALID, "quantize_mxfp4: buffers overlap");
   dw::launch_quantize_mxfp4(b->stream, dtype, x->ptr, q->ptr, scales->ptr, rows, k);
   API_END
 }
@@ -1288,6 +1289,7 @@ int dw_hip_dequantize_mxfp4(dw_hip_backend* be, int dtype, const dw_hip_buffer* 
   need_on(b, q, rows * blocks * 16, "dequantize_mxfp4: packed rows");
   need_on(b, scales, rows * blocks, "dequantize_mxfp4: scales");
   need_on(b, y, rows * k * es, "dequantize_mxfp4: output");
+  if (y == q || y == scales) dw::fail(DW_ERR_INVALID, "dequantize_mxfp4: buffers overlap");
   dw::launch_dequantize_mxfp4(b->stream, dtype, q->ptr, scales->ptr, y->ptr, rows, k);
   API_END
 }
@@ -1441,7 +1443,7 @@ int dw_hip_attention_mxfp4(dw_hip_backend* be, const dw_hip_buffer* q, size_t q_
   if (heads > 4096) dw::fail(DW_ERR_UNSUPPORTED, "attention_mxfp4: more than 4096 heads");
   if (tokens * heads > kMostMx || batch * heads > kMostMx / 4)
     dw::fail(DW_ERR_UNSUPPORTED, "attention_mxfp4: more than 2^24 rows, or 2^22 heads of all sequences");
-  if (!std::isfinite(scale)) dw::fail(DW_ERR_INVALID, "attention_mxfp4: scale must be finite");
+  if (!std::isfinite(scale * 1.44269504f)) dw::fail(DW_ERR_INVALID, "attention_mxfp4: scale must be finite");
   if (causal != 0 && causal != 1) dw::fail(DW_ERR_INVALID, "attention_mxfp4: causal must be 0 or 1");
   if (window && !causal) dw::fail(DW_ERR_UNSUPPORTED, "attention_mxfp4: a window needs causal attention");
   check_columns(q_stride, q_off, heads, head_dim, "attention_mxfp4: queries");

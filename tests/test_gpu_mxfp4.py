@@ -158,6 +158,63 @@ def test_large_product(backend, m, n, k, kind):
     check_product(run_product(backend, a, q, s, m, n, k, b, 2, np.float16), want, off)
 
 
+@pytest.mark.parametrize("kind", ["f16", "mxfp4", "far"])
+def test_product_on_the_largest_tiles(backend, kind):
+    # enough tiles of 256 x 256 that they are chosen; "far": factors that f16 does not hold among them
+    rng = np.random.default_rng(11)
+    m, n, k = 4091, 8189, 136
+    q, s = weights(rng, n, k, 0.1)
+    a = rng.normal(0, 1, (m, k)).astype(np.float16)
+    if kind == "far":
+        s[n // 3, 2], s[n - 1, 4] = 90, 150
+    wide = a.astype(np.float64)
+    if kind == "mxfp4":
+        a = ref.encode(wide)
+        wide = ref.decode(*a, k)
+    b = rng.normal(0, 1, n).astype(np.float32)
+    want, off = ref.product(wide, ref.decode(q, s, k), b.astype(np.float64))
+    check_product(run_product(backend, a, q, s, m, n, k, b, 0, np.float32), want, off)
+
+
+def test_product_past_32_bit_offsets(backend):
+    # rows of A that reach past 2^32 bytes: 1,024 rows again and again, so that the oracle is small
+    rng = np.random.default_rng(5)
+    m, n, k = 70 * 1024, 48, 32768
+    q, s = weights(rng, n, k)
+    part = rng.normal(0, 1, (1024, k)).astype(np.float16)
+    ba, bc = backend.alloc(m * k * 2), backend.alloc(m * n * 4)
+    backend.upload(ba, np.tile(part, (m // 1024, 1)))
+    ops.gemm_mxfp4(backend, F16, ba, None, backend.from_numpy(q), backend.from_numpy(s), None, F32, bc, m, n, k)
+    got = backend.to_numpy(bc, np.float32, (m // 1024, 1024, n))
+    ba.free()
+    np.testing.assert_array_equal(got, np.broadcast_to(got[:1], got.shape))
+    check_product(got[0], *ref.product(part.astype(np.float64), ref.decode(q, s, k)))
+
+
+def test_products_of_two_threads_on_one_backend(backend):
+    import threading
+    rng = np.random.default_rng(8)
+    work = []
+    for m, n, k in ((70, 300, 4100), (3, 500, 1001), (130, 200, 9000), (20, 900, 2050)):
+        q, s = weights(rng, n, k)
+        a = rng.normal(0, 1, (m, k)).astype(np.float16)
+        work.append((a, q, s, m, n, k, run_product(backend, a, q, s, m, n, k, None, 0, np.float32)))
+    bad = []
+
+    def run(mine):
+        for _ in range(10):
+            for a, q, s, m, n, k, want in mine:
+                if not np.array_equal(run_product(backend, a, q, s, m, n, k, None, 0, np.float32), want):
+                    bad.append((m, n, k))
+
+    threads = [threading.Thread(target=run, args=(w,)) for w in (work[:2], work[2:], work[::-1])]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 @pytest.mark.parametrize("kind", ["f16", "mxfp4"])
 @pytest.mark.parametrize("m", [1, 20, 150, 400])
 def test_product_of_far_apart_scales(backend, m, kind):
@@ -249,5 +306,10 @@ def test_refused_buffers(backend):
         ops.gemm_mxfp4(be, F16, x, None, q, s, s, F16, be.alloc(5 * 4 * 2), 4, 5, 64)
     with pytest.raises(HipError, match="operand"):
         ops.gemm_mxfp4(be, F16, x, None, be.alloc(64 * 32), be.alloc(64 * 2), None, F16, x, 4, 64, 64)
+    tiny = be.alloc(3 * 16)
+    with pytest.raises(HipError, match="overlap"):
+        ops.quantize_mxfp4(be, F16, tiny, tiny, be.alloc(3), 3, 8)
+    with pytest.raises(HipError, match="overlap"):
+        ops.dequantize_mxfp4(be, F16, tiny, be.alloc(3), tiny, 3, 8)
     with pytest.raises(HipError, match="null buffer"):
         ops.gemm_mxfp4(be, F16, x, None, None, s, None, F16, c, 4, 4, 64)

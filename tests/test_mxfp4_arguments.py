@@ -41,7 +41,7 @@ class Fake:
 def test_product():
     for sizes in ((0, 4, 64), (4, 0, 64), (4, 4, 0)):
         refused("zero size", *gemm(*sizes))
-    for sizes in ((BIG, 4, 64), (4, (1 << 24) + 1, 64), (4, 4, BIG)):
+    for sizes in ((BIG, 4, 64), (4, (1 << 24) + 1, 64), (4, 4, BIG), (4, 4, (1 << 22) + 1)):
         refused("2\\^24", *gemm(*sizes))
     refused("A must be", *gemm(a=ops.DTYPE_F32))
     refused("A must be", *gemm(a=17))
@@ -128,8 +128,13 @@ def test_attention_options():
     refused("4096", *attend(heads=4098))
     refused("finite", *attend(scale=float("nan")))
     refused("finite", *attend(scale=float("inf")))
+    refused("finite", *attend(scale=3e38))
     refused("causal", *attend(causal=2))
     refused("window", *attend(causal=False, window=5))
     refused("do not fit", *attend(stride=511))
     refused("do not fit", *attend(off=1))
+    big = dict(KV, tokens=1 << 20, batch=2)
+    refused("2\\^24 rows", ops.attention_mxfp4, None, 4096, 0, *[None] * 8, big["tokens"], 2, 32, *list(big.values())[2:],
+            0.1)
+    refused("2\\^22", ops.attention_mxfp4, None, 1 << 20, 0, *[None] * 8, 4, 60000, 128, *list(big.values())[2:], 0.1)
     refused("null backend", *attend())
