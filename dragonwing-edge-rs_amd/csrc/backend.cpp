@@ -1461,12 +1461,13 @@ int dw_hip_attention_mxfp4(dw_hip_backend* be, const dw_hip_buffer* q, size_t q_
   g.q_stride = q_stride;
   g.q_off = q_off;
   g.y = (uint16_t*)y->ptr;
+  g.tokens = (int)tokens;
   g.heads = (int)heads;
   g.causal = causal;
   g.window = window > (size_t)INT32_MAX ? 0 : (long long)window;
-  g.scale = fabsf(scale) * 1.44269504f;
+  g.scale = std::max(fabsf(scale) * 1.44269504f, 1e-37f);  // above 0, where -inf stays so; as 0, to a score
   g.negate = scale < 0;
-  dw::SplitArgs p{};
+  dw::AttnPlan p{};
   const size_t bytes = dw::attention_space(a, g, &p);
   dw::launch_attention(b->stream, a, g, p, bytes ? b->workspace(Backend::WS_ATTN, bytes) : nullptr);
   API_END

@@ -496,27 +496,37 @@ struct AttnArgs {
   const uint16_t* q;
   size_t q_stride, q_off;
   uint16_t* y;  // [tokens][heads][d]
-  int heads, causal, negate;  // negate: the scale is below zero
+  int tokens, heads, causal, negate;  // negate: the scale is below zero
   long long window;
   float scale;  // |scale| log2(e): p = 2^(scale (s - max))
 };
-// How attention is cut: whole tiles of many rows, or few rows split over keys
-// and what the splits leave.  Set by attention_space, which gives the bytes of
-// workspace.
+// One of attention's two forms, tiles of 128 rows (new tokens x heads of a kv
+// head) or of 16: how a sequence is cut into tiles, and the tiles' keys into
+// splits.  Tiles of 128 take the sequences of `big` rows or more, where those
+// come to `big_steps` steps of 64 keys in all.
 struct SplitArgs {
-  bool whole, join;        // join: an item may have several splits
-  int group, head_tiles;   // heads of a kv head, tiles of 16 of them
-  int tile_tokens, rows;   // new tokens of a tile, its rows (16 at most)
-  int waves, least;        // splits wanted, a split's fewest steps of 64 keys
-  int splits;              // of the grid
-  float* sums;             // [splits][rows][d]
-  float2* stats;           // [splits][rows]: reference, sum
-  int2* items;             // [tokens][kv heads x head tiles]: first split, splits
-  size_t stats_at, items_at;  // bytes into the workspace
+  long long big;
+  int big_tokens;  // new tokens of a tile of 128 rows
+  float big_steps;
+  int group, head_tiles;  // heads of a kv head, tiles of them
+  int tile_tokens, rows;  // new tokens of a tile, its rows
+  int chunk;              // keys of a step
+  int waves, least;       // splits wanted, a split's fewest steps
+  int whole;              // items of under `whole` splits' steps are not split
+  int items, splits;      // tiles x kv heads at most, and splits: the grid
+  int slots, joined;      // splits of items that have several and such items, at most; no slots: none has
+  float* sums;            // [slots][rows][d]
+  float2* stats;          // [slots][rows]: reference, sum
+  int4* table;            // [1 + joined]: their number; first slot, splits and tokens, first token, first head
 };
-size_t attention_space(const KvArgs& a, const AttnArgs& g, SplitArgs* p);
+struct AttnPlan {
+  SplitArgs tiles, few;  // of 128 rows, of 16; no splits: not used
+  size_t at[2][3];       // of their sums, stats and table: bytes into the workspace
+};
+// Sets the plan and gives the bytes of workspace.
+size_t attention_space(const KvArgs& a, const AttnArgs& g, AttnPlan* p);
 void launch_kv_append(hipStream_t st, const KvArgs& a, const void* k, size_t k_stride, size_t k_off, const void* v,
                       size_t v_stride, size_t v_off);
-void launch_attention(hipStream_t st, const KvArgs& a, const AttnArgs& g, SplitArgs p, void* space);
+void launch_attention(hipStream_t st, const KvArgs& a, const AttnArgs& g, AttnPlan p, void* space);
 
 }  // namespace dw

@@ -5,7 +5,6 @@
 // bytes and [page][head][slot][d / 32] scales: the rows are MXFP4 rows of d
 // elements (mxfp4.h), so the cache's values can be read back as such rows.
 #include <algorithm>
-#include <type_traits>
 
 #include "dw_common.h"
 #include "mxfp4.h"
@@ -69,15 +68,15 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a, const uint16_t
   }
 }
 
-// A wave's share of the work: keys [begin, end) of a tile of up to 16 rows
-// (new tokens of one sequence x heads of one kv head).
-constexpr int kChunk = 64;  // keys a step
-
+// A share of the work: some steps of the keys of an item, a tile of rows (new
+// tokens of one sequence x heads of one kv head).
 struct Split {
   int seq, token, count;  // the tile's first token and how many it has
   int kv_head, head;      // head: the tile's first
   int index, of;          // this split of the item's
-  int first, chunks;      // steps before this split, and its own
+  int slot;               // the item's first place in the workspace, where it has several splits
+  int item;               // and its place among such items
+  int first, steps;       // steps before this split, and its own
   long long pos, len;     // position of the tile's first token, keys of the sequence
 };
 
@@ -93,49 +92,102 @@ __device__ __forceinline__ int sums_upto(int v) {
   return v;
 }
 
-// Which split this wave has.  Every item (tile, kv head) of a sequence has
-// the same number of steps; all steps over the waves wanted is a split's
-// length, so that long and short sequences share the waves evenly whatever
-// their lengths, which only the device knows.  One load a 64 sequences.
-__device__ __forceinline__ bool plan(const KvArgs& a, const AttnArgs& g, const SplitArgs& p, int mine, Split* s) {
+// Which split number `mine` is; LAST: counted from the end.  Every item of a
+// sequence has the same number of steps; all steps over the splits wanted is a
+// split's length, so that long and short sequences share the chip evenly
+// whatever their lengths, which only the device knows.  One load a 64
+// sequences.  *joined: how many items have several splits (for split 0).
+//
+// An item has n = ceil(steps / length) splits: all items under the number of
+// items + `waves`, and the items that have two or more under 2 `waves`.
+constexpr long long kNever = 1ll << 62;
+template <bool LAST>
+__device__ __forceinline__ bool plan(const KvArgs& a, const AttnArgs& g, const SplitArgs& p, int mine, Split* s,
+                                     int* joined) {
   const int lane = threadIdx.x & 63, heads = p.head_tiles * a.kv_heads;
   const int most = a.max_pages << a.page_shift;
   int first, items, steps, count, len, raw;
-  auto of = [&](int b) {
-    first = count = items = len = raw = 0;
-    steps = 1;
+  bool on = true;  // tiles of 128 rows
+  auto load = [&](int b) {
+    first = count = len = raw = 0;
     if (b >= a.batch) return;
     const int t0 = a.start[b], t1 = a.start[b + 1];
     raw = a.len[b];
     first = max(t0, 0);
     count = max(min(t1, a.tokens) - first, 0);
     len = min(max(raw, 0), most);
-    items = (count + p.tile_tokens - 1) / p.tile_tokens * heads;
-    const int span = g.window > 0 ? (int)min((long long)len, g.window + p.tile_tokens + 14) : len;
-    steps = max(1, (span + kChunk - 1) / kChunk);
   };
-  // the total, in f32: it only has to be the same for all waves
-  float all = 0.0f;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    of(b0 + lane);
-    float v = (float)items * (float)steps;
+  auto is_big = [&] { return (long long)count * p.group >= p.big; };
+  auto steps_of = [&](int tokens, int chunk) {
+    const int span = g.window > 0 ? (int)min((long long)len, g.window + tokens + 14) : len;
+    return max(1, (span + chunk - 1) / chunk);
+  };
+  auto cut = [&] {
+    const bool mine_too = (on && is_big()) == LAST;
+    items = mine_too ? (count + p.tile_tokens - 1) / p.tile_tokens * heads : 0;
+    steps = steps_of(p.tile_tokens, p.chunk);
+  };
+  auto of = [&](int b) {
+    load(b);
+    cut();
+  };
+  auto total_of = [&](float v) {
 #pragma unroll
     for (int i = 1; i < 64; i *= 2) v += __shfl_xor(v, i);
-    all += v;
+    return v;
+  };
+  // the totals, in f32: they only have to be the same for all waves
+  load(lane);
+  if (p.big < kNever) {
+    float tiles = 0.0f;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+      if (a.batch > 64) load(b0 + lane);
+      const int n = is_big() ? (count + p.big_tokens - 1) / p.big_tokens * a.kv_heads : 0;
+      tiles += total_of((float)n * (float)steps_of(p.big_tokens, 64));
+    }
+    on = tiles >= p.big_steps;
+  }
+  cut();
+  float all = 0.0f;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    if (a.batch > 64) of(b0 + lane);
+    all += total_of((float)items * (float)steps);
   }
   const int length = max(p.least, (int)fminf(ceilf(all / (float)p.waves), 1e9f));
-  int before = 0;
+  auto parts = [&] { return steps < p.whole * length ? 1 : (steps - 1) / length + 1; };
+  *joined = 0;
+  if (mine == 0) {
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+      if (a.batch > 64) of(b0 + lane);
+      *joined += __builtin_amdgcn_readlane(sums_upto(parts() > 1 ? items : 0), 63);
+    }
+    if (a.batch > 64) of(lane);
+  }
+  if (LAST) {
+    int splits = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+      if (a.batch > 64) of(b0 + lane);
+      splits += __builtin_amdgcn_readlane(sums_upto(items * parts()), 63);
+    }
+    mine = splits - 1 - mine;
+    if (mine < 0) return false;
+  }
+  int before = 0, items_before = 0, slots_before = 0;
   for (int b0 = 0; b0 < a.batch && before <= mine; b0 += 64) {
     if (a.batch > 64) of(b0 + lane);
-    const int n = (steps - 1) / length + 1;
-    const int upto = sums_upto(items * n), here = items * n;
+    const int n = parts(), here = items * n, several = n > 1 ? items : 0;
+    const int upto = sums_upto(here), items_upto = sums_upto(several), slots_upto = sums_upto(several * n);
     const unsigned long long hit = __ballot(mine >= before + upto - here && mine < before + upto);
     if (hit) {
       const int src = __ffsll(hit) - 1;
       s->of = __builtin_amdgcn_readlane(n, src);
       const int at = mine - before - __builtin_amdgcn_readlane(upto - here, src);
-      const int item = at / s->of, tile = item / heads, hh = item - tile * heads;
-      s->index = at - item * s->of;
+      // the splits of a kv head side by side: on one XCD, where there are eight
+      const int each = __builtin_amdgcn_readlane(items, src);
+      s->index = at / each;
+      const int item = at - s->index * each, tile = item / heads, hh = item - tile * heads;
+      s->item = items_before + __builtin_amdgcn_readlane(items_upto - several, src) + item;
+      s->slot = slots_before + __builtin_amdgcn_readlane(slots_upto - several * n, src) + item * s->of;
       s->seq = b0 + src;
       s->kv_head = hh / p.head_tiles;
       s->head = s->kv_head * p.group + (hh - s->kv_head * p.head_tiles) * 16;
@@ -146,12 +198,24 @@ __device__ __forceinline__ bool plan(const KvArgs& a, const AttnArgs& g, const S
       // the raw length places the tokens, whatever the table holds
       s->pos = (long long)__builtin_amdgcn_readlane(raw, src) - whole + skip;
       s->first = s->index * length;
-      s->chunks = min(length, __builtin_amdgcn_readlane(steps, src) - s->first);
+      const int steps_all = __builtin_amdgcn_readlane(steps, src);
+      s->steps = s->of == 1 ? steps_all : min(length, steps_all - s->first);
       return true;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
+    items_before += __builtin_amdgcn_readlane(items_upto, 63);
+    slots_before += __builtin_amdgcn_readlane(slots_upto, 63);
   }
   return false;
+}
+
+// What the join needs to know: how many items have several splits, from split
+// 0, and of each of them, from its first.
+__device__ __forceinline__ void note_item(const SplitArgs& p, int id, const Split& s, bool have, int joined) {
+  if (!p.slots) return;
+  if (id == 0) p.table[0].x = joined;
+  if (have && s.of > 1 && s.index == 0 && (uint32_t)s.item < (uint32_t)p.joined)
+    p.table[1 + s.item] = make_int4(s.slot, s.of | s.count << 24, s.token, s.head);
 }
 
 __device__ __forceinline__ float max_of_rows(float v) {  // over the four lanes of a column
@@ -197,7 +261,9 @@ struct Piece {
       s = *(const uint16_t*)(scales + row * 8 + quarter * 2);
     }
   }
-  __device__ __forceinline__ float scale(int word) const { return mx_scale(D == 256 && word >= 4 ? s >> 8 : D == 256 ? s & 255u : s); }
+  __device__ __forceinline__ float scale(int word) const {
+    return mx_scale(D == 256 && word >= 4 ? s >> 8 : D == 256 ? s & 255u : s);
+  }
   __device__ __forceinline__ f16x8 eight(int word) const { return mx_eight(w[word], scale(word)); }
   // The piece's blocks that are NaN, or whose factor passes f16, as bits of the
   // row's blocks.
@@ -233,13 +299,22 @@ struct Piece {
 // in that order: values go through LDS as f16 rows and come back transposed,
 // four keys a read.  The running maximum moves only when a score passes it by
 // 2^8, so that most steps leave the sums as they are.
+constexpr int kChunk = 64;  // keys a step
+// A wave's accesses of its own LDS before here go before those behind.
+__device__ __forceinline__ void own_lds() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+constexpr int split_row(int d) { return d * 2 + 32; }  // bytes in LDS: four rows side by side meet no bank twice
 template <int D>
-__global__ __launch_bounds__(64) void attention_split_kernel(KvArgs a, AttnArgs g, SplitArgs p) {
-  constexpr int kRow = D * 2 + 32;  // bytes of a row in LDS: four rows side by side meet no bank twice
-  __shared__ __align__(16) uint8_t vt[32 * kRow];
-  const int lane = threadIdx.x, col = lane & 15, quad = lane >> 4;
+__device__ __forceinline__ bool attend_split(const KvArgs& a, const AttnArgs& g, const SplitArgs& p, int id, uint8_t* vt) {
+  constexpr int kRow = split_row(D);
+  const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
   Split s;
-  if (!plan(a, g, p, blockIdx.x, &s)) return;
+  int joined;
+  const bool have = plan<false>(a, g, p, id, &s, &joined);
+  if (lane == 0) note_item(p, id, s, have, joined);
+  if (!have) return false;
   // this lane's query
   const int within = p.tile_tokens > 1 ? col / p.group : 0;
   const int head = s.head + (p.tile_tokens > 1 ? col - within * p.group : col);
@@ -272,12 +347,12 @@ __global__ __launch_bounds__(64) void attention_split_kernel(KvArgs a, AttnArgs 
   float m = -INFINITY, l = 0.0f;  // the scores' reference (unscaled), the sum over this lane's keys
   uint32_t nan_blocks = 0;
   const int j0 = (from & ~15) + s.first * kChunk;
-  const int steps = min(s.chunks, (most - j0 + kChunk - 1) / kChunk);
+  const int steps = min(s.steps, (most - j0 + kChunk - 1) / kChunk);
   const int32_t* table = a.table + (size_t)s.seq * a.max_pages;
   const int mask = (1 << a.page_shift) - 1;
   int pages = -1;
   Piece<D> k[4], v[4];
-  uint32_t have = 0;  // tiles of 16 keys that lie on a page of the cache
+  uint32_t paged = 0;  // tiles of 16 keys that lie on a page of the cache
   auto load = [&](int step, Piece<D>* kk, Piece<D>* vv) {
     uint32_t ok = 0;
     if ((step & 15) == 0) {  // the pages of 64 tiles, one a lane
@@ -298,7 +373,7 @@ __global__ __launch_bounds__(64) void attention_split_kernel(KvArgs a, AttnArgs 
     }
     return ok;
   };
-  if (steps > 0) have = load(0, k, v);
+  if (steps > 0) paged = load(0, k, v);
   for (int step = 0; step < steps; ++step) {
     Piece<D> kn[4], vn[4];
     uint32_t next = 0;
@@ -311,12 +386,11 @@ __global__ __launch_bounds__(64) void attention_split_kernel(KvArgs a, AttnArgs 
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) t[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[u].eight(i), q[i], t[u], 0, 0, 0);
     }
-    uint32_t see = 0xFFFFu;
-    if (have != 15u || j + kChunk > every || j < all_from) {  // the same for the whole wave
-      see = 0;
+    if (paged != 15u || j + kChunk > every || j < all_from) {  // the same for the whole wave
+      uint32_t see = 0;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const bool there = have >> u & 1;
+        const bool there = paged >> u & 1;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int key = j + u * 16 + quad * 4 + r;
@@ -361,22 +435,21 @@ __global__ __launch_bounds__(64) void attention_split_kernel(KvArgs a, AttnArgs 
     for (int u = 0; u < 4; ++u) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float e = __builtin_amdgcn_exp2f(fmaf(t[u][r], g.scale, -ref));
-        e = see >> (u * 4 + r) & 1 ? e : 0.0f;
+        const float e = __builtin_amdgcn_exp2f(fmaf(t[u][r], g.scale, -ref));  // 0 for a masked one
         l += e;
         pr[u >> 1][(u & 1) * 4 + r] = (_Float16)e;
       }
     }
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      __syncthreads();
+      own_lds();
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         f16x8* dst = (f16x8*)(vt + (u * 16 + (lane >> 2)) * kRow + (lane & 3) * (D / 2));
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) dst[i] = v[half * 2 + u].eight(i);
       }
-      __syncthreads();
+      own_lds();
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
         // a group of 16 lanes reads 4 keys x 16 elements; lane e of it gets element e of the four
@@ -391,7 +464,7 @@ __global__ __launch_bounds__(64) void attention_split_kernel(KvArgs a, AttnArgs 
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) k[u] = kn[u], v[u] = vn[u];
-    have = next;
+    paged = next;
   }
   l = sum_of_rows(l);
   nan_blocks |= __shfl_xor(nan_blocks, 16);
@@ -401,11 +474,8 @@ __global__ __launch_bounds__(64) void attention_split_kernel(KvArgs a, AttnArgs 
     for (int i = 0; i < D / 16; ++i)
       if (nan_blocks >> (i / 2) & 1) o[i] = f32x4{NAN, NAN, NAN, NAN};
   }
-  if (s.index == 0 && lane == 0)
-    p.items[(size_t)s.token * a.kv_heads * p.head_tiles + s.kv_head * p.head_tiles +
-            (s.head - s.kv_head * p.group) / 16] = make_int2((int)blockIdx.x, s.of);
   if (s.of == 1) {
-    if (!real) return;
+    if (!real) return true;
     uint16_t* y = g.y + ((size_t)(s.token + within) * g.heads + head) * D + quad * 4;
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -415,144 +485,152 @@ __global__ __launch_bounds__(64) void attention_split_kernel(KvArgs a, AttnArgs 
       h.z = narrow<uint16_t>(o[i][2] * f), h.w = narrow<uint16_t>(o[i][3] * f);
       *(ushort4*)(y + i * 16) = h;
     }
-    return;
+    return true;
   }
-  if (!real) return;
-  float* out = p.sums + ((size_t)blockIdx.x * p.rows + col) * D + quad * 4;
+  const int slot = s.slot + s.index;
+  if (!real || (uint32_t)slot >= (uint32_t)p.slots) return true;
+  float* out = p.sums + ((size_t)slot * p.rows + col) * D + quad * 4;
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) *(f32x4*)(out + i * 16) = o[i];
-  if (quad == 0)
-    p.stats[(size_t)blockIdx.x * p.rows + col] = make_float2(m == -INFINITY ? -INFINITY : m * g.scale, l);
+  if (quad == 0) p.stats[(size_t)slot * p.rows + col] = make_float2(m == -INFINITY ? -INFINITY : m * g.scale, l);
+  return true;
+}
+
+template <int D>
+__global__ __launch_bounds__(64) void attention_split_kernel(KvArgs a, AttnArgs g, SplitArgs p) {
+  __shared__ __align__(16) uint8_t vt[32 * split_row(D)];
+  attend_split<D>(a, g, p, blockIdx.x, vt);
 }
 
 constexpr int kJoinSplits = 1024;
 
-// Joins the splits of an item, where it has several: a workgroup for each of
-// its rows, D / 4 threads a split, so that J = 512 reads 8 to 32 splits at a time;
+// Joins the splits of an item: a workgroup for some of its rows, one after the
+// other, D / 4 threads a split, so that J = 512 reads 8 to 32 splits at a time;
 // the threads' sums meet in LDS in a fixed order.
 template <int D, int J>
-__global__ __launch_bounds__(J) void attention_join_kernel(KvArgs a, AttnArgs g, SplitArgs p) {
+__device__ __forceinline__ void join_rows(const AttnArgs& g, const SplitArgs& p, int4 item, int from) {
   constexpr int kWide = J / (D / 4);  // splits at a time
-  __shared__ int found;
-  __shared__ float weight[kJoinSplits], part[J / 64];
+  __shared__ float weight[kJoinSplits], part[2][J / 64];
   __shared__ f32x4 sums[J];
-  const int tid = threadIdx.x, t = blockIdx.x, hh = blockIdx.y, col = blockIdx.z;
-  const int seq = sequence_of(a.start, a.batch, t, &found);
-  if (seq >= a.batch || t < a.start[seq]) return;
-  if ((t - max(a.start[seq], 0)) % p.tile_tokens) return;
-  const int within = p.tile_tokens > 1 ? col / p.group : 0, kv_head = hh / p.head_tiles;
-  const int head = kv_head * p.group + (hh - kv_head * p.head_tiles) * 16 + col - within * p.group;
-  if (head >= (kv_head + 1) * p.group || t + within >= min(a.start[seq + 1], a.tokens)) return;
-  const int2 item = p.items[((size_t)t * a.kv_heads) * p.head_tiles + hh];
-  if (item.y <= 1 || item.x < 0 || item.x >= p.splits || item.y > p.splits - item.x) return;
-  const float2* stats = p.stats + (size_t)item.x * p.rows + col;
-  float m = -INFINITY;
-  for (int i = tid; i < item.y; i += J) m = fmaxf(m, stats[(size_t)i * p.rows].x);
-  for (int i = 1; i < 64; i *= 2) m = fmaxf(m, __shfl_xor(m, i));
-  if ((tid & 63) == 0) part[tid >> 6] = m;
-  __syncthreads();
+  const int tid = threadIdx.x;
+  const int splits = item.y & 0xFFFFFF, count = (int)((uint32_t)item.y >> 24);
+  // lists that overlap may have left an entry unwritten
+  if (splits <= 1 || item.x < 0 || item.x > p.slots - splits || item.z < 0 || item.w < 0) return;
+  for (int col = from; col < p.rows; col += gridDim.y) {
+    const int within = p.tile_tokens > 1 ? col / p.group : 0, head = item.w + col - within * p.group;
+    if (within >= count || head >= (item.w / p.group + 1) * p.group) return;  // nor are the rows behind it
+    if (item.z >= g.tokens - within || head >= g.heads) return;
+    const float2* stats = p.stats + (size_t)item.x * p.rows + col;
+    float m = -INFINITY;
+    for (int i = tid; i < splits; i += J) m = fmaxf(m, stats[(size_t)i * p.rows].x);
+    for (int i = 1; i < 64; i *= 2) m = fmaxf(m, __shfl_xor(m, i));
+    __syncthreads();  // the row before is done
+    if ((tid & 63) == 0) part[0][tid >> 6] = m;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < J / 64; ++i) m = fmaxf(m, part[i]);
-  const float ref = m == -INFINITY ? 0.0f : m;
-  const int at = tid % (D / 4), lane = tid / (D / 4);
-  const float* src = p.sums + ((size_t)item.x * p.rows + col) * D + at * 4;
-  f32x4 o = {};
-  float l = 0.0f;
-  for (int i0 = 0; i0 < item.y; i0 += kJoinSplits) {
-    const int n = min(kJoinSplits, item.y - i0);
-    __syncthreads();
-    for (int i = tid; i < n; i += J) {
-      const float2 st = stats[(size_t)(i0 + i) * p.rows];
-      const float w = __builtin_amdgcn_exp2f(st.x - ref);
-      weight[i] = w;
-      l = fmaf(w, st.y, l);
-    }
-    __syncthreads();
+    for (int i = 0; i < J / 64; ++i) m = fmaxf(m, part[0][i]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    const int at = tid % (D / 4), lane = tid / (D / 4);
+    const float* src = p.sums + ((size_t)item.x * p.rows + col) * D + at * 4;
+    f32x4 o = {};
+    float l = 0.0f;
+    for (int i0 = 0; i0 < splits; i0 += kJoinSplits) {
+      const int n = min(kJoinSplits, splits - i0);
+      __syncthreads();
+      for (int i = tid; i < n; i += J) {
+        const float2 st = stats[(size_t)(i0 + i) * p.rows];
+        const float w = __builtin_amdgcn_exp2f(st.x - ref);
+        weight[i] = w;
+        l = fmaf(w, st.y, l);
+      }
+      __syncthreads();
 #pragma unroll 4
-    for (int i = lane; i < n; i += kWide) o += weight[i] * *(const f32x4*)(src + (size_t)(i0 + i) * p.rows * D);
+      for (int i = lane; i < n; i += kWide) o += weight[i] * *(const f32x4*)(src + (size_t)(i0 + i) * p.rows * D);
+    }
+    for (int i = 1; i < 64; i *= 2) l += __shfl_xor(l, i);
+    if ((tid & 63) == 0) part[1][tid >> 6] = l;
+    sums[tid] = o;
+    __syncthreads();
+    if (tid >= D / 4) continue;
+    l = part[1][0];
+#pragma unroll
+    for (int i = 1; i < J / 64; ++i) l += part[1][i];
+#pragma unroll
+    for (int i = 1; i < kWide; ++i) o += sums[i * (D / 4) + tid];
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    ushort4 h;
+    h.x = narrow<uint16_t>(o[0] * f), h.y = narrow<uint16_t>(o[1] * f);
+    h.z = narrow<uint16_t>(o[2] * f), h.w = narrow<uint16_t>(o[3] * f);
+    *(ushort4*)(g.y + ((size_t)(item.z + within) * g.heads + head) * D + tid * 4) = h;
   }
-  for (int i = 1; i < 64; i *= 2) l += __shfl_xor(l, i);
-  __syncthreads();
-  if ((tid & 63) == 0) part[tid >> 6] = l;
-  sums[tid] = o;
-  __syncthreads();
-  if (tid >= D / 4) return;
-  l = part[0];
-#pragma unroll
-  for (int i = 1; i < J / 64; ++i) l += part[i];
-#pragma unroll
-  for (int i = 1; i < kWide; ++i) o += sums[i * (D / 4) + tid];
-  const float f = l == 0.0f ? 0.0f : 1.0f / l;
-  ushort4 h;
-  h.x = narrow<uint16_t>(o[0] * f), h.y = narrow<uint16_t>(o[1] * f);
-  h.z = narrow<uint16_t>(o[2] * f), h.w = narrow<uint16_t>(o[3] * f);
-  *(ushort4*)(g.y + ((size_t)(t + within) * g.heads + head) * D + tid * 4) = h;
+}
+
+template <int D, int J>
+__global__ __launch_bounds__(J) void attention_join_kernel(AttnArgs g, SplitArgs p) {
+  // the entry need not wait for their number
+  const int4 item = p.table[1 + blockIdx.x];
+  if ((int)blockIdx.x < p.table[0].x) join_rows<D, J>(g, p, item, blockIdx.y);
+}
+
+// Those of both forms.
+template <int D>
+__global__ __launch_bounds__(64) void attention_join_both_kernel(AttnArgs g, SplitArgs one, SplitArgs two) {
+  const int n_one = one.slots ? min(one.table[0].x, one.joined) : 0, n_two = two.slots ? min(two.table[0].x, two.joined) : 0;
+  for (int i = blockIdx.x; i < n_one; i += gridDim.x) join_rows<D, 64>(g, one, one.table[1 + i], blockIdx.y);
+  for (int i = blockIdx.x; i < n_two; i += gridDim.x) join_rows<D, 64>(g, two, two.table[1 + i], blockIdx.y);
 }
 
 // --- many new tokens ---------------------------------------------------------------
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+constexpr int tile_keys(int d) { return d == 256 ? 32 : 64; }  // keys a step
+
 // A tile of up to 128 rows (new tokens of a sequence x heads of a kv head) over
-// all of its keys, 32 rows a wave.
+// all of its keys or a split of them, 32 rows a wave.
 //
 // KT keys a step: a thread widens a quarter of a key's and of a value's row to
 // f16 (their packed form was loaded a step before) and writes it to LDS, where
 // the four waves read it: the conversion, not the bytes, would bound the
-// kernel if each wave made its own.  S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16 matrix instructions:
-// the first's result leaves a lane keys of one row that are the second's B
-// operand as they stand, if V^T takes the keys in that order, which
-// transposing reads of LDS give it.  Two workgroups fit a CU up to d = 128, so
-// that one's exponentials run beside the other's products.  4,096 causal tokens
-// of 32 heads over 8 kv heads, d = 128: 193 us, 710 TFLOP/s (466 us as a wave
-// for each 16 rows); the exponentials and conversions take as long as the
-// products there.
+// kernel if each wave made its own.  S^T = K Q^T and O^T += V^T P^T on
+// 32 x 32 x 16 matrix instructions: the first's result leaves a lane keys of
+// one row that are the second's B operand as they stand, if V^T takes the keys
+// in that order, which transposing reads of LDS give it.  Two workgroups fit a
+// CU up to d = 128, so that one's exponentials run beside the other's products.
+//
+// 4,096 causal tokens of 32 heads over 8 kv heads, d = 128: 184 us, 747 TFLOP/s;
+// 512 of them after 32,768 keys 335 us, 814 TFLOP/s.  The exponentials and
+// conversions take longer than the products there.
+//
+// Sequences of few rows, whose splits are a wave's, take the workgroups behind
+// the tiles'.
 template <int D>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(KvArgs a, AttnArgs g, int tile_tokens, int tiles_most) {
-  constexpr int KT = D == 256 ? 32 : 64;
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(KvArgs a, AttnArgs g, SplitArgs p,
+                                                                                SplitArgs few) {
+  constexpr int KT = tile_keys(D);
   constexpr int kKeyRow = D * 2 + 16, kValueRow = D * 2 + 32;  // bytes: no bank twice for the lanes of a read
   constexpr int kBuffer = KT * (kKeyRow + kValueRow);
   extern __shared__ __align__(16) uint8_t lds[];
   __shared__ uint32_t nan_lds[2][KT];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = lane & 31, half = lane >> 5;
-  const int group = g.heads / a.kv_heads, kv_head = blockIdx.x % a.kv_heads;
-  // the tiles with the most keys, a sequence's last, go first
-  int tile = tiles_most - 1 - blockIdx.x / a.kv_heads;
-  int seq = -1, start = 0, count = 0;
-  for (int b0 = 0, before = 0; b0 < a.batch; b0 += 64) {
-    const int b = b0 + lane;
-    int t0 = 0, n = 0;
-    if (b < a.batch) {
-      t0 = max(a.start[b], 0);
-      n = max(min(a.start[b + 1], a.tokens) - t0, 0);
-    }
-    const int tiles = (n + tile_tokens - 1) / tile_tokens;
-    int upto = tiles;
-    for (int i = 1; i < 64; i *= 2) {
-      const int v = __shfl_up(upto, i);
-      if (lane >= i) upto += v;
-    }
-    const unsigned long long hit = __ballot(tile >= before + upto - tiles && tile < before + upto);
-    if (hit) {
-      const int src = __ffsll(hit) - 1;
-      seq = b0 + src;
-      tile = __builtin_amdgcn_readfirstlane(tile - before - __shfl(upto - tiles, src));
-      start = __builtin_amdgcn_readfirstlane(__shfl(t0, src));
-      count = __builtin_amdgcn_readfirstlane(__shfl(n, src));
-      break;
-    }
-    before += __shfl(upto, 63);
+  if ((int)blockIdx.x >= p.splits) {  // sequences of few rows
+    for (int id = ((int)blockIdx.x - p.splits) * 4 + wave; id < few.splits; id += ((int)gridDim.x - p.splits) * 4)
+      if (!attend_split<D>(a, g, few, id, lds + wave * 32 * split_row(D))) break;
+    return;
   }
-  if (seq < 0) return;
-  const long long table_keys = (long long)a.max_pages << a.page_shift;
-  const long long raw = a.len[seq], len = min(max(raw, 0ll), table_keys);
-  const int skip = tile * tile_tokens, mine = min(count - skip, tile_tokens);
-  const long long pos0 = raw - count + skip, pos1 = pos0 + mine - 1;
+  // a sequence's last tiles, which see the most keys, go first
+  Split s;
+  int joined;
+  const bool have = plan<true>(a, g, p, blockIdx.x, &s, &joined);
+  if (tid == 0) note_item(p, blockIdx.x, s, have, joined);
+  if (!have) return;
+  const int kv_head = s.kv_head, seq = s.seq, start = s.token;
+  const long long len = s.len, pos0 = s.pos, pos1 = pos0 + s.count - 1;
   // this lane's row
-  const int r = wave * 32 + row, within = r / group, head = kv_head * group + r - within * group;
-  const bool real = within < mine;
-  const int token = start + skip + within;
+  const int r = wave * 32 + row, within = r / p.group, head = s.head + r - within * p.group;
+  const bool real = within < s.count;
+  const int token = start + within;
   const long long pos = pos0 + within;
   const int hi = !real ? 0 : (int)(g.causal ? max(0ll, min(len, pos + 1)) : len);
   const int lo = !real || g.window <= 0 ? 0 : (int)max(0ll, pos - g.window + 1);
@@ -577,7 +655,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(K
   f32x16 o[D / 32] = {};
   float m = -INFINITY, l = 0.0f;
   uint32_t nan_blocks = 0;
-  const int j0 = from & ~15, steps = (most - j0 + KT - 1) / KT;
+  const int j0 = (from & ~15) + s.first * KT, steps = min(s.steps, (most - j0 + KT - 1) / KT);
   const int32_t* table = a.table + (size_t)seq * a.max_pages;
   const int mask = (1 << a.page_shift) - 1;
   // the page of key `lane` of a step, or -1
@@ -660,9 +738,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(K
         t[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q[i], t[u], 0, 0, 0);
       }
     }
-    uint32_t see = ~0u;
     if (!whole(step, there)) {
-      see = 0;
+      uint32_t see = 0;
 #pragma unroll
       for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
@@ -696,15 +773,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(K
     }
     // 2^6 times: a p of 2^-20 of the largest is still a normal f16 number
     const float ref = (m == -INFINITY ? 0.0f : m * g.scale) - 6.0f;
-    f16x8 p[KT / 16];
+    f16x8 pr[KT / 16];
 #pragma unroll
     for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        float x = __builtin_amdgcn_exp2f(fmaf(t[u][e], g.scale, -ref));
-        x = see >> (u * 16 + e) & 1 ? x : 0.0f;
+        const float x = __builtin_amdgcn_exp2f(fmaf(t[u][e], g.scale, -ref));  // 0 for a masked one
         l += x;
-        p[u * 2 + e / 8][e % 8] = (_Float16)x;
+        pr[u * 2 + e / 8][e % 8] = (_Float16)x;
       }
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
@@ -718,7 +794,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(K
         const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)src);
         const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(src + 8 * kValueRow));
         const s16x8 xy = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, xy), p[u], o[i], 0, 0, 0);
+        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, xy), pr[u], o[i], 0, 0, 0);
       }
     there = there_next;
     there_next = there_after;
@@ -727,6 +803,21 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(K
   l += __shfl_xor(l, 32);
   nan_blocks |= __shfl_xor(nan_blocks, 32);
   if (!real) return;
+  if (s.of > 1) {
+    const int slot = s.slot + s.index;
+    if ((uint32_t)slot >= (uint32_t)p.slots) return;
+    float* out = p.sums + ((size_t)slot * p.rows + r) * D + half * 4;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f32x4 v = {o[i][e * 4], o[i][e * 4 + 1], o[i][e * 4 + 2], o[i][e * 4 + 3]};
+        if (nan_blocks >> i & 1) v = f32x4{NAN, NAN, NAN, NAN};
+        *(f32x4*)(out + i * 32 + e * 8) = v;
+      }
+    if (half == 0) p.stats[(size_t)slot * p.rows + r] = make_float2(m == -INFINITY ? -INFINITY : m * g.scale, l);
+    return;
+  }
   uint16_t* y = g.y + ((size_t)token * g.heads + head) * D + half * 4;
   const float f = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -754,72 +845,99 @@ void launch_kv_append(hipStream_t st, const KvArgs& a, const void* k, size_t k_s
 namespace {
 
 template <int D>
-void launch_tiles(hipStream_t st, const KvArgs& a, const AttnArgs& g) {
-  constexpr int kKeys = D == 256 ? 32 : 64, kLds = 2 * kKeys * (D * 4 + 48);
-  const int tile_tokens = 128 / (g.heads / a.kv_heads), tiles = std::min(a.tokens, a.tokens / tile_tokens + a.batch);
-  hipLaunchKernelGGL(attention_tile_kernel<D>, dim3((unsigned)(tiles * a.kv_heads)), dim3(256), kLds, st, a, g,
-                     tile_tokens, tiles);
-}
-
-template <int D>
-void launch_splits(hipStream_t st, const KvArgs& a, const AttnArgs& g, const SplitArgs& p) {
-  // Rows of few splits are many: a wave each then.
-  const dim3 rows((unsigned)a.tokens, (unsigned)(a.kv_heads * p.head_tiles), (unsigned)p.rows);
-  const bool few = (long long)a.tokens * g.heads <= 512;
-  hipLaunchKernelGGL(attention_split_kernel<D>, dim3((unsigned)p.splits), dim3(64), 0, st, a, g, p);
-  if (!p.join) return;  // a split takes all keys that the table has room for
-  if (few)
-    hipLaunchKernelGGL((attention_join_kernel<D, 512>), rows, dim3(512), 0, st, a, g, p);
+void launch_parts(hipStream_t st, const KvArgs& a, const AttnArgs& g, const AttnPlan& p) {
+  if (p.tiles.splits) {
+    constexpr int kLds = std::max(2 * tile_keys(D) * (D * 4 + 48), 4 * 32 * split_row(D));
+    const unsigned grid = p.tiles.splits + std::min((p.few.splits + 3) / 4, 1024);
+    hipLaunchKernelGGL(attention_tile_kernel<D>, dim3(grid), dim3(256), kLds, st, a, g, p.tiles, p.few);
+  } else {
+    hipLaunchKernelGGL(attention_split_kernel<D>, dim3((unsigned)p.few.splits), dim3(64), 0, st, a, g, p.few);
+  }
+  if (!p.tiles.slots && !p.few.slots) return;
+  // rows of few splits are many: a wave each then, or for eight of a tile's
+  const dim3 grid(p.few.joined, p.few.rows);
+  if (p.tiles.splits)
+    hipLaunchKernelGGL(attention_join_both_kernel<D>, dim3(256, 16), dim3(64), 0, st, g, p.tiles, p.few);
+  else if ((long long)a.tokens * g.heads > 512)
+    hipLaunchKernelGGL((attention_join_kernel<D, 64>), grid, dim3(64), 0, st, g, p.few);
   else
-    hipLaunchKernelGGL((attention_join_kernel<D, 64>), rows, dim3(64), 0, st, a, g, p);
+    hipLaunchKernelGGL((attention_join_kernel<D, 512>), grid, dim3(512), 0, st, g, p.few);
 }
 
 }  // namespace
 
-size_t attention_space(const KvArgs& a, const AttnArgs& g, SplitArgs* p) {
-  p->group = g.heads / a.kv_heads;
-  // Whole tiles are faster where there are enough of them, and full: 512 new
-  // tokens of 32 heads 24 us, 53 us split; 256 of them after 8,192 keys (64
-  // tiles, 8,192 rows) 250 us, 110 us split; 8 sequences of up to 64 after
-  // 2,048 keys 68 us, 31 us split.
-  p->whole = p->group <= 128 && (long long)a.tokens * g.heads >= 12288 &&
-             (long long)a.tokens * p->group >= 128ll * a.batch;
-  if (p->whole) return 0;
-  p->head_tiles = (p->group + 15) / 16;
-  p->tile_tokens = std::max(1, 16 / p->group);
-  const long long tiles = std::min<long long>(a.tokens, a.tokens / p->tile_tokens + (long long)a.batch);
-  const long long heads = (long long)a.kv_heads * p->head_tiles;
-  p->waves = 2048;
-  p->waves = a.d == 256 ? 1024 : 2048;  // that the chip holds at a time
-  // A split takes two steps of 64 keys or more, or all of them where joining
-  // would take longer: one sequence of 1,024 keys 12.2 us in splits of two, 20.9
-  // us in splits of eight; 64 of up to 512 17.5 us split, 14.1 us whole.
-  const int steps = ((a.max_pages << a.page_shift) + kChunk - 1) / kChunk;  // of the longest sequence
-  p->join = steps > (tiles * heads >= 256 ? 8 : 4);
-  p->least = p->join ? 2 : 8;
-  p->splits = (int)(tiles * heads + p->waves + 1);
-  p->rows = std::min(16, p->group * p->tile_tokens);
-  p->stats_at = (size_t)p->splits * p->rows * a.d * 4;
-  p->items_at = p->stats_at + (size_t)p->splits * p->rows * 8;
-  return p->items_at + (size_t)a.tokens * heads * 8;
+size_t attention_space(const KvArgs& a, const AttnArgs& g, AttnPlan* plan) {
+  const int group = g.heads / a.kv_heads, longest = a.max_pages << a.page_shift;
+  const long long rows = (long long)a.tokens * group;
+  // Tiles of 128 rows do the work in half the time, tiles of 16 rows are done
+  // sooner where there is little of it: 8 sequences of up to 128 new tokens
+  // after 1,024 keys (32 heads over 8, d = 128) 47 us, 24 us in tiles of 16; 256
+  // new tokens after 8,192 (64 tiles x 128 steps) 78 us, 89 us; 512 after 8,192 116
+  // us, 161 us; 4,096 and as many keys 184 us, 317 us.
+  constexpr int kBigRows = 128, kBigSteps = 6144;
+  const bool tiles = group <= 128 && (double)rows * a.kv_heads / 128 * ((longest + 63) / 64) >= kBigSteps;
+  auto fill = [&](SplitArgs* p, int most_rows, int chunk, int waves, int whole, int least) {
+    p->big = tiles ? kBigRows : kNever;
+    p->big_tokens = tiles ? 128 / group : 1;
+    p->big_steps = kBigSteps;
+    p->group = group;
+    p->head_tiles = (group + most_rows - 1) / most_rows;
+    p->tile_tokens = std::max(1, most_rows / group);
+    p->rows = std::min(most_rows, group * p->tile_tokens);
+    p->chunk = chunk;
+    p->waves = waves;
+    p->whole = whole;
+    p->least = least;
+    const long long heads = (long long)a.kv_heads * p->head_tiles;
+    p->items = (int)(std::min<long long>(a.tokens, a.tokens / p->tile_tokens + (long long)a.batch) * heads);
+    // 16 and 64: the steps' sum is rounded
+    p->splits = p->items + waves + 16;
+    p->slots = (longest + chunk - 1) / chunk > least ? 2 * waves + 64 : 0;
+    p->joined = std::min(p->items, waves + 32);
+  };
+  const int many = a.d == 256 ? 1024 : 2048;  // waves that the chip holds at a time
+  // A split of 128 rows leaves 64 KiB of sums at d = 128: items are split where
+  // that shares them out over twice the workgroups or more (2 sequences of up to
+  // 1,536 new tokens after 4,096 keys 137 us, 179 us with splits for every
+  // uneven share), into eight steps or more.
+  if (tiles) fill(&plan->tiles, 128, tile_keys(a.d), many / 4, 2, 8 * 64 / tile_keys(a.d));
+  // A split of 16 rows takes two steps of 64 keys or more, or all of them where
+  // joining would take longer: one sequence of 1,024 keys 12.2 us in splits of
+  // two, 20.9 us in splits of eight; 64 of up to 512 17.5 us split, 14.1 us whole.
+  fill(&plan->few, 16, kChunk, many, 1, 2);
+  const int steps = (longest + kChunk - 1) / kChunk;
+  if (steps <= (plan->few.items >= 256 ? 8 : 4)) plan->few.least = 8, plan->few.slots = 0;
+  size_t bytes = 0;
+  int i = 0;
+  for (const SplitArgs* p : {&plan->tiles, &plan->few}) {
+    auto take = [&](size_t n) {
+      const size_t at = bytes;
+      bytes += (n + 255) / 256 * 256;
+      return at;
+    };
+    size_t* at = plan->at[i++];
+    if (!p->slots) continue;
+    at[0] = take((size_t)p->slots * p->rows * a.d * 4);
+    at[1] = take((size_t)p->slots * p->rows * 8);
+    at[2] = take((size_t)(p->joined + 1) * 16);
+  }
+  return bytes;
 }
 
-void launch_attention(hipStream_t st, const KvArgs& a, const AttnArgs& g, SplitArgs p, void* space) {
-  auto run = [&](auto d) {
-    constexpr int D = decltype(d)::value;
-    p.whole ? launch_tiles<D>(st, a, g) : launch_splits<D>(st, a, g, p);
-  };
-  if (!p.whole) {
-    p.sums = (float*)space;
-    p.stats = (float2*)((char*)space + p.stats_at);
-    p.items = (int2*)((char*)space + p.items_at);
+void launch_attention(hipStream_t st, const KvArgs& a, const AttnArgs& g, AttnPlan p, void* space) {
+  int i = 0;
+  for (SplitArgs* s : {&p.tiles, &p.few}) {
+    const size_t* at = p.at[i++];
+    s->sums = (float*)((char*)space + at[0]);
+    s->stats = (float2*)((char*)space + at[1]);
+    s->table = (int4*)((char*)space + at[2]);
   }
   if (a.d == 64)
-    run(std::integral_constant<int, 64>{});
+    launch_parts<64>(st, a, g, p);
   else if (a.d == 128)
-    run(std::integral_constant<int, 128>{});
+    launch_parts<128>(st, a, g, p);
   else
-    run(std::integral_constant<int, 256>{});
+    launch_parts<256>(st, a, g, p);
   DW_HIP(hipGetLastError());
 }
 

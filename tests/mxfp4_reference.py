@@ -126,8 +126,8 @@ class Cache:
         return decode(self.q[name][p, h, s], self.s[name][p, h, s], self.d)
 
 
-def attention(q, cache, scale, causal=True, window=0):
-    """y [tokens, heads, d] in f64 (NaN rows where no sequence owns them), and what the kernel may be off:
+def attention(q, cache, scale, causal=True, window=0, some=None):
+    """y [tokens, heads, d] in f64 (NaN rows where no sequence owns them, and where `some` [tokens, heads] is not), and what the kernel may be off:
     scores are f32 sums of d exact products, p rounds to f16 (2^-11, and 2^-25 absolute), sums of n terms in f32, the
     result to f16."""
     heads, d = q.shape[1], cache.d
@@ -147,6 +147,8 @@ def attention(q, cache, scale, causal=True, window=0):
             k, v = cache.rows("k", b, h // group), cache.rows("v", b, h // group)
             x = q[rows, h]
             for i, r in enumerate(rows):
+                if some is not None and not some[r, h]:
+                    continue
                 m = see[i]
                 if not m.any():
                     y[r, h], off[r, h] = 0, 0

@@ -213,7 +213,6 @@ def test_many_sequences_of_many_new_tokens(backend):
     kv = [n + int(x) for n, x in zip(nq, rng.integers(0, 60, 80))]
     c = ref.Cache(rng, nq, kv, 2, 64, 16)
     q = rng.normal(0, 1, (c.tokens, 16, 64)).astype(np.float16)
-    assert c.tokens * 16 >= 12288
     check(attend(backend, c, q, 0.125), *ref.attention(q.astype(np.float64), c, 0.125))
 
 
@@ -228,16 +227,15 @@ def test_many_heads_of_a_kv_head(backend, heads, kv_heads, nq):
 
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 100)])
-def test_prompts_of_whole_tiles(backend, d, causal, window):
+def test_prompts_of_many_heads(backend, d, causal, window):
     rng = np.random.default_rng(d + window)
     c = ref.Cache(rng, [260, 0, 131], [300, 20, 500], 2, d, 64, extra=2)
     q = rng.normal(0, 1, (c.tokens, 32, d)).astype(np.float16)
-    assert c.tokens * 32 >= 12288
     check(attend(backend, c, q, d ** -0.5, causal, window), *ref.attention(q.astype(np.float64), c, d ** -0.5, causal,
                                                                         window))
 
 
-def test_whole_tiles_with_bad_pages_nan_and_empty_rows(backend):
+def test_prompts_with_bad_pages_nan_and_empty_rows(backend):
     rng = np.random.default_rng(77)
     c = ref.Cache(rng, [300, 200], [280, 333], 1, 128, 16)
     for name, b, j, blk in (("v", 0, 250, 3), ("k", 0, 270, 1), ("v", 1, 300, 0)):
@@ -261,6 +259,124 @@ def test_whole_tiles_with_bad_pages_nan_and_empty_rows(backend):
     e = k @ q[r, h].astype(np.float64) * 0.1
     e = np.exp(e - e.max())
     np.testing.assert_allclose(got[r, h], e @ v / e.sum(), rtol=2.0 ** -10, atol=8 * 2.0 ** -11)
+
+
+def large(rng, nq, kv, heads, kv_heads, d, page, window=0, extra=0):
+    """A batch whose prompts are so long that tiles of 128 rows are used (6,144 steps of 64 keys), its queries, and some of
+    its rows: all of the first and last tokens of each sequence, and 2% of the others."""
+    c = ref.Cache(rng, nq, kv, kv_heads, d, page, extra=extra)
+    group = heads // kv_heads
+    tile = 128 // group
+    assert sum(-(-n // tile) * kv_heads * max(1, -(-min(k, window + tile + 14 if window else k) // 64))
+               for n, k in zip(nq, kv) if n * group >= 128) >= 6144
+    q = rng.normal(0, 1, (c.tokens, heads, d)).astype(np.float16)
+    some = rng.random((c.tokens, heads)) < 0.02
+    for b in range(c.batch):
+        some[c.start[b]:min(c.start[b] + 2, c.start[b + 1])] = True
+        some[max(c.start[b], c.start[b + 1] - 2):c.start[b + 1]] = True
+    return c, q, some
+
+
+def check_some(got, want, off, some, owned):
+    bad = ~((np.abs(got - want) <= off) | (np.isnan(got) & np.isnan(want)))[some]
+    assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:3], got[some][bad][:3], want[some][bad][:3])
+    assert (got[owned:] == 777).all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 1000)])
+def test_long_prompts_beside_single_tokens(backend, d, causal, window):
+    rng = np.random.default_rng(d + window)
+    nq, kv = [1300, 0, 1, 33, 1, 300, 15], [1400, 40, 2500, 2000, 1, 2100, 15]
+    c, q, some = large(rng, nq, kv, 32, 4, d, 64, window, extra=2)
+    some[-2:] = False
+    want, off = ref.attention(q.astype(np.float64), c, d ** -0.5, causal, window, some)
+    check_some(attend(backend, c, q, d ** -0.5, causal, window), want, off, some, c.start[-1])
+
+
+@pytest.mark.parametrize("heads,kv_heads,nq,kv", [(8, 8, 1000, 6200), (7, 1, 900, 8200), (40, 1, 200, 6000), (100, 1, 200, 2200),
+                                                  (128, 1, 190, 2100), (16, 1, 130, 24000)])
+def test_groups_of_long_prompts(backend, heads, kv_heads, nq, kv):
+    # the last: 17 tiles that split over their keys, and a single token's keys with them
+    rng = np.random.default_rng(heads)
+    c, q, some = large(rng, [nq, 1], [kv, 900], heads, kv_heads, 64, 32)
+    want, off = ref.attention(q.astype(np.float64), c, 0.125, some=some)
+    check_some(attend(backend, c, q, 0.125), want, off, some, c.start[-1])
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_tiles_split_over_keys(backend, d):
+    rng = np.random.default_rng(d)
+    c, q, some = large(rng, [240, 5, 40], [12000, 3000, 11000], 16, 1, d, 128)
+    want, off = ref.attention(q.astype(np.float64), c, d ** -0.5, some=some)
+    got = attend(backend, c, q, d ** -0.5)
+    check_some(got, want, off, some, c.start[-1])
+    for _ in range(3):
+        np.testing.assert_array_equal(attend(backend, c, q, d ** -0.5), got)
+
+
+def test_long_prompts_with_bad_pages_nan_and_empty_rows(backend):
+    rng = np.random.default_rng(77)
+    c, q, some = large(rng, [600, 200, 1], [580, 17000, 3000], 16, 1, 128, 16)
+    for name, b, j, blk in (("v", 0, 550, 3), ("k", 0, 570, 1), ("v", 1, 16950, 0), ("v", 2, 77, 2)):
+        c.s[name][c.table[b, j // 16], 0, j % 16, blk] = 255
+    # a factor past f16 where only some rows see the value, behind those that are compared
+    c.s["v"][c.table[1, 16990 // 16], 0, 16990 % 16, 1] = 200
+    some[790:800] = False
+    want, off = ref.attention(q.astype(np.float64), c, 0.1, some=some)
+    got = attend(backend, c, q, 0.1)
+    np.testing.assert_array_equal(np.isnan(got)[some], np.isnan(want)[some])
+    check_some(got, want, np.where(np.isnan(off), 0, off), some, c.start[-1])
+    assert (got[:20] == 0).all()  # the first 20 of 600 new tokens have no key among 580
+    # pages outside the cache: as if their keys were masked
+    bufs = put(backend, c)
+    table = c.table.copy()
+    table[1, 2], table[1, 700] = c.num_pages, -3
+    bufs[4] = backend.from_numpy(table)
+    got = attend(backend, c, q, 0.1, bufs=bufs)
+    r, h = 600 + 20, 5
+    j = np.array([x for x in range(17000 - 200 + 20 + 1) if x // 16 not in (2, 700)])
+    k, v = c.rows("k", 1, 0)[j], c.rows("v", 1, 0)[j]
+    e = k @ q[r, h].astype(np.float64) * 0.1
+    e = np.exp(e - e.max())
+    np.testing.assert_allclose(got[r, h], e @ v / e.sum(), rtol=2.0 ** -10, atol=8 * 2.0 ** -11)
+
+
+def test_growing_scores_of_a_long_prompt(backend):
+    rng = np.random.default_rng(7)
+    c, q, some = large(rng, [1000], [3200], 16, 1, 64, 16)
+    j = np.arange(3200)
+    x, s = ref.encode(np.full((1, 64), 6.0) * 2.0 ** (j[:, None] / 400 - 3), -23)
+    c.q["k"][c.table[0, j // 16], 0, j % 16], c.s["k"][c.table[0, j // 16], 0, j % 16] = x, s
+    q[:] = 1
+    q[:, 1::3] = -1
+    q[:, 2::3] = 0.01
+    want, off = ref.attention(q.astype(np.float64), c, 1.0, some=some)
+    check_some(attend(backend, c, q, 1.0), want, off, some, 1000)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1e-40])
+def test_scales_out_of_the_ordinary(backend, scale):
+    rng = np.random.default_rng(4)
+    c = ref.Cache(rng, [1, 30, 4], [90, 40, 3], 2, 64, 16)
+    q = rng.normal(0, 1, (c.tokens, 6, 64)).astype(np.float16)
+    check(attend(backend, c, q, scale), *ref.attention(q.astype(np.float64), c, scale))
+
+
+def test_lists_that_overlap_stay_in_bounds(backend):
+    # as many sequences as tokens, each of them all tokens: more work than a grid is made for
+    rng = np.random.default_rng(3)
+    c = ref.Cache(rng, [400] + [0] * 39, [4000] + [0] * 39, 1, 64, 16)
+    q = rng.normal(0, 1, (c.tokens, 16, 64)).astype(np.float16)
+    for first in (0, -7):
+        bufs = put(backend, c)
+        start = np.full(41, 400, np.int32)
+        start[:40:2] = first
+        bufs[5], bufs[6] = backend.from_numpy(start), backend.from_numpy(np.full(40, 4000, np.int32))
+        bufs[4] = backend.from_numpy(np.tile(c.table[:1], (40, 1)))
+        attend(backend, c, q, 0.1, bufs=bufs)
+        attend(backend, c, q[:, :2].copy(), 0.1, bufs=bufs)
+    backend.synchronize()
 
 
 def test_long_splits(backend):
