@@ -218,6 +218,10 @@ __device__ __forceinline__ void note_item(const SplitArgs& p, int id, const Spli
     p.table[1 + s.item] = make_int4(s.slot, s.of | s.count << 24, s.token, s.head);
 }
 
+// A value that all lanes have, in a scalar register (64-bit comparisons leave
+// vector ones).
+__device__ __forceinline__ int shared(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 __device__ __forceinline__ float max_of_rows(float v) {  // over the four lanes of a column
   v = fmaxf(v, __shfl_xor(v, 16));
   return fmaxf(v, __shfl_xor(v, 32));
@@ -239,7 +243,9 @@ __device__ __forceinline__ f16x8 mx_eight(uint32_t w, float scale) {
   return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// A lane's quarter of a row: D / 4 elements, their words and scale bytes.
+// A lane's quarter of a row: D / 4 elements, their words and scale bytes.  The
+// scales come in the 32 bits that hold them, and ready() takes them out where
+// the piece is used: done with the load, it would wait for it.
 template <int D>
 struct Piece {
   uint32_t w[D / 32];
@@ -249,17 +255,22 @@ struct Piece {
     if constexpr (D == 64) {
       const uint2 v = *(const uint2*)p;
       w[0] = v.x, w[1] = v.y;
-      s = scales[row * 2 + (quarter >> 1)];
+      s = ((const uint32_t*)scales)[row / 2];
     } else if constexpr (D == 128) {
       const uint4 v = *(const uint4*)p;
       w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-      s = scales[row * 4 + quarter];
+      s = ((const uint32_t*)scales)[row];
     } else {
       const uint4 v = *(const uint4*)p, u = *(const uint4*)(p + 4);
       w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
       w[4] = u.x, w[5] = u.y, w[6] = u.z, w[7] = u.w;
-      s = *(const uint16_t*)(scales + row * 8 + quarter * 2);
+      s = ((const uint32_t*)scales)[row * 2 + (quarter >> 1)];
     }
+  }
+  __device__ __forceinline__ void ready(int row, int quarter) {  // row: its last bit
+    if constexpr (D == 64) s = s >> ((row & 1) * 16 + (quarter >> 1) * 8) & 255u;
+    if constexpr (D == 128) s = s >> (quarter * 8) & 255u;
+    if constexpr (D == 256) s = s >> ((quarter & 1) * 16) & 0xFFFFu;
   }
   __device__ __forceinline__ float scale(int word) const {
     return mx_scale(D == 256 && word >= 4 ? s >> 8 : D == 256 ? s & 255u : s);
@@ -324,10 +335,10 @@ __device__ __forceinline__ bool attend_split(const KvArgs& a, const AttnArgs& g,
   const int hi = !real ? 0 : (int)(g.causal ? max(0ll, min(s.len, pos + 1)) : s.len);
   const int lo = !real || g.window <= 0 ? 0 : (int)max(0ll, pos - g.window + 1);
   const long long last = s.pos + s.count - 1;
-  const int most = (int)(g.causal ? max(0ll, min(s.len, last + 1)) : s.len);  // keys that some row sees: [from, most)
-  const int from = g.window > 0 ? (int)min((long long)most, max(0ll, s.pos - g.window + 1)) : 0;
-  const int every = (int)(g.causal ? max(0ll, min(s.len, s.pos + 1)) : s.len);  // that all rows see, up to here
-  const int all_from = g.window > 0 ? (int)max(0ll, last - g.window + 1) : 0;
+  const int most = shared((int)(g.causal ? max(0ll, min(s.len, last + 1)) : s.len));  // keys that some row sees: [from, most)
+  const int from = shared(g.window > 0 ? (int)min((long long)most, max(0ll, s.pos - g.window + 1)) : 0);
+  const int every = shared((int)(g.causal ? max(0ll, min(s.len, s.pos + 1)) : s.len));  // that all rows see, up to here
+  const int all_from = shared(g.window > 0 ? (int)max(0ll, last - g.window + 1) : 0);
   f16x8 q[D / 32];
   {
     const uint16_t* src = g.q + (size_t)(s.token + within) * g.q_stride + g.q_off + (size_t)head * D + quad * (D / 4);
@@ -363,7 +374,7 @@ __device__ __forceinline__ bool attend_split(const KvArgs& a, const AttnArgs& g,
     for (int u = 0; u < 4; ++u) {
       const int j = j0 + step * kChunk + u * 16;
       int page = __builtin_amdgcn_readlane(pages, (step * 4 + u) & 63);
-      if (page >= 0 && page < a.num_pages)
+      if ((uint32_t)page < (uint32_t)a.num_pages)
         ok |= 1u << u;
       else
         page = 0;
@@ -379,6 +390,8 @@ __device__ __forceinline__ bool attend_split(const KvArgs& a, const AttnArgs& g,
     uint32_t next = 0;
     if (step + 1 < steps) next = load(step + 1, kn, vn);
     const int j = j0 + step * kChunk;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) k[u].ready(col, quad), v[u].ready(lane >> 2, lane & 3);
     f32x4 t[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -586,6 +599,15 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int tile_keys(int d) { return d == 256 ? 32 : 64; }  // keys a step
 
+// All waves' accesses of LDS before here go before those behind; loads of global
+// memory stay in flight (__syncthreads would wait for them).
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // LDS alone
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // A tile of up to 128 rows (new tokens of a sequence x heads of a kv head) over
 // all of its keys or a split of them, 32 rows a wave.
 //
@@ -598,9 +620,11 @@ constexpr int tile_keys(int d) { return d == 256 ? 32 : 64; }  // keys a step
 // in that order, which transposing reads of LDS give it.  Two workgroups fit a
 // CU up to d = 128, so that one's exponentials run beside the other's products.
 //
-// 4,096 causal tokens of 32 heads over 8 kv heads, d = 128: 184 us, 747 TFLOP/s;
-// 512 of them after 32,768 keys 335 us, 814 TFLOP/s.  The exponentials and
-// conversions take longer than the products there.
+// 4,096 causal tokens of 32 heads over 8 kv heads, d = 128: 168 us, 815 TFLOP/s
+// (184 us before the scores went a step ahead, with LDS conflicts of the
+// values and without priorities).  The products take a third of that and the
+// vector instructions (exponentials, conversions) half; two waves a SIMD do
+// not hide all of either.
 //
 // Sequences of few rows, whose splits are a wave's, take the workgroups behind
 // the tiles'.
@@ -608,8 +632,13 @@ template <int D>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(KvArgs a, AttnArgs g, SplitArgs p,
                                                                                 SplitArgs few) {
   constexpr int KT = tile_keys(D);
-  constexpr int kKeyRow = D * 2 + 16, kValueRow = D * 2 + 32;  // bytes: no bank twice for the lanes of a read
-  constexpr int kBuffer = KT * (kKeyRow + kValueRow);
+  // Bytes of a row in LDS, such that lanes that go together meet no bank twice:
+  // a key's with 16 behind it; a value's 16-byte pieces stand at their index
+  // xor 5 s, for 4 rows beside each other that are read by 64 bytes each and
+  // written by 16.
+  constexpr int kKeyRow = D * 2 + 16, kValueRow = D * 2;
+  constexpr int kBuffer = KT * (kKeyRow + kValueRow), kReads = 3, kPairs = 4;
+  auto turned = [](int row) { return 5 * (D == 64 ? row >> 1 & 1 : row & 3); };
   extern __shared__ __align__(16) uint8_t lds[];
   __shared__ uint32_t nan_lds[2][KT];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -634,10 +663,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(K
   const long long pos = pos0 + within;
   const int hi = !real ? 0 : (int)(g.causal ? max(0ll, min(len, pos + 1)) : len);
   const int lo = !real || g.window <= 0 ? 0 : (int)max(0ll, pos - g.window + 1);
-  const int most = (int)(g.causal ? max(0ll, min(len, pos1 + 1)) : len);  // keys that some row sees: [from, most)
-  const int from = g.window > 0 ? (int)min((long long)most, max(0ll, pos0 - g.window + 1)) : 0;
-  const int every = (int)(g.causal ? max(0ll, min(len, pos0 + 1)) : len);  // that all rows see, up to here
-  const int all_from = g.window > 0 ? (int)max(0ll, pos1 - g.window + 1) : 0;
+  const int most = shared((int)(g.causal ? max(0ll, min(len, pos1 + 1)) : len));  // keys that some row sees: [from, most)
+  const int from = shared(g.window > 0 ? (int)min((long long)most, max(0ll, pos0 - g.window + 1)) : 0);
+  const int every = shared((int)(g.causal ? max(0ll, min(len, pos0 + 1)) : len));  // that all rows see, up to here
+  const int all_from = shared(g.window > 0 ? (int)max(0ll, pos1 - g.window + 1) : 0);
   f16x8 q[D / 16];
   {
     const uint16_t* src = g.q + (size_t)(real ? token : start) * g.q_stride + g.q_off + (size_t)head * D + half * 8;
@@ -653,153 +682,219 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(K
     }
   }
   f32x16 o[D / 32] = {};
-  float m = -INFINITY, l = 0.0f;
+  float m = -INFINITY, l = 0.0f, l1 = 0.0f;
   uint32_t nan_blocks = 0;
-  const int j0 = (from & ~15) + s.first * KT, steps = min(s.steps, (most - j0 + KT - 1) / KT);
+  const int j0 = shared((from & ~15) + s.first * KT), steps = shared(min(s.steps, (most - j0 + KT - 1) / KT));
   const int32_t* table = a.table + (size_t)seq * a.max_pages;
   const int mask = (1 << a.page_shift) - 1;
   // the page of key `lane` of a step, or -1
   auto page_of = [&](int step) {
     const long long j = (long long)j0 + (long long)step * KT + lane;
-    const int page = lane < KT && j < most ? table[j >> a.page_shift] : -1;
-    return page < a.num_pages ? page : -1;
+    return lane < KT && j < most ? table[j >> a.page_shift] : -1;
   };
+  auto on_page = [&](int page) { return (uint32_t)page < (uint32_t)a.num_pages; };
   // this thread's part of the widening: a quarter of one key's row
   const bool does_k = KT == 64 || wave < 2, does_v = KT == 64 || wave >= 2;
   const int key = (tid >> 2) % KT, quarter = tid & 3;
   Piece<D> k, v;
-  auto fetch = [&](int step, int pages) {
+  auto row_of = [&](int step, int pages) {
     const int j = j0 + step * KT + key;
-    const int page = max(__shfl(pages, key), 0);  // a key on no page is seen by no row: any row's bytes will do
-    const size_t at = (((size_t)page * a.kv_heads + kv_head) << a.page_shift) + (j & mask);
-    if (does_k) k.load(a.kc, a.ks, at, quarter);
-    if (does_v) v.load(a.vc, a.vs, at, quarter);
+    int page = __shfl(pages, key);
+    page = on_page(page) ? page : 0;  // a key on no page is seen by no row: any row's bytes will do
+    return (((size_t)page * a.kv_heads + kv_head) << a.page_shift) + (j & mask);
+  };
+  // kept from being added to the four bases ahead of the loop, whose registers
+  // would push others to memory
+  auto anew = [](int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+  };
+  auto fetch_k = [&](Piece<D>& to, int step, int pages) {
+    const size_t at = row_of(step, pages);
+    if (does_k) to.load(a.kc, a.ks, at, anew(quarter));
+  };
+  auto fetch_v = [&](int step, int pages) {
+    const size_t at = row_of(step, pages);
+    if (does_v) v.load(a.vc, a.vs, at, anew(quarter));
   };
   auto whole = [&](int step, unsigned long long there) {
     const int j = j0 + step * KT;
     return there == ~0ull >> (64 - KT) && j + KT <= every && j >= all_from;
   };
-  auto widen_to = [&](int step, unsigned long long there) {
-    uint8_t* kb = lds + (step & 1) * kBuffer + key * kKeyRow + quarter * (D / 2);
-    uint8_t* vb = lds + (step & 1) * kBuffer + KT * kKeyRow + key * kValueRow + quarter * (D / 2);
-    if (does_k) {
+  // Values that no row sees must not reach the sums, whatever they hold, nor
+  // those that only some see, if they are NaN.
+  auto clean_v = [&](int step, unsigned long long there) {
+    if (!does_v || whole(step, there)) return;
+    const int j = j0 + step * KT + key;
+    if (!(there >> key & 1) || j >= most || j < from) v.clear();
+    const uint32_t own = v.nan_bits(quarter);
+    uint32_t bits = own | __shfl_xor(own, 1);
+    bits |= __shfl_xor(bits, 2);
+    if (own) v.clear_nan();
+    if (quarter == 0) nan_lds[step & 1][key] = bits;
+  };
+  auto widen_k = [&](const Piece<D>& piece, int step, int i) {
+    if (does_k)
+      *(f16x8*)(lds + (step & 1) * kBuffer + key * kKeyRow + quarter * (D / 2) + i * 16) = piece.eight(i);
+  };
+  auto widen_v = [&](int step, int i) {
+    if (does_v)
+      *(f16x8*)(lds + (step & 1) * kBuffer + KT * kKeyRow + key * kValueRow +
+                (((quarter * (D / 32) + i) ^ turned(key)) * 16)) = v.eight(i);
+  };
+  // Scores of 32 keys, with other work beside each product.
+  auto scores = [&](int step, int u, f32x16& t, auto beside) {
+    const uint8_t* kb = lds + (step & 1) * kBuffer + (u * 32 + row) * kKeyRow + half * 16;
+    f16x8 x[D / 16];
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) *(f16x8*)(kb + i * 16) = k.eight(i);
-    }
-    if (does_v) {
-      if (!whole(step, there)) {
-        // values that no row sees must not reach the sums, whatever they hold,
-        // nor those that only some see, if they are NaN
-        const int j = j0 + step * KT + key;
-        if (!(there >> key & 1) || j >= most || j < from) v.clear();
-        const uint32_t own = v.nan_bits(quarter);
-        uint32_t bits = own | __shfl_xor(own, 1);
-        bits |= __shfl_xor(bits, 2);
-        if (own) v.clear_nan();
-        if (quarter == 0) nan_lds[step & 1][key] = bits;
-      }
+    for (int i = 0; i < kReads; ++i) x[i] = *(const f16x8*)(kb + i * 32);
+    t = f32x16{};
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) *(f16x8*)(vb + i * 16) = v.eight(i);
+    for (int i = 0; i < D / 16; ++i) {
+      if (i + kReads < D / 16) x[i + kReads] = *(const f16x8*)(kb + (i + kReads) * 32);
+      t = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[i], q[i], t, 0, 0, 0);
+      beside(i);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
-  unsigned long long there = 0, there_next = 0;
+  // a lane's place among the values: its row and, in it, piece and half, without
+  // the part of the turn that goes over 64 bytes
+  const int e16 = lane & 15, value_turn = turned(e16 >> 2) & 12;
+  const int value_at = (4 * half + (e16 >> 2)) * kValueRow +
+                       ((((lane >> 4) & 1) * 2 + ((e16 & 3) >> 1)) ^ (turned(e16 >> 2) & 3)) * 16 + (e16 & 1) * 8;
+  // Step s's scores are formed a step ahead, beside the exponentials of the step
+  // before: its keys are in LDS then, its values a step later.
+  unsigned long long there = 0, there1 = 0, there2 = 0;
+  int pages_v = -1, pages_k = -1;
+  f32x16 t[KT / 32];
   if (steps > 0) {
-    int pages = page_of(0);
-    there = __ballot(pages >= 0);
-    fetch(0, pages);
-    widen_to(0, there);
+    const int pages0 = page_of(0), pages1 = page_of(1), pages2 = page_of(2);
+    pages_k = page_of(3);
+    there = __ballot(on_page(pages0)), there1 = __ballot(on_page(pages1)), there2 = __ballot(on_page(pages2));
+    Piece<D> next;
+    fetch_k(k, 0, pages0);
+    fetch_v(0, pages0);
+    if (steps > 1) fetch_k(next, 1, pages1);
+    k.ready(key, quarter), v.ready(key, quarter);
+    clean_v(0, there);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) widen_k(k, 0, i), widen_v(0, i);
     if (steps > 1) {
-      pages = page_of(1);
-      there_next = __ballot(pages >= 0);
-      fetch(1, pages);
+      next.ready(key, quarter);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) widen_k(next, 1, i);
+      fetch_v(1, pages1);
     }
+    if (steps > 2) fetch_k(k, 2, pages2);
+    pages_v = pages2;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < KT / 32; ++u) scores(0, u, t[u], [](int) {});
   }
-  int pages = steps > 2 ? page_of(2) : -1;
-  __syncthreads();
   for (int step = 0; step < steps; ++step) {
-    unsigned long long there_after = 0;
-    if (step + 1 < steps) {
-      widen_to(step + 1, there_next);
-      if (step + 2 < steps) {
-        there_after = __ballot(pages >= 0);
-        fetch(step + 2, pages);
-        if (step + 3 < steps) pages = page_of(step + 3);
-      }
-    }
-    const uint8_t* kb = lds + (step & 1) * kBuffer;
-    const uint8_t* vb = kb + KT * kKeyRow;
-    f32x16 t[KT / 32];
-#pragma unroll
-    for (int u = 0; u < KT / 32; ++u) {
-      t[u] = f32x16{};
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const f16x8 x = *(const f16x8*)(kb + (u * 32 + row) * kKeyRow + i * 32 + half * 16);
-        t[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q[i], t[u], 0, 0, 0);
-      }
-    }
     if (!whole(step, there)) {
-      uint32_t see = 0;
+      // this lane's keys are 8 (e / 4) + e % 4 of each 32, from `base` on
+      const int base = j0 + step * KT + 4 * half;
+      auto first = [](int n) { return n >= 64 ? ~0ull : (1ull << max(n, 0)) - 1; };
+      const unsigned long long see = there >> (4 * half) & first(hi - base) & ~first(lo - base);
 #pragma unroll
       for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int c = u * 32 + 8 * (e / 4) + 4 * half + e % 4, j = j0 + step * KT + c;
-          const bool yes = (there >> c & 1) && j < hi && j >= lo;
-          see |= (uint32_t)yes << (u * 16 + e);
-          t[u][e] = yes ? t[u][e] : -INFINITY;
-        }
+        for (int e = 0; e < 16; ++e) t[u][e] = see >> (u * 32 + 8 * (e / 4) + e % 4) & 1 ? t[u][e] : -INFINITY;
       const uint32_t any = lane < KT ? nan_lds[step & 1][lane] : 0u;
       if (__ballot(any != 0)) {
+        const uint32_t* of = &nan_lds[step & 1][4 * half];
 #pragma unroll
         for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (see >> (u * 16 + e) & 1) nan_blocks |= nan_lds[step & 1][u * 32 + 8 * (e / 4) + 4 * half + e % 4];
+          for (int e = 0; e < 16; ++e) {
+            const int c = u * 32 + 8 * (e / 4) + e % 4;
+            if (see >> c & 1) nan_blocks |= of[c];
+          }
       }
     }
-    float top = t[0][0];
+    float top = -INFINITY, top1 = -INFINITY;
 #pragma unroll
     for (int u = 0; u < KT / 32; ++u)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) top = fmaxf(top, t[u][e]);
+      for (int e = 0; e < 16; e += 4)
+        top = fmaxf(fmaxf(top, t[u][e]), t[u][e + 1]), top1 = fmaxf(fmaxf(top1, t[u][e + 2]), t[u][e + 3]);
+    top = fmaxf(top, top1);
     if (__ballot(m == -INFINITY ? top > m : (top - m) * g.scale > 8.0f)) {
       const float now = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
       const float f = now == m ? 1.0f : m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - now) * g.scale);
-      l *= f;
+      l *= f, l1 *= f;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) o[i] *= f;
       m = now;
     }
+    k.ready(key, quarter), v.ready(key, quarter);
+    if (step + 1 < steps) clean_v(step + 1, there1);
     // 2^6 times: a p of 2^-20 of the largest is still a normal f16 number
     const float ref = (m == -INFINITY ? 0.0f : m * g.scale) - 6.0f;
     f16x8 pr[KT / 16];
+    // the matrix instructions of a wave go before the other's fetching and masks
+    __builtin_amdgcn_s_setprio(1);
+    auto exponential = [&](int u, int e) {
+      const float x = __builtin_amdgcn_exp2f(fmaf(t[u][e], g.scale, -ref));  // 0 for a masked one
+      (e & 1 ? l1 : l) += x;
+      pr[u * 2 + e / 8][e % 8] = (_Float16)x;
+      if (e & 1) asm volatile("" : "+v"(l), "+v"(l1));  // here, not all at the step's end
+    };
 #pragma unroll
-    for (int u = 0; u < KT / 32; ++u)
+    for (int e = 0; e < 16; ++e) exponential(0, e);
+    __builtin_amdgcn_sched_barrier(0);
+    // The next step's scores, behind the last one of what LDS holds (nothing
+    // comes of it), take the registers that the exponentials leave.
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(t[u][e], g.scale, -ref));  // 0 for a masked one
-        l += x;
-        pr[u * 2 + e / 8][e % 8] = (_Float16)x;
-      }
+    for (int u = 1; u < KT / 32; ++u)
+      scores(step + 1, u - 1, t[u - 1], [&](int i) {
+        constexpr int n = 16 / (D / 16);
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i)
+        for (int e = 0; e < n; ++e) exponential(u, i * n + e);
+      });
+    // values and keys go into the places that the step before read last
+    scores(step + 1, KT / 32 - 1, t[KT / 32 - 1], [&](int i) {
+      if (i < D / 32)
+        widen_v(step + 1, i);
+      else
+        widen_k(k, step + 2, i - D / 32);
+    });
+    // Four groups of 16 lanes read 4 keys x 16 elements each, and lane e of one
+    // gets element e of the four.
+    const uint8_t* vb = lds + (step & 1) * kBuffer + KT * kKeyRow + value_at;
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    auto values = [&](int n) {
+      typedef __attribute__((address_space(3))) s16x4* Lds;
+      const int i = n / (KT / 16), u = n % (KT / 16);
+      const uint8_t* src = vb + (((i * 4) ^ value_turn) * 16 + u * 16 * kValueRow);
+      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)src);
+      const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(src + 8 * kValueRow));
+      return s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+    };
+    constexpr int kProducts = D / 32 * (KT / 16);
+    s16x8 pair[kProducts];
 #pragma unroll
-      for (int u = 0; u < KT / 16; ++u) {
-        // four groups of 16 lanes: 4 keys x 16 elements each
-        typedef __attribute__((address_space(3))) s16x4* Lds;
-        typedef short s16x8 __attribute__((ext_vector_type(8)));
-        const int e = lane & 15;
-        const uint8_t* src = vb + (u * 16 + 4 * half + (e >> 2)) * kValueRow + i * 64 + ((lane >> 4) & 1) * 32 + (e & 3) * 8;
-        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)src);
-        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(src + 8 * kValueRow));
-        const s16x8 xy = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, xy), pr[u], o[i], 0, 0, 0);
-      }
-    there = there_next;
-    there_next = there_after;
-    __syncthreads();
+    for (int n = 0; n < kPairs; ++n) pair[n] = values(n);
+#pragma unroll
+    for (int n = 0; n < kProducts; ++n) {
+      if (n + kPairs < kProducts) pair[n + kPairs] = values(n + kPairs);
+      const int i = n / (KT / 16), u = n % (KT / 16);
+      o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, pair[n]), pr[u], o[i], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    if (step + 2 < steps) fetch_v(step + 2, pages_v);
+    there = there1, there1 = there2;
+    if (step + 3 < steps) {
+      fetch_k(k, step + 3, pages_k);
+      there2 = __ballot(on_page(pages_k));
+      pages_v = pages_k;
+      pages_k = page_of(step + 4);
+    }
+    lds_barrier();
   }
+  l += l1;
   l += __shfl_xor(l, 32);
   nan_blocks |= __shfl_xor(nan_blocks, 32);
   if (!real) return;
@@ -847,7 +942,7 @@ namespace {
 template <int D>
 void launch_parts(hipStream_t st, const KvArgs& a, const AttnArgs& g, const AttnPlan& p) {
   if (p.tiles.splits) {
-    constexpr int kLds = std::max(2 * tile_keys(D) * (D * 4 + 48), 4 * 32 * split_row(D));
+    constexpr int kLds = std::max(2 * tile_keys(D) * (D * 4 + 16), 4 * 32 * split_row(D));
     const unsigned grid = p.tiles.splits + std::min((p.few.splits + 3) / 4, 1024);
     hipLaunchKernelGGL(attention_tile_kernel<D>, dim3(grid), dim3(256), kLds, st, a, g, p.tiles, p.few);
   } else {
@@ -872,8 +967,8 @@ size_t attention_space(const KvArgs& a, const AttnArgs& g, AttnPlan* plan) {
   // Tiles of 128 rows do the work in half the time, tiles of 16 rows are done
   // sooner where there is little of it: 8 sequences of up to 128 new tokens
   // after 1,024 keys (32 heads over 8, d = 128) 47 us, 24 us in tiles of 16; 256
-  // new tokens after 8,192 (64 tiles x 128 steps) 78 us, 89 us; 512 after 8,192 116
-  // us, 161 us; 4,096 and as many keys 184 us, 317 us.
+  // new tokens after 8,192 (64 tiles x 128 steps) 75 us, 87 us; 512 after 8,192 106
+  // us, 161 us; 4,096 and as many keys 168 us, 317 us.
   constexpr int kBigRows = 128, kBigSteps = 6144;
   const bool tiles = group <= 128 && (double)rows * a.kv_heads / 128 * ((longest + 63) / 64) >= kBigSteps;
   auto fill = [&](SplitArgs* p, int most_rows, int chunk, int waves, int whole, int least) {
@@ -898,7 +993,7 @@ size_t attention_space(const KvArgs& a, const AttnArgs& g, AttnPlan* plan) {
   const int many = a.d == 256 ? 1024 : 2048;  // waves that the chip holds at a time
   // A split of 128 rows leaves 64 KiB of sums at d = 128: items are split where
   // that shares them out over twice the workgroups or more (2 sequences of up to
-  // 1,536 new tokens after 4,096 keys 137 us, 179 us with splits for every
+  // 1,536 new tokens after 4,096 keys 140 us, 179 us with splits for every
   // uneven share), into eight steps or more.
   if (tiles) fill(&plan->tiles, 128, tile_keys(a.d), many / 4, 2, 8 * 64 / tile_keys(a.d));
   // A split of 16 rows takes two steps of 64 keys or more, or all of them where
