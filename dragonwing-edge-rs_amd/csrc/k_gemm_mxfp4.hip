@@ -23,21 +23,39 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-// bias, activation and the one rounding of a sum
-__device__ __forceinline__ float finish(const GemmMxArgs& a, int col, float s) {
-  if (a.bias) s += a.c_half ? h2f_ieee(((const uint16_t*)a.bias)[col]) : ((const float*)a.bias)[col];
-  if (a.act == ACT_RELU) s = s < 0.0f ? 0.0f : s;  // a NaN stays
-  if (a.act == ACT_SILU) s = s / (1.0f + expf(-s));
-  return s;
+// Bias of four neighbours from column n on, 0 behind the row's end.
+__device__ __forceinline__ f32x4 bias4(const GemmMxArgs& a, int n) {
+  f32x4 b = {};
+  if (!a.bias) return b;
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (n + r < a.n) b[r] = a.c_half ? h2f_ieee(((const uint16_t*)a.bias)[n + r]) : ((const float*)a.bias)[n + r];
+  return b;
 }
 
-// Four neighbours of a row of C, from column n on.
-__device__ __forceinline__ void store4(const GemmMxArgs& a, size_t row, int n, f32x4 s) {
+// e^-s is 2^(hi + lo), hi + lo = -s log2(e) to 2^-48 of it: exp2 and the
+// reciprocal leave 2^-22 of the result (with expf and a division to
+// 2^-24 a product of 1,209 x 7,712 x 832 takes 52 us, 33 us so).
+__device__ __forceinline__ float silu(float s) {
+  const float hi = s * -1.44269504f, lo = fmaf(s, -1.44269504f, -hi) + s * -1.92596300e-8f;
+  const float e = __builtin_amdgcn_exp2f(hi);
+  // an infinite e has no use for lo (nor has one of 0)
+  const float d = 1.0f + (e < 3.0e38f ? fmaf(e * 0.693147181f, lo, e) : e);
+  return s * __builtin_amdgcn_rcpf(d);
+}
+
+// Four neighbours of a row of C, from column n on: bias, activation and the
+// one rounding of a sum.
+__device__ __forceinline__ void store4(const GemmMxArgs& a, size_t row, int n, f32x4 s, f32x4 bias) {
   if (n >= a.n) return;
   const size_t at = row * a.n + n;
-  if (n + 4 <= a.n) {
+  s += bias;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) s[r] = finish(a, n + r, s[r]);
+  for (int r = 0; r < 4; ++r) {
+    if (a.act == ACT_RELU) s[r] = s[r] < 0.0f ? 0.0f : s[r];  // a NaN stays
+    if (a.act == ACT_SILU) s[r] = silu(s[r]);
+  }
+  if (n + 4 <= a.n) {
     if (a.c_half) {
       Loose<uint16_t, 4> h;
 #pragma unroll
@@ -54,11 +72,10 @@ __device__ __forceinline__ void store4(const GemmMxArgs& a, size_t row, int n, f
 #pragma unroll
   for (int r = 0; r < 4; ++r)
     if (n + r < a.n) {
-      const float v = finish(a, n + r, s[r]);
       if (a.c_half)
-        ((uint16_t*)a.c)[at + r] = narrow<uint16_t>(v);
+        ((uint16_t*)a.c)[at + r] = narrow<uint16_t>(s[r]);
       else
-        ((float*)a.c)[at + r] = v;
+        ((float*)a.c)[at + r] = s[r];
     }
 }
 
@@ -302,25 +319,56 @@ __global__ __launch_bounds__(MT* NT == 1 ? 1024 : 512) void gemm_mx_rows_kernel(
         for (int i = 1; i < waves; ++i) s += sums[(i * NT * MT + t * MT + u) * 64 + lane];
       }
       const int m = u * 16 + (lane & 15);
-      if (m < a.m) store4(a, m, n0 + t * 16 + (lane >> 4) * 4, s);
+      const int n = n0 + t * 16 + (lane >> 4) * 4;
+      if (m < a.m) store4(a, m, n, s, bias4(a, n));
     }
 }
 
-// A's rows at a stride of whole 16 bytes, zeros behind their ends.
-__global__ __launch_bounds__(256) void pad_rows_kernel(const uint16_t* __restrict__ x, uint16_t* __restrict__ y, int m,
-                                                       int k, int lda) {
-  const int j = (blockIdx.x * 256 + threadIdx.x) * 8;
-  if (j >= lda) return;
-  for (int r = blockIdx.y; r < m; r += gridDim.y) {
-    const uint16_t* p = x + (size_t)r * k + j;
-    Loose<uint16_t, 8> v;
-    if (j + 8 <= k) {
-      v = load_loose<uint16_t, 8>(p);
-    } else {
+// What is laid out anew before a product: f16 rows of A at a stride of whole 16
+// bytes, zeros behind their ends; scale bytes with each row at a stride of 16
+// bytes or more, 127 behind its end.  One launch: its first workgroups do one,
+// the others the other.
+struct Pads {
+  const uint16_t* x;  // rows [m][k], or null
+  uint16_t* x_to;     // [m][lda]
+  const uint8_t* s[2];  // scales [rows][blocks], or null
+  uint32_t* s_to[2];    // [rows][words]
+  size_t rows[2];
+  int m, k, lda, blocks, words;
+  unsigned first;  // workgroups of x and s[0]; those behind them have s[1]
+};
+
+__global__ __launch_bounds__(256) void pad_kernel(Pads p) {
+  const bool one = blockIdx.x < p.first;
+  const unsigned groups = one ? p.first : gridDim.x - p.first;
+  const size_t from = (size_t)(one ? blockIdx.x : blockIdx.x - p.first) * 256 + threadIdx.x, step = (size_t)groups * 256;
+  if (one && p.x) {
+    const unsigned pieces = p.lda / 8;
+    for (size_t i = from; i < (size_t)p.m * pieces; i += step) {
+      const size_t r = i / pieces;
+      const int j = (int)(i - r * pieces) * 8;
+      const uint16_t* x = p.x + r * p.k + j;
+      Loose<uint16_t, 8> v;
+      if (j + 8 <= p.k) {
+        v = load_loose<uint16_t, 8>(x);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v.v[i] = j + i < k ? p[i] : (uint16_t)0;
+        for (int e = 0; e < 8; ++e) v.v[e] = j + e < p.k ? x[e] : (uint16_t)0;
+      }
+      *(Loose<uint16_t, 8>*)__builtin_assume_aligned(p.x_to + i * 8, 16) = v;
     }
-    *(Loose<uint16_t, 8>*)__builtin_assume_aligned(y + (size_t)r * lda + j, 16) = v;
+    return;
+  }
+  const uint8_t* s = one ? p.s[0] : p.s[1];
+  uint32_t* to = one ? p.s_to[0] : p.s_to[1];
+  const size_t rows = one ? p.rows[0] : p.rows[1];
+  for (size_t i = from; i < rows * p.words; i += step) {
+    const size_t r = i / (unsigned)p.words;
+    const int b = (int)(i - r * p.words) * 4;
+    uint32_t v = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v |= (b + j < p.blocks ? (uint32_t)s[r * p.blocks + b + j] : 127u) << (8 * j);
+    to[i] = v;
   }
 }
 
@@ -633,10 +681,11 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_mx_tile_kernel(GemmMxArgs a,
   const int m1 = m0 + wave % WM * TM * 16 + (lane & 15), n1 = n0 + wave / WM * TN * 16 + (lane >> 4) * 4;
   if (gridDim.y == 1) {
 #pragma unroll
-    for (int u = 0; u < TM; ++u) {
-      if (m1 + u * 16 >= a.m) continue;
+    for (int i = 0; i < TN; ++i) {
+      const f32x4 bias = bias4(a, n1 + i * 16);
 #pragma unroll
-      for (int i = 0; i < TN; ++i) store4(a, m1 + u * 16, n1 + i * 16, acc[i][u]);
+      for (int u = 0; u < TM; ++u)
+        if (m1 + u * 16 < a.m) store4(a, m1 + u * 16, n1 + i * 16, acc[i][u], bias);
     }
     return;
   }
@@ -655,24 +704,12 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_mx_tile_kernel(GemmMxArgs a,
 __global__ __launch_bounds__(256) void gemm_mx_join_kernel(GemmMxArgs a, int shares) {
   const int n = (blockIdx.x * 256 + threadIdx.x) * 4;
   if (n >= a.n) return;
+  const f32x4 bias = bias4(a, n);
   for (int m = blockIdx.y; m < a.m; m += gridDim.y) {
     const float* p = a.parts + (size_t)m * a.ldp + n;
     f32x4 s = *(const f32x4*)p;
     for (int i = 1; i < shares; ++i) s += *(const f32x4*)(p + (size_t)i * a.m * a.ldp);
-    store4(a, m, n, s);
-  }
-}
-
-// Scale bytes with each row at a stride of 16 bytes or more, 127 behind its end.
-__global__ __launch_bounds__(256) void pad_scales_kernel(const uint8_t* __restrict__ s, uint32_t* __restrict__ y,
-                                                         size_t rows, int blocks, int words) {
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < rows * words; i += (size_t)gridDim.x * 256) {
-    const size_t r = i / words;
-    const int b = (int)(i - r * words) * 4;
-    uint32_t v = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v |= (b + j < blocks ? (uint32_t)s[r * blocks + b + j] : 127u) << (8 * j);
-    y[i] = v;
+    store4(a, m, n, s, bias);
   }
 }
 
@@ -680,7 +717,7 @@ __global__ __launch_bounds__(256) void pad_scales_kernel(const uint8_t* __restri
 
 namespace {
 
-// How a product of more than 64 rows is cut, and where its workspace lies.
+// How a product is cut, and where its workspace lies.
 struct Plan {
   bool big;      // tiles of 256 columns, else of 128
   int shares;    // of K
@@ -711,7 +748,7 @@ Plan plan(const GemmMxArgs& a) {
   for (int big = 0; big < 2; ++big) {
     const int rows = big ? 256 : 128, cols = rows, slots = big ? 256 : 512;
     const size_t tiles = (size_t)((a.m + rows - 1) / rows) * ((a.n + cols - 1) / cols);
-    for (int shares = 1; shares <= 16 && shares <= spans; shares *= 2) {
+    for (int shares = 1; shares <= 64 && shares <= spans; shares *= 2) {
       const double rounds = (double)((tiles * shares + slots - 1) / slots);
       const double one = std::min(tiles * shares / 256.0, 1.0);                         // share of CUs that have one
       const double two = std::min(std::max(tiles * shares / 256.0 - 1.0, 0.0), 1.0);  // and that have two
@@ -740,30 +777,33 @@ size_t gemm_mx_space(const GemmMxArgs& a) { return plan(a).bytes; }
 void launch_gemm_mx(hipStream_t st, GemmMxArgs a, void* space) {
   const Plan p = plan(a);
   char* base = (char*)space;
-  a.lda = a.k;
+  const int blocks = (a.k + 31) / 32, words = (blocks + 15) / 16 * 4;
+  a.lda = (a.k + 7) / 8 * 8;
+  a.pitch = words * 4;
+  Pads pads{};
+  pads.m = a.m, pads.k = a.k, pads.lda = a.lda, pads.blocks = blocks, pads.words = words;
+  auto groups = [](size_t units) { return (unsigned)std::min<size_t>((units + 255) / 256, 4096); };
+  unsigned others = 0;
   if (!a.as && a.k % 8) {
-    a.lda = (a.k + 7) / 8 * 8;
-    void* y = base + p.rows;
-    hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)((a.lda + 2047) / 2048), (unsigned)std::min(a.m, 65535)),
-                       dim3(256), 0, st, (const uint16_t*)a.a, (uint16_t*)y, a.m, a.k, a.lda);
-    a.a = y;
+    pads.x = (const uint16_t*)a.a;
+    a.a = pads.x_to = (uint16_t*)(base + p.rows);
+    pads.first = groups((size_t)a.m * (a.lda / 8));
   }
+  if (a.m > kFewRows && blocks % 16) {
+    if (a.as) {
+      pads.s[0] = a.as, pads.rows[0] = a.m;
+      a.as = (const uint8_t*)(pads.s_to[0] = (uint32_t*)(base + p.scales_a));
+      pads.first = groups((size_t)a.m * words);
+    }
+    pads.s[1] = a.ws, pads.rows[1] = a.n;
+    a.ws = (const uint8_t*)(pads.s_to[1] = (uint32_t*)(base + p.scales_w));
+    others = groups((size_t)a.n * words);
+  }
+  if (pads.first + others) hipLaunchKernelGGL(pad_kernel, dim3(pads.first + others), dim3(256), 0, st, pads);
   if (a.m <= kFewRows) {
     rows(st, a);
     DW_HIP(hipGetLastError());
     return;
-  }
-  const int blocks = (a.k + 31) / 32, words = (blocks + 15) / 16 * 4;
-  a.pitch = words * 4;
-  if (blocks % 16) {
-    auto pad = [&](const uint8_t*& s, size_t rows, size_t at) {
-      uint32_t* y = (uint32_t*)(base + at);
-      hipLaunchKernelGGL(pad_scales_kernel, dim3((unsigned)std::min<size_t>((rows * words + 255) / 256, 4096)), dim3(256),
-                         0, st, s, y, rows, blocks, words);
-      s = (const uint8_t*)y;
-    };
-    if (a.as) pad(a.as, a.m, p.scales_a);
-    pad(a.ws, a.n, p.scales_w);
   }
   a.parts = (float*)(base + p.parts);
   a.ldp = (a.n + 3) / 4 * 4;
