@@ -39,9 +39,9 @@ __device__ __forceinline__ f32x4 bias4(const GemmMxArgs& a, int n) {
 __device__ __forceinline__ float silu(float s) {
   const float hi = s * -1.44269504f, lo = fmaf(s, -1.44269504f, -hi) + s * -1.92596300e-8f;
   const float e = __builtin_amdgcn_exp2f(hi);
-  // an infinite e has no use for lo (nor has one of 0)
-  const float d = 1.0f + (e < 3.0e38f ? fmaf(e * 0.693147181f, lo, e) : e);
-  return s * __builtin_amdgcn_rcpf(d);
+  // an infinite e, or one of 0, has no use for lo, which an infinite s makes NaN
+  const float d = 1.0f + (e > 0.0f && e < 3.0e38f ? fmaf(e * 0.693147181f, lo, e) : e);
+  return 0.25f * s * __builtin_amdgcn_rcpf(0.25f * d);  // a reciprocal under 2^-126 would be 0
 }
 
 // Four neighbours of a row of C, from column n on: bias, activation and the
@@ -384,12 +384,14 @@ void launch_rows(hipStream_t st, const GemmMxArgs& a) {
 
 // Two tiles of 16 weight rows a wave halve what is read of A, where enough
 // waves are left (16 f16 rows x 5120 x 5120: 10.9 us, 15.8 us with one tile;
-// x 4096 x 14336: 22.6 us, 19.7 us with one).  Up to four f16 rows come
-// through LDS (one row x 4096 x 14336: 8.8 us, 9.9 us without).
+// x 4096 x 14336: 22.6 us, 19.7 us with one; 24 x 4096 x 4096: 11.1 us, 9.4 us
+// with one).  Up to four f16 rows come through LDS (one row x 4096 x 14336: 8.8
+// us, 9.9 us without).
 void rows(hipStream_t st, const GemmMxArgs& a) {
   const bool wide = a.n >= 5120;
   if (a.m > 16)
-    a.as ? launch_rows<true, 2, 2>(st, a) : launch_rows<false, 2, 2>(st, a);
+    if (wide) a.as ? launch_rows<true, 2, 2>(st, a) : launch_rows<false, 2, 2>(st, a);
+    else a.as ? launch_rows<true, 2, 1>(st, a) : launch_rows<false, 2, 1>(st, a);
   else if (a.as)
     wide ? launch_rows<true, 1, 2>(st, a) : launch_rows<true, 1, 1>(st, a);
   else if (a.m <= 4)

@@ -143,7 +143,7 @@ def test_product(backend, m, n, k, kind):
 
 @pytest.mark.parametrize("kind", ["f16", "mxfp4"])
 @pytest.mark.parametrize("m,n,k", [(3303, 4001, 100), (1900, 7300, 288), (6500, 2050, 129), (70, 2050, 8200),
-                                   (130, 1030, 14000)])
+                                   (130, 1030, 14000), (31, 5301, 700), (13, 5200, 333), (40, 130, 33000)])
 def test_large_product(backend, m, n, k, kind):
     # many tiles, and few with a long K that is shared
     rng = np.random.default_rng(m)
@@ -174,6 +174,25 @@ def test_product_on_the_largest_tiles(backend, kind):
     b = rng.normal(0, 1, n).astype(np.float32)
     want, off = ref.product(wide, ref.decode(q, s, k), b.astype(np.float64))
     check_product(run_product(backend, a, q, s, m, n, k, b, 0, np.float32), want, off)
+
+
+@pytest.mark.parametrize("m", [1, 20, 150])
+def test_silu_over_its_range(backend, m):
+    # from -110 to 110, and infinities and NaN, as biases of products of zeros
+    bias = np.linspace(-110, 110, 400).astype(np.float32)
+    bias[[5, 77, 390]] = np.inf, -np.inf, np.nan
+    q, s = ref.encode(np.zeros((400, 64)))
+    a = np.zeros((m, 64), np.float16)
+    got = run_product(backend, a, q, s, m, 400, 64, bias, 2, np.float32)
+    with np.errstate(over="ignore", invalid="ignore"):
+        y = bias.astype(np.float64)
+        want = np.where(np.isinf(y), np.where(y > 0, y, np.nan), y / (1 + np.exp(-y)))
+    np.testing.assert_array_equal(np.isnan(got), np.broadcast_to(np.isnan(want), got.shape))
+    ok = np.isfinite(want)
+    # where e^-y is no f32 number (above 2^128) it is infinite, and the quotient 0
+    gone = np.where(y[ok] < -128 * np.log(2), np.abs(want[ok]), 0)
+    assert (np.abs(got[:, ok] - want[ok]) <= 8 * 2.0 ** -24 * np.abs(want[ok]) + 2.0 ** -126 + gone).all()
+    assert (got[:, want == np.inf] == np.inf).all()
 
 
 def test_product_past_32_bit_offsets(backend):
