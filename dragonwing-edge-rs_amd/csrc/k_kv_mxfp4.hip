@@ -969,12 +969,16 @@ size_t attention_space(const KvArgs& a, const AttnArgs& g, AttnPlan* plan) {
   // after 1,024 keys (32 heads over 8, d = 128) 47 us, 24 us in tiles of 16; 256
   // new tokens after 8,192 (64 tiles x 128 steps) 75 us, 87 us; 512 after 8,192 106
   // us, 161 us; 4,096 and as many keys 168 us, 317 us.
-  constexpr int kBigRows = 128, kBigSteps = 6144;
-  const bool tiles = group <= 128 && (double)rows * a.kv_heads / 128 * ((longest + 63) / 64) >= kBigSteps;
+  // At d = 256 a CU holds four waves of them alone, and tiles pay sooner: 1,600 new
+  // tokens of 7 heads over one after 1,200 keys 99 us, 149 us in tiles of 16; 512
+  // alone 39.7 us, 35.0 us.
+  constexpr int kBigRows = 128;
+  const int big_steps = a.d == 256 ? 3000 : 6144;
+  const bool tiles = group <= 128 && (double)rows * a.kv_heads / 128 * ((longest + 63) / 64) >= big_steps;
   auto fill = [&](SplitArgs* p, int most_rows, int chunk, int waves, int whole, int least) {
     p->big = tiles ? kBigRows : kNever;
     p->big_tokens = tiles ? 128 / group : 1;
-    p->big_steps = kBigSteps;
+    p->big_steps = big_steps;
     p->group = group;
     p->head_tiles = (group + most_rows - 1) / most_rows;
     p->tile_tokens = std::max(1, most_rows / group);
