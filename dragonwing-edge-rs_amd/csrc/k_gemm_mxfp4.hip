@@ -682,12 +682,16 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_mx_tile_kernel(GemmMxArgs a,
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int m1 = m0 + wave % WM * TM * 16 + (lane & 15), n1 = n0 + wave / WM * TN * 16 + (lane >> 4) * 4;
   if (gridDim.y == 1) {
+    // A row's columns go one after the other, so that its lines fill at once: 4,096
+    // x 8,192 x 8,192 MXFP4 157 us, 188 us with a column's rows in turn.
+    f32x4 bias[TN];
 #pragma unroll
-    for (int i = 0; i < TN; ++i) {
-      const f32x4 bias = bias4(a, n1 + i * 16);
+    for (int i = 0; i < TN; ++i) bias[i] = bias4(a, n1 + i * 16);
 #pragma unroll
-      for (int u = 0; u < TM; ++u)
-        if (m1 + u * 16 < a.m) store4(a, m1 + u * 16, n1 + i * 16, acc[i][u], bias);
+    for (int u = 0; u < TM; ++u) {
+      if (m1 + u * 16 >= a.m) continue;
+#pragma unroll
+      for (int i = 0; i < TN; ++i) store4(a, m1 + u * 16, n1 + i * 16, acc[i][u], bias[i]);
     }
     return;
   }
