@@ -424,6 +424,10 @@ typedef __attribute__((address_space(3))) void* LdsPtr;
 // over the end of a stage.  Scales come four bytes an operand row and 128
 // elements: 16 bytes a row at a time, which last for 512 elements, because
 // each such load touches a line for every row.
+//
+// 4,096 x 8,192 x 8,192: MXFP4 rows 157 us (3.5 PFLOP/s); f16 rows 460 us (1.20
+// PFLOP/s, a library's f16 product reaches 1.20), bound by the conversions of
+// the weights, which larger tiles share among more rows (128 x 128: 482 us).
 template <bool MX, int WM, int WN, int TM, int TN>
 struct Tile {
   static constexpr int kWaves = WM * WN, kRowsA = WM * TM * 16, kRowsW = WN * TN * 16;

@@ -5,7 +5,8 @@
 // leaves 2^-30 of a turn, and only its fraction becomes f32: in f32 the
 // angle of position 500,000 would be off by 0.03 radians.  The cosines and
 // sines of a token are computed once and shared by its heads through LDS.
-// Bound by memory: every element is read and written once.
+// Bound by memory: every element is read and written once.  12,289 tokens x 24
+// heads x 80 f32: 40 us (4.8 TB/s, what a large copy reaches).
 #include <algorithm>
 
 #include "dw_common.h"

@@ -348,7 +348,8 @@ int dw_hip_qlinear_global_avg_pool_u8(dw_hip_backend* be, const dw_hip_buffer* x
  * x / 2^(s - 127) to the nearest, ties to even, 6 at most; 255 for a block
  * that holds an infinity or a NaN; elements behind a row's end are 0.
  * dtype: of x or y, F32 or F16 (f16 subnormals at their IEEE value).
- * Dequantize to F16 rounds to nearest even, and to F32 is exact. */
+ * Dequantize to F16 rounds to nearest even, and to F32 is exact where f32 holds
+ * the value (scales of 2^126 and 2^127 with large elements give infinities). */
 int dw_hip_quantize_mxfp4(dw_hip_backend* be, int dtype, const dw_hip_buffer* x, dw_hip_buffer* q,
                           dw_hip_buffer* scales, size_t rows, size_t k);
 int dw_hip_dequantize_mxfp4(dw_hip_backend* be, int dtype, const dw_hip_buffer* q, const dw_hip_buffer* scales,
