@@ -521,6 +521,7 @@ struct SplitArgs {
 };
 struct AttnPlan {
   SplitArgs tiles, few;  // of 128 rows, of 16; no splits: not used
+  bool whole_groups;     // items of 16 rows by workgroups, in place of splits
   size_t at[2][3];       // of their sums, stats and table: bytes into the workspace
 };
 // Sets the plan and gives the bytes of workspace.

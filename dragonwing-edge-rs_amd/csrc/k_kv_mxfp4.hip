@@ -319,8 +319,11 @@ __device__ __forceinline__ void own_lds() {
   __builtin_amdgcn_wave_barrier();
 }
 constexpr int split_row(int d) { return d * 2 + 32; }  // bytes in LDS: four rows side by side meet no bank twice
-template <int D>
-__device__ __forceinline__ bool attend_split(const KvArgs& a, const AttnArgs& g, const SplitArgs& p, int id, uint8_t* vt) {
+// W > 1: the W waves of a workgroup share the item's keys, and their sums meet
+// in LDS (`met`: their statistics).
+template <int D, int W = 1>
+__device__ __forceinline__ bool attend_split(const KvArgs& a, const AttnArgs& g, const SplitArgs& p, int id, uint8_t* vt,
+                                             int wave = 0, float2* met = nullptr) {
   constexpr int kRow = split_row(D);
   const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
   Split s;
@@ -328,6 +331,11 @@ __device__ __forceinline__ bool attend_split(const KvArgs& a, const AttnArgs& g,
   const bool have = plan<false>(a, g, p, id, &s, &joined);
   if (lane == 0) note_item(p, id, s, have, joined);
   if (!have) return false;
+  if constexpr (W > 1) {
+    const int each = (s.steps + W - 1) / W;
+    s.first = wave * each;
+    s.steps = min(each, s.steps - s.first);
+  }
   // this lane's query
   const int within = p.tile_tokens > 1 ? col / p.group : 0;
   const int head = s.head + (p.tile_tokens > 1 ? col - within * p.group : col);
@@ -489,6 +497,36 @@ __device__ __forceinline__ bool attend_split(const KvArgs& a, const AttnArgs& g,
     for (int i = 0; i < D / 16; ++i)
       if (nan_blocks >> (i / 2) & 1) o[i] = f32x4{NAN, NAN, NAN, NAN};
   }
+  if constexpr (W > 1) {
+    own_lds();
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) *(f32x4*)((float*)vt + col * D + i * 16 + quad * 4) = o[i];
+    if (quad == 0) met[wave * 16 + col] = make_float2(m == -INFINITY ? -INFINITY : m * g.scale, l);
+    __syncthreads();
+    const uint8_t* first = vt - wave * 32 * kRow;
+    for (int t = threadIdx.x; t < 16 * (D / 4); t += W * 64) {
+      const int r = t / (D / 4), c = t % (D / 4), in = p.tile_tokens > 1 ? r / p.group : 0, h = s.head + r - in * p.group;
+      if (in >= s.count || h >= (s.kv_head + 1) * p.group) continue;
+      float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) top = fmaxf(top, met[w * 16 + r].x);
+      top = top == -INFINITY ? 0.0f : top;
+      f32x4 y = {};
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float2 st = met[w * 16 + r];
+        const float weight = __builtin_amdgcn_exp2f(st.x - top);
+        sum = fmaf(weight, st.y, sum);
+        y += weight * *(const f32x4*)((const float*)(first + w * 32 * kRow) + r * D + c * 4);
+      }
+      const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+      ushort4 n;
+      n.x = narrow<uint16_t>(y[0] * f), n.y = narrow<uint16_t>(y[1] * f);
+      n.z = narrow<uint16_t>(y[2] * f), n.w = narrow<uint16_t>(y[3] * f);
+      *(ushort4*)(g.y + ((size_t)(s.token + in) * g.heads + h) * D + c * 4) = n;
+    }
+    return true;
+  }
   if (s.of == 1) {
     if (!real) return true;
     uint16_t* y = g.y + ((size_t)(s.token + within) * g.heads + head) * D + quad * 4;
@@ -515,6 +553,18 @@ template <int D>
 __global__ __launch_bounds__(64) void attention_split_kernel(KvArgs a, AttnArgs g, SplitArgs p) {
   __shared__ __align__(16) uint8_t vt[32 * split_row(D)];
   attend_split<D>(a, g, p, blockIdx.x, vt);
+}
+
+// Few steps: a workgroup takes an item whole, and nothing is joined by another
+// launch.
+constexpr int group_waves(int d) { return d == 256 ? 4 : 8; }
+template <int D>
+__global__ __launch_bounds__(64 * group_waves(D)) void attention_group_kernel(KvArgs a, AttnArgs g, SplitArgs p) {
+  constexpr int W = group_waves(D);
+  extern __shared__ __align__(16) uint8_t group_lds[];
+  __shared__ float2 met[W * 16];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  attend_split<D, W>(a, g, p, blockIdx.x, group_lds + wave * 32 * split_row(D), wave, met);
 }
 
 constexpr int kJoinSplits = 1024;
@@ -947,6 +997,10 @@ void launch_parts(hipStream_t st, const KvArgs& a, const AttnArgs& g, const Attn
     constexpr int kLds = std::max(2 * tile_keys(D) * (D * 4 + 16), 4 * 32 * split_row(D));
     const unsigned grid = p.tiles.splits + std::min((p.few.splits + 3) / 4, 1024);
     hipLaunchKernelGGL(attention_tile_kernel<D>, dim3(grid), dim3(256), kLds, st, a, g, p.tiles, p.few);
+  } else if (p.whole_groups) {
+    constexpr int W = group_waves(D);
+    hipLaunchKernelGGL(attention_group_kernel<D>, dim3((unsigned)p.few.items), dim3(64 * W), W * 32 * split_row(D), st, a,
+                       g, p.few);
   } else {
     hipLaunchKernelGGL(attention_split_kernel<D>, dim3((unsigned)p.few.splits), dim3(64), 0, st, a, g, p.few);
   }
@@ -1002,12 +1056,18 @@ size_t attention_space(const KvArgs& a, const AttnArgs& g, AttnPlan* plan) {
   // 1,536 new tokens after 4,096 keys 140 us, 179 us with splits for every
   // uneven share), into eight steps or more.
   if (tiles) fill(&plan->tiles, 128, tile_keys(a.d), many / 4, 2, 8 * 64 / tile_keys(a.d));
-  // A split of 16 rows takes two steps of 64 keys or more, or all of them where
-  // joining would take longer: one sequence of 1,024 keys 12.2 us in splits of
-  // two, 20.9 us in splits of eight; 64 of up to 512 17.5 us split, 14.1 us whole.
+  // A split of 16 rows takes two steps of 64 keys or more (one sequence of 1,024
+  // keys 12.2 us so, 20.9 us in splits of eight).  Few steps need no second launch:
+  // as many items as workgroups fit the chip take a workgroup each, a step a wave
+  // (32 sequences of up to 500 keys 9.7 us, 15.9 us with a wave each; one of 500
+  // 9.6 us, 12.3 us split and joined; two steps a wave at d = 128: one of 1,024
+  // 12.0 us, 11.7 us split), and more items a wave each (64 of up to 500 16.4 us,
+  // 17.5 us with a workgroup each).
   fill(&plan->few, 16, kChunk, many, 1, 2);
-  const int steps = (longest + kChunk - 1) / kChunk;
-  if (steps <= (plan->few.items >= 256 ? 8 : 4)) plan->few.least = 8, plan->few.slots = 0;
+  const int steps = (longest + kChunk - 1) / kChunk, items = plan->few.items;
+  plan->whole_groups = !tiles && steps > 1 && (a.d == 64 ? steps <= 16 && items <= 512
+                                                         : steps <= group_waves(a.d) && items <= 256);
+  if (plan->whole_groups || (steps <= 8 && items >= 256)) plan->few.least = steps, plan->few.slots = 0;
   size_t bytes = 0;
   int i = 0;
   for (const SplitArgs* p : {&plan->tiles, &plan->few}) {

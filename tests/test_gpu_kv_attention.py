@@ -261,6 +261,24 @@ def test_prompts_with_bad_pages_nan_and_empty_rows(backend):
     np.testing.assert_allclose(got[r, h], e @ v / e.sum(), rtol=2.0 ** -10, atol=8 * 2.0 ** -11)
 
 
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 2, 64), (7, 1, 128), (32, 2, 128), (3, 1, 256), (40, 1, 256)])
+@pytest.mark.parametrize("kv", [65, 200, 512, 1000])
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 70)])
+def test_few_steps_of_keys(backend, heads, kv_heads, d, kv, causal, window):
+    # few enough that a workgroup takes them whole, or just not
+    rng = np.random.default_rng(heads + d + kv)
+    c = ref.Cache(rng, [1, 0, 5, 2, 1], [kv, 3, kv // 2, 1, 40], kv_heads, d, 16, extra=1)
+    for name, b, blk in (("v", 0, 0), ("k", 2, 1), ("v", 2, 1)):
+        j = c.kv[b] - 1
+        c.s[name][c.table[b, j // 16], 0, j % 16, blk] = 255
+    q = rng.normal(0, 1, (c.tokens, heads, d)).astype(np.float16)
+    want, off = ref.attention(q.astype(np.float64), c, d ** -0.5, causal, window)
+    got = attend(backend, c, q, d ** -0.5, causal, window)
+    np.testing.assert_array_equal(np.isnan(got)[:-1], np.isnan(want)[:-1])
+    off[:-1][np.isnan(off[:-1])] = 0  # NaN where NaN is wanted; the last row is of no sequence
+    check(got, want, off)
+
+
 def large(rng, nq, kv, heads, kv_heads, d, page, window=0, extra=0):
     """A batch whose prompts are so long that tiles of 128 rows are used (6,144 steps of 64 keys), its queries, and some of
     its rows: all of the first and last tokens of each sequence, and 2% of the others."""
