@@ -7,6 +7,7 @@
 #include <algorithm>
 
 #include "dw_common.h"
+#include "kv_lists.h"
 #include "mxfp4.h"
 
 namespace dw {
@@ -113,10 +114,9 @@ __device__ __forceinline__ bool plan(const KvArgs& a, const AttnArgs& g, const S
   auto load = [&](int b) {
     first = count = len = raw = 0;
     if (b >= a.batch) return;
-    const int t0 = a.start[b], t1 = a.start[b + 1];
+    const NewTokens t = new_tokens(a.start[b], a.start[b + 1], a.tokens);
     raw = a.len[b];
-    first = max(t0, 0);
-    count = max(min(t1, a.tokens) - first, 0);
+    first = t.first, count = t.count;
     len = min(max(raw, 0), most);
   };
   auto is_big = [&] { return (long long)count * p.group >= p.big; };
