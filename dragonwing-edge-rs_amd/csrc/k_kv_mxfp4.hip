@@ -579,8 +579,7 @@ __device__ __forceinline__ void join_rows(const AttnArgs& g, const SplitArgs& p,
   __shared__ f32x4 sums[J];
   const int tid = threadIdx.x;
   const int splits = item.y & 0xFFFFFF, count = (int)((uint32_t)item.y >> 24);
-  // lists that overlap may have left an entry unwritten
-  if (splits <= 1 || item.x < 0 || item.x > p.slots - splits || item.z < 0 || item.w < 0) return;
+  if (!entry_fits(item.x, splits, item.z, item.w, p.slots, g.tokens, g.heads)) return;
   for (int col = from; col < p.rows; col += gridDim.y) {
     const int within = p.tile_tokens > 1 ? col / p.group : 0, head = item.w + col - within * p.group;
     if (within >= count || head >= (item.w / p.group + 1) * p.group) return;  // nor are the rows behind it

@@ -15,4 +15,13 @@ __host__ __device__ __forceinline__ NewTokens new_tokens(int t0, int t1, int tok
   return {first, end > first ? end - first : 0};
 }
 
+// Whether an entry of the joins' table (first slot, splits, first token, first
+// head) can be followed.  Lists that overlap make more items than the splits
+// that note them: an entry may then hold anything, and a head near an int's end
+// would wrap as the rows' heads are counted from it.
+__host__ __device__ __forceinline__ bool entry_fits(int slot, int splits, int token, int head, int slots, int tokens,
+                                                    int heads) {
+  return splits > 1 && slot >= 0 && slot <= slots - splits && token >= 0 && token < tokens && head >= 0 && head < heads;
+}
+
 }  // namespace dw
