@@ -8,9 +8,11 @@
 // times its factor is an f16 value for factors of 2^-23 to 2^13, that is for
 // any weights met in earnest.  Each wave looks at its scale bytes as it goes,
 // and where one is outside that range (and its block not all zeros) it
-// computes its part again in a form that holds for every factor: weights as
-// bf16 (exact from 2^-126 up), each f16 element as the sum of two bf16 ones,
-// so that every product is exact there too.
+// computes its part again in a form that holds for every factor: a quarter of
+// the weights as bf16, four times each f16 element as the sum of two bf16 ones,
+// so that every product is exact there too.  The quarter is what lets bf16 hold
+// all of them: 6 x 2^127 is beyond its largest number, and 0.5 x 2^-127 / 4 is
+// one of its subnormal numbers, which the matrix instruction takes as they are.
 #include <algorithm>
 
 #include "dw_common.h"
@@ -107,21 +109,29 @@ template <int J>
 __device__ __forceinline__ h16x2 pair_f16(uint32_t w, float s) {
   return __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, J);
 }
-template <int J>
-__device__ __forceinline__ bf16x2 pair_bf16(uint32_t w, float s) {
-  return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, J);
-}
 __device__ __forceinline__ f16x8 eight_f16(uint32_t w, float s) {
   const h16x2 a = pair_f16<0>(w, s), b = pair_f16<1>(w, s), c = pair_f16<2>(w, s), d = pair_f16<3>(w, s);
   return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
-__device__ __forceinline__ bf16x8 eight_bf16(uint32_t w, float s) {
-  const bf16x2 a = pair_bf16<0>(w, s), b = pair_bf16<1>(w, s), c = pair_bf16<2>(w, s), d = pair_bf16<3>(w, s);
-  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+// A quarter of eight weights; `s` has their scale byte in bits 30:23.
+__device__ __forceinline__ bf16x8 quarters_bf16(uint32_t w, float s) {
+  const uint32_t byte = __builtin_bit_cast(uint32_t, s) >> 23 & 255u;
+  // 2^(byte - 129): below 2^-126 the bits of subnormal numbers
+  const uint32_t bits = byte == 255u ? 0x7FC00000u : byte > 2u ? (byte - 2u) << 23 : 1u << (20 + byte);
+  const float factor = __builtin_bit_cast(float, bits);
+  float v[8];
+  mx_decode8(w, 1.0f, v);
+  uint32_t h[4];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t t = __builtin_bit_cast(uint32_t, v[e] * factor);  // two bits of significand: its upper half is bf16
+    h[e / 2] = e % 2 ? h[e / 2] | (t & 0xFFFF0000u) : t >> 16;
+  }
+  return __builtin_bit_cast(bf16x8, make_uint4(h[0], h[1], h[2], h[3]));
 }
-// f16 elements as bf16 ones whose sum they are: the upper eight bits of the
-// significand, and what is left (nothing, for an infinity).  Both are bf16
-// values, the upper halves of their f32 forms.
+// Four times f16 elements as bf16 ones whose sum they are: the upper eight bits
+// of the significand, and what is left (nothing, for an infinity).  Both are
+// bf16 values, the upper halves of their f32 forms.
 __device__ __forceinline__ void halves(f16x8 x, bf16x8* hi, bf16x8* lo) {
   const uint4 words = __builtin_bit_cast(uint4, x);
   uint32_t h[4], l[4];
@@ -130,8 +140,8 @@ __device__ __forceinline__ void halves(f16x8 x, bf16x8* hi, bf16x8* lo) {
     const uint16_t b = (uint16_t)(word(words, e / 2) >> (16 * (e & 1)));
     const bool odd = (b & 0x7C00u) == 0x7C00u;  // infinities and NaN
     const float top = h2f_ieee(odd ? b : (uint16_t)(b & 0xFFF8u));
-    const uint32_t t = __builtin_bit_cast(uint32_t, top);
-    const uint32_t r = odd ? 0u : __builtin_bit_cast(uint32_t, h2f_ieee(b) - top);
+    const uint32_t t = __builtin_bit_cast(uint32_t, 4.0f * top);
+    const uint32_t r = odd ? 0u : __builtin_bit_cast(uint32_t, 4.0f * (h2f_ieee(b) - top));
     h[e / 2] = e % 2 ? h[e / 2] | (t & 0xFFFF0000u) : t >> 16;
     l[e / 2] = e % 2 ? l[e / 2] | (r & 0xFFFF0000u) : r >> 16;
   }
@@ -141,7 +151,7 @@ __device__ __forceinline__ void halves(f16x8 x, bf16x8* hi, bf16x8* lo) {
 __device__ __forceinline__ f32x4 times_exact(uint32_t w, float s, f16x8 x, f32x4 acc) {
   bf16x8 hi, lo;
   halves(x, &hi, &lo);
-  const bf16x8 v = eight_bf16(w, s);
+  const bf16x8 v = quarters_bf16(w, s);
   acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, hi, acc, 0, 0, 0);
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, lo, acc, 0, 0, 0);
 }

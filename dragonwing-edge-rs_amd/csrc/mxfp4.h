@@ -13,7 +13,6 @@
 
 namespace dw {
 
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 // Scale byte j of a word, as the conversions' factor operand.
