@@ -516,7 +516,7 @@ struct SplitArgs {
   int items, splits;      // tiles x kv heads at most, and splits: the grid
   int slots, joined;      // splits of items that have several and such items, at most; no slots: none has
   float* sums;            // [slots][rows][d]
-  float2* stats;          // [slots][rows]: reference, sum
+  float2* stats;          // [slots][rows]: reference (a score, unscaled), sum
   int4* table;            // [1 + joined]: their number; first slot, splits and tokens, first token, first head
 };
 struct AttnPlan {

@@ -313,6 +313,11 @@ struct Piece {
 // four keys a read.  The running maximum moves only when a score passes it by
 // 2^8, so that most steps leave the sums as they are.
 constexpr int kChunk = 64;  // keys a step
+// An exponent is score * scale - ref in one rounding, ref being the reference's
+// own product, rounded by up to 2^-24 of it.  Beyond kFar that is more than the
+// exponentials' own error (and from 2^25 on whole powers of two, up to infinite
+// or vanishing ones): scores are taken relative to the reference first there.
+constexpr float kFar = 1024.0f;
 // A wave's accesses of its own LDS before here go before those behind.
 __device__ __forceinline__ void own_lds() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -452,7 +457,15 @@ __device__ __forceinline__ bool attend_split(const KvArgs& a, const AttnArgs& g,
       m = now;
     }
     // 2^6 times: a p of 2^-20 of the largest is still a normal f16 number
-    const float ref = (m == -INFINITY ? 0.0f : m * g.scale) - 6.0f;
+    float ref = (m == -INFINITY ? 0.0f : m * g.scale) - 6.0f;
+    if (__ballot(fabsf(ref) > kFar)) {
+      const float from_m = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t[u][r] -= from_m;
+      ref = -6.0f;
+    }
     f16x8 pr[2];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -501,7 +514,7 @@ __device__ __forceinline__ bool attend_split(const KvArgs& a, const AttnArgs& g,
     own_lds();
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) *(f32x4*)((float*)vt + col * D + i * 16 + quad * 4) = o[i];
-    if (quad == 0) met[wave * 16 + col] = make_float2(m == -INFINITY ? -INFINITY : m * g.scale, l);
+    if (quad == 0) met[wave * 16 + col] = make_float2(m, l);
     __syncthreads();
     const uint8_t* first = vt - wave * 32 * kRow;
     for (int t = threadIdx.x; t < 16 * (D / 4); t += W * 64) {
@@ -515,7 +528,7 @@ __device__ __forceinline__ bool attend_split(const KvArgs& a, const AttnArgs& g,
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         const float2 st = met[w * 16 + r];
-        const float weight = __builtin_amdgcn_exp2f(st.x - top);
+        const float weight = __builtin_amdgcn_exp2f((st.x - top) * g.scale);
         sum = fmaf(weight, st.y, sum);
         y += weight * *(const f32x4*)((const float*)(first + w * 32 * kRow) + r * D + c * 4);
       }
@@ -545,7 +558,7 @@ __device__ __forceinline__ bool attend_split(const KvArgs& a, const AttnArgs& g,
   float* out = p.sums + ((size_t)slot * p.rows + col) * D + quad * 4;
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) *(f32x4*)(out + i * 16) = o[i];
-  if (quad == 0) p.stats[(size_t)slot * p.rows + col] = make_float2(m == -INFINITY ? -INFINITY : m * g.scale, l);
+  if (quad == 0) p.stats[(size_t)slot * p.rows + col] = make_float2(m, l);
   return true;
 }
 
@@ -603,7 +616,7 @@ __device__ __forceinline__ void join_rows(const AttnArgs& g, const SplitArgs& p,
       __syncthreads();
       for (int i = tid; i < n; i += J) {
         const float2 st = stats[(size_t)(i0 + i) * p.rows];
-        const float w = __builtin_amdgcn_exp2f(st.x - ref);
+        const float w = __builtin_amdgcn_exp2f((st.x - ref) * g.scale);
         weight[i] = w;
         l = fmaf(w, st.y, l);
       }
@@ -882,7 +895,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(K
     k.ready(key, quarter), v.ready(key, quarter);
     if (step + 1 < steps) clean_v(step + 1, there1);
     // 2^6 times: a p of 2^-20 of the largest is still a normal f16 number
-    const float ref = (m == -INFINITY ? 0.0f : m * g.scale) - 6.0f;
+    float ref = (m == -INFINITY ? 0.0f : m * g.scale) - 6.0f;
+    if (__ballot(fabsf(ref) > kFar)) {
+      const float from_m = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int u = 0; u < KT / 32; ++u) t[u] -= from_m;
+      ref = -6.0f;
+    }
     f16x8 pr[KT / 16];
     // the matrix instructions of a wave go before the other's fetching and masks
     __builtin_amdgcn_s_setprio(1);
@@ -961,7 +980,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attention_tile_kernel(K
         if (nan_blocks >> i & 1) v = f32x4{NAN, NAN, NAN, NAN};
         *(f32x4*)(out + i * 32 + e * 8) = v;
       }
-    if (half == 0) p.stats[(size_t)slot * p.rows + r] = make_float2(m == -INFINITY ? -INFINITY : m * g.scale, l);
+    if (half == 0) p.stats[(size_t)slot * p.rows + r] = make_float2(m, l);
     return;
   }
   uint16_t* y = g.y + ((size_t)token * g.heads + head) * D + half * 4;
