@@ -113,19 +113,22 @@ __device__ __forceinline__ f16x8 eight_f16(uint32_t w, float s) {
   const h16x2 a = pair_f16<0>(w, s), b = pair_f16<1>(w, s), c = pair_f16<2>(w, s), d = pair_f16<3>(w, s);
   return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
+template <int J>
+__device__ __forceinline__ uint32_t pair_bf16(uint32_t w, float s) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, J));
+}
 // A quarter of eight weights; `s` has their scale byte in bits 30:23.
 __device__ __forceinline__ bf16x8 quarters_bf16(uint32_t w, float s) {
   const uint32_t byte = __builtin_bit_cast(uint32_t, s) >> 23 & 255u;
-  // 2^(byte - 129): below 2^-126 the bits of subnormal numbers
-  const uint32_t bits = byte == 255u ? 0x7FC00000u : byte > 2u ? (byte - 2u) << 23 : 1u << (20 + byte);
-  const float factor = __builtin_bit_cast(float, bits);
-  float v[8];
-  mx_decode8(w, 1.0f, v);
-  uint32_t h[4];
+  const float f = mx_scale(byte == 255u ? 255u : max(byte, 2u) - 2u);
+  uint32_t h[4] = {pair_bf16<0>(w, f), pair_bf16<1>(w, f), pair_bf16<2>(w, f), pair_bf16<3>(w, f)};
+  if (__ballot(byte < 2u)) {  // factors of 2^-129 and 2^-128, which no scale byte stands for
+    const float rest = byte == 0u ? 0.25f : byte == 1u ? 0.5f : 1.0f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint32_t t = __builtin_bit_cast(uint32_t, v[e] * factor);  // two bits of significand: its upper half is bf16
-    h[e / 2] = e % 2 ? h[e / 2] | (t & 0xFFFF0000u) : t >> 16;
+    for (int i = 0; i < 4; ++i) {
+      const float lo = __builtin_bit_cast(float, h[i] << 16) * rest, hi = __builtin_bit_cast(float, h[i] & 0xFFFF0000u) * rest;
+      h[i] = __builtin_bit_cast(uint32_t, lo) >> 16 | (__builtin_bit_cast(uint32_t, hi) & 0xFFFF0000u);
+    }
   }
   return __builtin_bit_cast(bf16x8, make_uint4(h[0], h[1], h[2], h[3]));
 }
@@ -139,19 +142,18 @@ __device__ __forceinline__ void halves(f16x8 x, bf16x8* hi, bf16x8* lo) {
   for (int e = 0; e < 8; ++e) {
     const uint16_t b = (uint16_t)(word(words, e / 2) >> (16 * (e & 1)));
     const bool odd = (b & 0x7C00u) == 0x7C00u;  // infinities and NaN
-    const float top = h2f_ieee(odd ? b : (uint16_t)(b & 0xFFF8u));
-    const uint32_t t = __builtin_bit_cast(uint32_t, 4.0f * top);
-    const uint32_t r = odd ? 0u : __builtin_bit_cast(uint32_t, 4.0f * (h2f_ieee(b) - top));
+    const float top = 4.0f * h2f_ieee(odd ? b : (uint16_t)(b & 0xFFF8u));
+    const uint32_t t = __builtin_bit_cast(uint32_t, top);
+    const uint32_t r = odd ? 0u : __builtin_bit_cast(uint32_t, fmaf(h2f_ieee(b), 4.0f, -top));
     h[e / 2] = e % 2 ? h[e / 2] | (t & 0xFFFF0000u) : t >> 16;
     l[e / 2] = e % 2 ? l[e / 2] | (r & 0xFFFF0000u) : r >> 16;
   }
   *hi = __builtin_bit_cast(bf16x8, make_uint4(h[0], h[1], h[2], h[3]));
   *lo = __builtin_bit_cast(bf16x8, make_uint4(l[0], l[1], l[2], l[3]));
 }
-__device__ __forceinline__ f32x4 times_exact(uint32_t w, float s, f16x8 x, f32x4 acc) {
+__device__ __forceinline__ f32x4 times_exact(bf16x8 v, f16x8 x, f32x4 acc) {
   bf16x8 hi, lo;
   halves(x, &hi, &lo);
-  const bf16x8 v = quarters_bf16(w, s);
   acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, hi, acc, 0, 0, 0);
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, lo, acc, 0, 0, 0);
 }
@@ -267,9 +269,10 @@ struct Rows {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if constexpr (EXACT) {
+              const bf16x8 e = quarters_bf16(word(wv[t][i], j), f);
 #pragma unroll
               for (int u = 0; u < MT; ++u)
-                acc[t][u] = times_exact(word(wv[t][i], j), f, __builtin_bit_cast(f16x8, xv[u][i * 4 + j]), acc[t][u]);
+                acc[t][u] = times_exact(e, __builtin_bit_cast(f16x8, xv[u][i * 4 + j]), acc[t][u]);
             } else {
               const f16x8 e = eight_f16(word(wv[t][i], j), f);
 #pragma unroll
@@ -570,8 +573,9 @@ struct Tile {
       } else {
         const float f = __builtin_bit_cast(float, r.fw[t] << (23 - 8 * part));
         if constexpr (EXACT) {
+          const bf16x8 v = quarters_bf16(r.word[t], f);
 #pragma unroll
-          for (int u = 0; u < TM; ++u) acc[t][u] = times_exact(r.word[t], f, __builtin_bit_cast(f16x8, r.x[u]), acc[t][u]);
+          for (int u = 0; u < TM; ++u) acc[t][u] = times_exact(v, __builtin_bit_cast(f16x8, r.x[u]), acc[t][u]);
         } else {
           // factors of 2^-15 to 1, as weights have them, both parts' at a time
           if (part == 0) *far |= (r.fw[t] ^ 0x7070u) & 0xF0F0u;
