@@ -15,12 +15,7 @@ namespace dw {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// Scale byte j of a word, as the conversions' factor operand.
-template <int J>
-__device__ __forceinline__ float mx_scale_of(uint32_t w) {
-  static_assert(J >= 0 && J < 4, "byte of a word");
-  return __builtin_bit_cast(float, J == 0 ? w << 23 : J == 1 ? w << 15 : J == 2 ? w << 7 : w >> 1);
-}
+// A scale byte as the conversions' factor operand.
 __device__ __forceinline__ float mx_scale(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
 
 // The scale byte of a block whose largest magnitude has these f32 bits
