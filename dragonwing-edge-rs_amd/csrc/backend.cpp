@@ -1363,25 +1363,7 @@ int dw_hip_rope_axes(dw_hip_backend* be, int dtype, const dw_hip_buffer* x, size
     if (x_stride != y_stride || (x_off != y_off && x_off < y_off + w && y_off < x_off + w))
       dw::fail(DW_ERR_INVALID, "rope_axes: input and output overlap");
   }
-  Backend* b = B(be);
-  std::lock_guard<std::mutex> lock(b->mu);
-  need_on(b, x, tokens * x_stride * es, "rope_axes: input");
-  need_on(b, y, tokens * y_stride * es, "rope_axes: output");
-  need_on(b, positions, axes * tokens * 4, "rope_axes: positions");
-  if (positions == y) dw::fail(DW_ERR_INVALID, "rope_axes: the positions are the output");
   dw::RopeArgs a{};
-  a.x = x->ptr;
-  a.y = y->ptr;
-  a.pos = (const int32_t*)positions->ptr;
-  a.x_stride = x_stride;
-  a.x_off = x_off;
-  a.y_stride = y_stride;
-  a.y_off = y_off;
-  a.tokens = tokens;
-  a.heads = (int)heads;
-  a.head_dim = (int)head_dim;
-  a.half = (int)half;
-  a.copy = !(x == y && x_off == y_off);
   // the axis of each pair, and its frequency base^(-2 i / rotary_dim), i the
   // pair's index in the head (freq 0) or base^(-j / n), j its index among the
   // n pairs of its axis (freq 1): powers by repeated products in 80 bits
@@ -1398,10 +1380,30 @@ int dw_hip_rope_axes(dw_hip_backend* be, int dtype, const dw_hip_buffer* x, size
     a.table.axis[i] = (uint8_t)next;
     const size_t f = freq ? next : axes;
     a.table.freq[i] = (double)(power[f] / kTurn);
+    if (!std::isfinite(a.table.freq[i] * 0x1p31))
+      dw::fail(DW_ERR_INVALID, "rope_axes: base is so small that angles are no f64 numbers");
     power[f] *= step[f];
     ++used[next];
     if (order) next = (next + 1) % axes;
   }
+  Backend* b = B(be);
+  std::lock_guard<std::mutex> lock(b->mu);
+  need_on(b, x, tokens * x_stride * es, "rope_axes: input");
+  need_on(b, y, tokens * y_stride * es, "rope_axes: output");
+  need_on(b, positions, axes * tokens * 4, "rope_axes: positions");
+  if (positions == y) dw::fail(DW_ERR_INVALID, "rope_axes: the positions are the output");
+  a.x = x->ptr;
+  a.y = y->ptr;
+  a.pos = (const int32_t*)positions->ptr;
+  a.x_stride = x_stride;
+  a.x_off = x_off;
+  a.y_stride = y_stride;
+  a.y_off = y_off;
+  a.tokens = tokens;
+  a.heads = (int)heads;
+  a.head_dim = (int)head_dim;
+  a.half = (int)half;
+  a.copy = !(x == y && x_off == y_off);
   dw::launch_rope(b->stream, dtype, a, pairs);
   API_END
 }

@@ -378,7 +378,8 @@ int dw_hip_gemm_mxfp4(dw_hip_backend* be, int a_dtype, const dw_hip_buffer* a, c
  * axes' pairs one axis after the other; 1: in turn among the axes that have
  * pairs left.  freq 0: e(i) = i / r; 1: e(i) = j / sections[axis(i)] with j
  * the pair's place among those of its axis.  positions [axes][tokens] int32,
- * any value; angles are formed in 64 bits.  rotary_dim <= 256, axes <= 8. */
+ * any value; angles are formed in 64 bits.  rotary_dim <= 256, axes <= 8; base
+ * is above 0, and one so small that an angle is no f64 number is refused. */
 int dw_hip_rope_axes(dw_hip_backend* be, int dtype, const dw_hip_buffer* x, size_t x_stride, size_t x_off,
                      dw_hip_buffer* y, size_t y_stride, size_t y_off, const dw_hip_buffer* positions, size_t tokens,
                      size_t heads, size_t head_dim, size_t rotary_dim, const size_t* sections, size_t axes, int order,
