@@ -164,3 +164,25 @@ def attention(q, cache, scale, causal=True, window=0, some=None):
                                  + len(s) * 2.0 ** -25 * np.abs(v[m]).max(0) / e.sum()
                                  + 2.0 ** -11 * np.abs(y[r, h]) + 2.0 ** -25)
     return y, off
+
+
+def whole_product(rng, m, n, k, kind):
+    """Rows ("f16" or "mxfp4") and weights without a zero whose products f32 sums exactly in any order (whole numbers of
+    1/16 or 1/32, together below 2^24 of them up to k = 33,000): the operands, the weights, and the product."""
+    nb = blocks(k)
+    codes = rng.integers(1, 8, (n, nb * 32), dtype=np.uint8) | rng.integers(0, 2, (n, nb * 32), dtype=np.uint8) << 3
+    codes[:, k:] = 0
+    s = rng.integers(124, 128, (n, nb), dtype=np.uint8)
+    q = codes[:, 0::2] | codes[:, 1::2] << 4
+    w = decode(q, s, k)
+    if kind == "f16":
+        a = (rng.integers(1, 4, (m, k)) * rng.choice([-1, 1], (m, k))).astype(np.float16)
+        wide = a.astype(np.float64)
+    else:
+        codes = rng.integers(1, 5, (m, nb * 32), dtype=np.uint8) | rng.integers(0, 2, (m, nb * 32), dtype=np.uint8) << 3
+        codes[:, k:] = 0
+        a = codes[:, 0::2] | codes[:, 1::2] << 4, np.full((m, nb), 127, np.uint8)
+        wide = decode(*a, k)
+    # f32 holds every sum of them, in any order
+    assert np.abs(wide).max() * np.abs(w).max() * k * (16 if kind == "f16" else 32) < 2 ** 24
+    return a, q, s, wide, w, wide.astype(np.float32) @ w.astype(np.float32).T
