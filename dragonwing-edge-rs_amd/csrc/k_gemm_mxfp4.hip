@@ -36,8 +36,10 @@ __device__ __forceinline__ f32x4 bias4(const GemmMxArgs& a, int n) {
 }
 
 // e^-s is 2^(hi + lo), hi + lo = -s log2(e) to 2^-48 of it: exp2 and the
-// reciprocal leave 2^-22 of the result (with expf and a division to
-// 2^-24 a product of 1,209 x 7,712 x 832 takes 52 us, 33 us so).
+// reciprocal leave 2^-22 of the result, below an f16 C's 2^-11 and near the
+// sum's own error in an f32 one.  1,209 x 7,712 x 832: MXFP4 rows 28.5 us, 33.4
+// us with expf and a division, which leave 2^-24, and 23.6 us without SiLU; f16
+// rows 39.4, 44.3 and 34.5 us.
 __device__ __forceinline__ float silu(float s) {
   const float hi = s * -1.44269504f, lo = fmaf(s, -1.44269504f, -hi) + s * -1.92596300e-8f;
   const float e = __builtin_amdgcn_exp2f(hi);
@@ -166,7 +168,8 @@ __device__ __forceinline__ f32x4 times_exact(bf16x8 v, f16x8 x, f32x4 acc) {
 // operand is a whole block, four lanes side by side read 64 bytes of a row,
 // and four steps' loads are in flight at a time; each workgroup reads the
 // rows of A again from L2, which NT divides.  One f16 row x 14336 x 4096:
-// 10.3 us (3.0 TB/s); 16 MXFP4 rows x 8192 x 8192: 10.1 us (3.6 TB/s).
+// 10.1 us a call among others (3.1 TB/s); 16 MXFP4 rows x 8192 x 8192: 9.8 us
+// (3.7 TB/s).
 // FEW: f16 rows, at most four, that a wave brings to LDS whole, an element
 // once: the matrix instruction's operand has 16 columns, and as loads of its
 // own each would cost 64 bytes a lane and step.
@@ -438,9 +441,10 @@ typedef __attribute__((address_space(3))) void* LdsPtr;
 // elements: 16 bytes a row at a time, which last for 512 elements, because
 // each such load touches a line for every row.
 //
-// 4,096 x 8,192 x 8,192: MXFP4 rows 157 us (3.5 PFLOP/s); f16 rows 460 us (1.20
-// PFLOP/s, a library's f16 product reaches 1.20), bound by the conversions of
-// the weights, which larger tiles share among more rows (128 x 128: 482 us).
+// 4,096 x 8,192 x 8,192: MXFP4 rows 152 us (3.6 PFLOP/s; 190 us in tiles of 128
+// x 128); f16 rows 420 us (1.31 PFLOP/s; a library's product with f16 weights in
+// the same layout reaches 1.58), bound by the conversions of the weights, which
+// larger tiles share among more rows (128 x 128: 508 us).
 template <bool MX, int WM, int WN, int TM, int TN>
 struct Tile {
   static constexpr int kWaves = WM * WN, kRowsA = WM * TM * 16, kRowsW = WN * TN * 16;
@@ -701,7 +705,7 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_mx_tile_kernel(GemmMxArgs a,
   const int m1 = m0 + wave % WM * TM * 16 + (lane & 15), n1 = n0 + wave / WM * TN * 16 + (lane >> 4) * 4;
   if (gridDim.y == 1) {
     // A row's columns go one after the other, so that its lines fill at once: 4,096
-    // x 8,192 x 8,192 MXFP4 157 us, 188 us with a column's rows in turn.
+    // x 8,192 x 8,192 MXFP4 152 us, 185 us with a column's rows in turn.
     f32x4 bias[TN];
 #pragma unroll
     for (int i = 0; i < TN; ++i) bias[i] = bias4(a, n1 + i * 16);

@@ -312,6 +312,10 @@ struct Piece {
 // in that order: values go through LDS as f16 rows and come back transposed,
 // four keys a read.  The running maximum moves only when a score passes it by
 // 2^8, so that most steps leave the sums as they are.
+//
+// Each p is rounded to f16, the matrix instruction's type: 2^-11 of it, where the
+// cache's own rounding of a value is 2^-3.  p in two halves would take the second
+// product twice.  The sum of p stays f32, of p before it is rounded.
 constexpr int kChunk = 64;  // keys a step
 // An exponent is score * scale - ref in one rounding, ref being the reference's
 // own product, rounded by up to 2^-24 of it.  Beyond kFar that is more than the
@@ -684,11 +688,9 @@ __device__ __forceinline__ void lds_barrier() {
 // in that order, which transposing reads of LDS give it.  Two workgroups fit a
 // CU up to d = 128, so that one's exponentials run beside the other's products.
 //
-// 4,096 causal tokens of 32 heads over 8 kv heads, d = 128: 168 us, 815 TFLOP/s
-// (184 us before the scores went a step ahead, with LDS conflicts of the
-// values and without priorities).  The products take a third of that and the
-// vector instructions (exponentials, conversions) half; two waves a SIMD do
-// not hide all of either.
+// 4,096 causal tokens of 32 heads over 8 kv heads, d = 128: 159 us, 865 TFLOP/s.
+// The products take a third of that and the vector instructions (exponentials,
+// conversions) half; two waves a SIMD do not hide all of either.
 //
 // Sequences of few rows, whose splits are a wave's, take the workgroups behind
 // the tiles'.
@@ -1040,12 +1042,15 @@ size_t attention_space(const KvArgs& a, const AttnArgs& g, AttnPlan* plan) {
   const long long rows = (long long)a.tokens * group;
   // Tiles of 128 rows do the work in half the time, tiles of 16 rows are done
   // sooner where there is little of it: 8 sequences of up to 128 new tokens
-  // after 1,024 keys (32 heads over 8, d = 128) 47 us, 24 us in tiles of 16; 256
-  // new tokens after 8,192 (64 tiles x 128 steps) 75 us, 87 us; 512 after 8,192 106
-  // us, 161 us; 4,096 and as many keys 168 us, 317 us.
+  // after 1,024 keys (32 heads over 8, d = 128) 51 us, 27 us in tiles of 16; 256
+  // new tokens after 8,192 (64 tiles x 128 steps) 74 us, 86 us; 512 after 8,192 105
+  // us, 162 us; 4,096 and as many keys 159 us, 315 us.
   // At d = 256 a CU holds four waves of them alone, and tiles pay sooner: 1,600 new
-  // tokens of 7 heads over one after 1,200 keys 99 us, 149 us in tiles of 16; 512
-  // alone 39.7 us, 35.0 us.
+  // tokens of 7 heads over one after 1,200 keys 99 us, 145 us in tiles of 16; 512
+  // after 1,200 65 us, 45 us, and alone 38 us, 26 us.
+  //
+  // The lengths are the device's: here and below, what the host chooses by is the
+  // keys that the table has room for.
   constexpr int kBigRows = 128;
   const int big_steps = a.d == 256 ? 3000 : 6144;
   const bool tiles = group <= 128 && (double)rows * a.kv_heads / 128 * ((longest + 63) / 64) >= big_steps;

@@ -347,7 +347,8 @@ int dw_hip_qlinear_global_avg_pool_u8(dw_hip_backend* be, const dw_hip_buffer* x
  * Quantize: s = max(floor(log2 max|x|) - 2 + 127, 0) and each element
  * x / 2^(s - 127) to the nearest, ties to even, 6 at most; 255 for a block
  * that holds an infinity or a NaN; elements behind a row's end are 0.
- * dtype: of x or y, F32 or F16 (f16 subnormals at their IEEE value).
+ * dtype: of x or y, F32 or F16 (f16 subnormals at their IEEE value); rows and k
+ * below 2^31.
  * Dequantize to F16 rounds to nearest even, and to F32 is exact where f32 holds
  * the value (scales of 2^126 and 2^127 with large elements give infinities). */
 int dw_hip_quantize_mxfp4(dw_hip_backend* be, int dtype, const dw_hip_buffer* x, dw_hip_buffer* q,
@@ -359,9 +360,10 @@ int dw_hip_dequantize_mxfp4(dw_hip_backend* be, int dtype, const dw_hip_buffer* 
  * (a_dtype F16, a_scales NULL) or MXFP4 rows with their scales (MXFP4).
  * c_dtype: of C and of the bias (may be NULL), F32 or F16.  Products are
  * exact and summed in f32 in an order of the library's own; bias and
- * activation (DW_ACT_*) are f32, and C is rounded once.  Elements of W and A
- * behind a row's k must be 0, as quantize writes them.  m and n at most 2^24,
- * k at most 2^22. */
+ * activation (DW_ACT_*) are f32, SiLU to 2^-22 of its value, and C is rounded
+ * once; terms and sums below 2^-126 may be lost.  Elements of W and A behind a
+ * row's k must be 0, as quantize writes them.  m and n at most 2^24, k at most
+ * 2^22. */
 int dw_hip_gemm_mxfp4(dw_hip_backend* be, int a_dtype, const dw_hip_buffer* a, const dw_hip_buffer* a_scales,
                       const dw_hip_buffer* w, const dw_hip_buffer* w_scales, const dw_hip_buffer* bias, int c_dtype,
                       dw_hip_buffer* c, size_t m, size_t n, size_t k, int act);
@@ -378,8 +380,10 @@ int dw_hip_gemm_mxfp4(dw_hip_backend* be, int a_dtype, const dw_hip_buffer* a, c
  * axes' pairs one axis after the other; 1: in turn among the axes that have
  * pairs left.  freq 0: e(i) = i / r; 1: e(i) = j / sections[axis(i)] with j
  * the pair's place among those of its axis.  positions [axes][tokens] int32,
- * any value; angles are formed in 64 bits.  rotary_dim <= 256, axes <= 8; base
- * is above 0, and one so small that an angle is no f64 number is refused. */
+ * any value; angles are formed in 64 bits, and what they are beyond whole turns
+ * is rounded to f32 (2^-25 of a turn).  tokens below 2^24, strides at most 2^24,
+ * heads and head_dim at most 4096, rotary_dim at most 256, axes at most 8; base is
+ * above 0, and one so small that an angle is no f64 number is refused. */
 int dw_hip_rope_axes(dw_hip_backend* be, int dtype, const dw_hip_buffer* x, size_t x_stride, size_t x_off,
                      dw_hip_buffer* y, size_t y_stride, size_t y_off, const dw_hip_buffer* positions, size_t tokens,
                      size_t heads, size_t head_dim, size_t rotary_dim, const size_t* sections, size_t axes, int order,
@@ -389,12 +393,16 @@ int dw_hip_rope_axes(dw_hip_backend* be, int dtype, const dw_hip_buffer* x, size
  * [num_pages][kv_heads][page_size] MXFP4 rows of head_dim elements, k_scales
  * and v_scales their scales (so dw_hip_dequantize_mxfp4 reads them as
  * num_pages * kv_heads * page_size rows).  page_size is a power of two, 16 to
- * 65536; head_dim 64, 128 or 256.  On the device, int32:
+ * 65536; head_dim 64, 128 or 256.  tokens below 2^24, strides at most 2^24, batch
+ * at most 65535, kv_heads at most 1024, num_pages below 2^31, max_pages * page_size
+ * at most 2^30.  On the device, int32:
  *   block_table [batch][max_pages]  page of each page_size tokens of a sequence
  *   q_start [batch + 1]   first new token (row of q, k, v) of each sequence,
  *                         ascending; rows from q_start[batch] on belong to none
  *   kv_len [batch]        tokens of each sequence, the new ones included
- * New token i of n of a sequence has position kv_len - n + i.
+ * New token i of n of a sequence has position kv_len - n + i.  Lists that say
+ * otherwise (starts that descend or pass the tokens, lengths of any int) give
+ * unspecified rows, never an access outside the buffers.
  *
  * Append writes the new tokens' keys and values (f16, kv_heads heads from
  * column k_off / v_off of rows of k_stride / v_stride elements), quantized
@@ -420,7 +428,12 @@ int dw_hip_kv_append_mxfp4(dw_hip_backend* be, const dw_hip_buffer* k, size_t k_
  * Values of the cache are read as f16: scales above 2^13, which append never
  * writes, may give infinities or NaN in the rows that see them.
  * Scores and sums are f32; p is rounded to f16 before it meets the values.
- * Rows of y that belong to no sequence are left as they were. */
+ * Rows of y that belong to no sequence are left as they were.
+ * heads at most 4096, tokens * heads at most 2^24, batch * heads at most 2^22;
+ * scale finite, also times log2(e).
+ * How the work is cut goes by max_pages * page_size, the keys that the table
+ * has room for: a call is fastest with a table as wide as its longest sequence
+ * (32 single tokens over 500 keys each: 10 us, 18 us with room for 131,072). */
 int dw_hip_attention_mxfp4(dw_hip_backend* be, const dw_hip_buffer* q, size_t q_stride, size_t q_off,
                            const dw_hip_buffer* k_cache, const dw_hip_buffer* k_scales, const dw_hip_buffer* v_cache,
                            const dw_hip_buffer* v_scales, const dw_hip_buffer* block_table,
