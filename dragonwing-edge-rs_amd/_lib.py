@@ -120,6 +120,10 @@ SIGNATURES = {
     "dw_hip_rope_axes": (I, [P, I, P, Z, Z, P, Z, Z, P, Z, Z, Z, Z, P, Z, I, I, I, C.c_double]),
     "dw_hip_kv_append_mxfp4": (I, [P, P, Z, Z, P, Z, Z] + [P] * 7 + [Z] * 7),
     "dw_hip_attention_mxfp4": (I, [P, P, Z, Z] + [P] * 8 + [Z] * 8 + [F, I, Z]),
+    "dw_hip_route_experts": (I, [P, I, P, Z, Z, P, P, P, Z, Z, Z, I, Z, Z, I, I, F]),
+    "dw_hip_order_experts": (I, [P, P, P, P, Z, Z]),
+    "dw_hip_gemm_mxfp4_experts": (I, [P, I, P, P, P, P, P, I, P, P, P, Z, Z, Z, Z, I, Z, I]),
+    "dw_hip_combine_experts": (I, [P, I, P, P, P, P, P, Z, Z, Z, Z]),
     "dw_hip_yolo_detect_tail": (I, [P, I, P, P, P, P, I, Z, I, I, P]),
     "dw_graph_from_onnx": (I, [P, Z, P]),
     "dw_onnx_inspect": (I, [P, Z, P, Z, P]),

@@ -1475,4 +1475,168 @@ int dw_hip_attention_mxfp4(dw_hip_backend* be, const dw_hip_buffer* q, size_t q_
   API_END
 }
 
+// A mixture of experts: the sizes that its calls share.
+static void check_experts(size_t slots, size_t experts, const char* what) {
+  if (!slots || !experts) dw::fail(DW_ERR_INVALID, std::string(what) + ": zero size");
+  if (slots > kMostMx || experts > 1024)
+    dw::fail(DW_ERR_UNSUPPORTED, std::string(what) + ": more than 2^24 slots or 1024 experts");
+}
+static void check_choices(size_t tokens, size_t top_k, size_t experts, const char* what) {
+  if (!tokens || !top_k) dw::fail(DW_ERR_INVALID, std::string(what) + ": zero size");
+  if (top_k > 32) dw::fail(DW_ERR_UNSUPPORTED, std::string(what) + ": top_k above 32");
+  if (tokens > kMostMx) dw::fail(DW_ERR_UNSUPPORTED, std::string(what) + ": more than 2^24 slots or 1024 experts");
+  check_experts(tokens * top_k, experts, what);
+}
+
+int dw_hip_route_experts(dw_hip_backend* be, int dtype, const dw_hip_buffer* logits, size_t stride, size_t off,
+                         const dw_hip_buffer* bias, dw_hip_buffer* ids, dw_hip_buffer* weights, size_t tokens,
+                         size_t experts, size_t top_k, int score, size_t groups, size_t top_groups, int group_best,
+                         int renorm, float scale) {
+  API_BEGIN
+  const size_t es = float_bytes(dtype, "route_experts");
+  check_choices(tokens, top_k, experts, "route_experts");
+  if (score != DW_SCORE_SOFTMAX && score != DW_SCORE_SIGMOID) dw::fail(DW_ERR_INVALID, "route_experts: unknown score");
+  if (!groups || !top_groups || top_groups > groups || groups > experts || experts % groups)
+    dw::fail(DW_ERR_INVALID, "route_experts: groups must divide the experts, top_groups be 1 to groups");
+  if (top_k > top_groups * (experts / groups))
+    dw::fail(DW_ERR_INVALID, "route_experts: top_k is more than the experts that take part");
+  if (group_best != 1 && group_best != 2) dw::fail(DW_ERR_INVALID, "route_experts: group_best must be 1 or 2");
+  if (renorm != 0 && renorm != 1) dw::fail(DW_ERR_INVALID, "route_experts: renorm must be 0 or 1");
+  if (!std::isfinite(scale)) dw::fail(DW_ERR_INVALID, "route_experts: scale must be finite");
+  check_columns(stride, off, 1, experts, "route_experts: logits");
+  Backend* b = B(be);
+  std::lock_guard<std::mutex> lock(b->mu);
+  need_on(b, logits, tokens * stride * es, "route_experts: logits");
+  if (bias) need_on(b, bias, experts * 4, "route_experts: bias");
+  need_on(b, ids, tokens * top_k * 4, "route_experts: ids");
+  need_on(b, weights, tokens * top_k * 4, "route_experts: weights");
+  if (ids == weights || ids == logits || ids == bias || weights == logits || weights == bias)
+    dw::fail(DW_ERR_INVALID, "route_experts: buffers overlap");
+  dw::RouteArgs a{};
+  a.x = (const char*)logits->ptr + off * es;
+  a.bias = bias ? (const float*)bias->ptr : nullptr;
+  a.ids = (int32_t*)ids->ptr;
+  a.weights = (float*)weights->ptr;
+  a.stride = stride;
+  a.tokens = tokens;
+  a.half = dtype == DW_DTYPE_F16;
+  a.experts = (int)experts;
+  a.top_k = (int)top_k;
+  a.sigmoid = score == DW_SCORE_SIGMOID;
+  a.groups = (int)groups;
+  a.top_groups = (int)top_groups;
+  a.group_best = group_best;
+  a.renorm = renorm;
+  a.scale = scale;
+  dw::launch_route(b->stream, a);
+  API_END
+}
+
+int dw_hip_order_experts(dw_hip_backend* be, const dw_hip_buffer* ids, dw_hip_buffer* offsets, dw_hip_buffer* order,
+                         size_t slots, size_t experts) {
+  API_BEGIN
+  check_experts(slots, experts, "order_experts");
+  Backend* b = B(be);
+  std::lock_guard<std::mutex> lock(b->mu);
+  need_on(b, ids, slots * 4, "order_experts: ids");
+  need_on(b, offsets, (experts + 1) * 4, "order_experts: offsets");
+  need_on(b, order, slots * 4, "order_experts: order");
+  if (ids == offsets || ids == order || offsets == order) dw::fail(DW_ERR_INVALID, "order_experts: buffers overlap");
+  dw::OrderArgs a{};
+  a.ids = (const int32_t*)ids->ptr;
+  a.offsets = (int32_t*)offsets->ptr;
+  a.order = (int32_t*)order->ptr;
+  a.slots = (int)slots;
+  a.experts = (int)experts;
+  const size_t bytes = dw::order_space(a);
+  dw::launch_order(b->stream, a, bytes ? b->workspace(Backend::WS_ORDER, bytes) : nullptr);
+  API_END
+}
+
+int dw_hip_gemm_mxfp4_experts(dw_hip_backend* be, int a_dtype, const dw_hip_buffer* a, const dw_hip_buffer* a_scales,
+                              const dw_hip_buffer* w, const dw_hip_buffer* w_scales, const dw_hip_buffer* bias,
+                              int c_dtype, dw_hip_buffer* c, const dw_hip_buffer* offsets, const dw_hip_buffer* order,
+                              size_t slots, size_t experts, size_t n, size_t k, int act, size_t gather, int scatter) {
+  API_BEGIN
+  if (a_dtype != DW_DTYPE_F16 && a_dtype != DW_DTYPE_MXFP4)
+    dw::fail(DW_ERR_UNSUPPORTED, "gemm_mxfp4_experts: A must be f16 or MXFP4");
+  const size_t es = float_bytes(c_dtype, "gemm_mxfp4_experts: C");
+  if (act != DW_ACT_SWIGLU) check_act(act, "gemm_mxfp4_experts");
+  check_experts(slots, experts, "gemm_mxfp4_experts");
+  if (!n || !k) dw::fail(DW_ERR_INVALID, "gemm_mxfp4_experts: zero size");
+  if (n > kMostMx || k > kMostMx / 4) dw::fail(DW_ERR_UNSUPPORTED, "gemm_mxfp4_experts: n above 2^24 or k above 2^22");
+  if (act == DW_ACT_SWIGLU && n % 2) dw::fail(DW_ERR_INVALID, "gemm_mxfp4_experts: gated columns come in pairs");
+  if (gather && slots % gather) dw::fail(DW_ERR_INVALID, "gemm_mxfp4_experts: gather must divide the slots");
+  if (scatter != 0 && scatter != 1) dw::fail(DW_ERR_INVALID, "gemm_mxfp4_experts: scatter must be 0 or 1");
+  const bool mx = a_dtype == DW_DTYPE_MXFP4;
+  if (mx != (a_scales != nullptr))
+    dw::fail(DW_ERR_INVALID, "gemm_mxfp4_experts: scales of A for MXFP4 rows, and only for them");
+  if ((gather || scatter) && !order) dw::fail(DW_ERR_INVALID, "gemm_mxfp4_experts: rows by order need the order");
+  const size_t blocks = (k + 31) / 32, rows = gather ? slots / gather : slots;
+  if (rows * (mx ? blocks * 16 : (k + 7) / 8 * 16) > (size_t)1 << 36)
+    dw::fail(DW_ERR_UNSUPPORTED, "gemm_mxfp4_experts: A above 64 GiB");
+  Backend* b = B(be);
+  std::lock_guard<std::mutex> lock(b->mu);
+  need_on(b, a, mx ? rows * blocks * 16 : rows * k * 2, "gemm_mxfp4_experts: A");
+  if (mx) need_on(b, a_scales, rows * blocks, "gemm_mxfp4_experts: scales of A");
+  need_on(b, w, experts * n * blocks * 16, "gemm_mxfp4_experts: W");
+  need_on(b, w_scales, experts * n * blocks, "gemm_mxfp4_experts: scales of W");
+  if (bias) need_on(b, bias, experts * n * es, "gemm_mxfp4_experts: bias");
+  need_on(b, c, slots * (act == DW_ACT_SWIGLU ? n / 2 : n) * es, "gemm_mxfp4_experts: C");
+  need_on(b, offsets, (experts + 1) * 4, "gemm_mxfp4_experts: offsets");
+  if (order) need_on(b, order, slots * 4, "gemm_mxfp4_experts: order");
+  if (c == a || c == a_scales || c == w || c == w_scales || c == bias || c == offsets || c == order)
+    dw::fail(DW_ERR_INVALID, "gemm_mxfp4_experts: C is an operand");
+  dw::GemmExpertsArgs x{};
+  x.g.a = a->ptr;
+  x.g.as = mx ? (const uint8_t*)a_scales->ptr : nullptr;
+  x.g.w = (const uint8_t*)w->ptr;
+  x.g.ws = (const uint8_t*)w_scales->ptr;
+  x.g.bias = bias ? bias->ptr : nullptr;
+  x.g.c = c->ptr;
+  x.g.m = (int)slots;
+  x.g.n = (int)n;
+  x.g.k = (int)k;
+  x.g.act = act;
+  x.g.c_half = c_dtype == DW_DTYPE_F16;
+  x.offsets = (const int32_t*)offsets->ptr;
+  x.order = order ? (const int32_t*)order->ptr : nullptr;
+  x.experts = (int)experts;
+  x.gather = (int)gather;
+  x.scatter = scatter;
+  const size_t bytes = dw::gemm_experts_space(x);
+  dw::launch_gemm_experts(b->stream, x, bytes ? b->workspace(Backend::WS_GEMM4, bytes) : nullptr);
+  API_END
+}
+
+int dw_hip_combine_experts(dw_hip_backend* be, int dtype, const dw_hip_buffer* x, const dw_hip_buffer* ids,
+                           const dw_hip_buffer* weights, const dw_hip_buffer* base, dw_hip_buffer* y, size_t tokens,
+                           size_t top_k, size_t experts, size_t n) {
+  API_BEGIN
+  const size_t es = float_bytes(dtype, "combine_experts");
+  check_choices(tokens, top_k, experts, "combine_experts");
+  if (!n) dw::fail(DW_ERR_INVALID, "combine_experts: zero size");
+  if (n > kMostMx) dw::fail(DW_ERR_UNSUPPORTED, "combine_experts: n above 2^24");
+  Backend* b = B(be);
+  std::lock_guard<std::mutex> lock(b->mu);
+  need_on(b, x, tokens * top_k * n * es, "combine_experts: rows");
+  need_on(b, ids, tokens * top_k * 4, "combine_experts: ids");
+  need_on(b, weights, tokens * top_k * 4, "combine_experts: weights");
+  if (base) need_on(b, base, tokens * n * es, "combine_experts: base");
+  need_on(b, y, tokens * n * es, "combine_experts: output");
+  if (y == x || y == ids || y == weights) dw::fail(DW_ERR_INVALID, "combine_experts: the output is an input");
+  dw::CombineArgs a{};
+  a.x = x->ptr;
+  a.ids = (const int32_t*)ids->ptr;
+  a.weights = (const float*)weights->ptr;
+  a.base = base ? base->ptr : nullptr;
+  a.y = y->ptr;
+  a.tokens = tokens;
+  a.n = (int)n;
+  a.top_k = (int)top_k;
+  a.experts = (int)experts;
+  dw::launch_combine(b->stream, dtype, a);
+  API_END
+}
+
 }  // extern "C"

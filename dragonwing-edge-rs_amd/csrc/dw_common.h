@@ -29,7 +29,7 @@ __host__ __device__ inline int dtype_size(int dt) {
 }
 
 // Activations (match DW_ACT_*).
-enum Act : int { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2 };
+enum Act : int { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_SWIGLU = 3 };  // the last: products of experts only
 
 // Implicit-GEMM epilogues.
 enum Epi : int {
@@ -465,6 +465,52 @@ struct GemmMxArgs {
 // Bytes of workspace that the product wants.
 size_t gemm_mx_space(const GemmMxArgs& a);
 void launch_gemm_mx(hipStream_t st, GemmMxArgs a, void* space);
+
+// Mixtures of experts (k_experts.hip, k_gemm_experts.hip).  Slot t * top_k + j
+// is choice j of token t.
+struct RouteArgs {
+  const void* x;      // logits: row t from x + t * stride
+  const float* bias;  // [experts], or null
+  int32_t* ids;       // [tokens][top_k]
+  float* weights;     // [tokens][top_k]
+  size_t stride, tokens;
+  int half, experts, top_k, sigmoid, groups, top_groups, group_best, renorm;
+  float scale;
+};
+void launch_route(hipStream_t st, const RouteArgs& a);
+
+struct OrderArgs {
+  const int32_t* ids;  // [slots]
+  int32_t* offsets;    // [experts + 1]
+  int32_t* order;      // [slots]
+  int slots, experts;
+};
+// Bytes of workspace that the sort wants.
+size_t order_space(const OrderArgs& a);
+void launch_order(hipStream_t st, const OrderArgs& a, void* space);
+
+struct CombineArgs {
+  const void* x;         // [tokens * top_k][n]
+  const int32_t* ids;    // [tokens][top_k]
+  const float* weights;  // [tokens][top_k]
+  const void* base;      // [tokens][n], or null
+  void* y;               // [tokens][n]
+  size_t tokens;
+  int n, top_k, experts;
+};
+void launch_combine(hipStream_t st, int dtype, const CombineArgs& a);
+
+// g: W, its scales and bias those of all experts, one after the other; g.m is
+// C's rows (the slots).
+struct GemmExpertsArgs {
+  GemmMxArgs g;
+  const int32_t* offsets;  // [experts + 1]: first place of each expert among the sorted slots
+  const int32_t* order;    // [slots]: the slot of each place, where rows are gathered or scattered
+  int experts, gather, scatter;  // A's row is place, or order[place] / gather; C's is place, or order[place]
+  int few;                 // set by the launcher: experts of up to `few` rows are the other kernel's
+};
+size_t gemm_experts_space(const GemmExpertsArgs& a);
+void launch_gemm_experts(hipStream_t st, GemmExpertsArgs a, void* space);
 
 // Rotary positions: heads of x [tokens][x_stride] from column x_off, to y.
 struct RopeTable {

@@ -83,18 +83,6 @@ struct Split {
   long long pos, len;     // position of the tile's first token, keys of the sequence
 };
 
-// Sums up to and with each lane, in the lanes' registers (six steps of data
-// parallel primitives; each shuffle through LDS would cost several times one).
-__device__ __forceinline__ int sums_upto(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // the lane one to the left in its row of 16
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);   // two
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);   // four
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);   // eight
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // the last of row 0 to row 1, of 2 to 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // the last of row 1 to rows 2 and 3
-  return v;
-}
-
 // Which split number `mine` is; LAST: counted from the end.  Every item of a
 // sequence has the same number of steps; all steps over the splits wanted is a
 // split's length, so that long and short sequences share the chip evenly

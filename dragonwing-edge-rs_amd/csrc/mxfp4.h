@@ -42,6 +42,18 @@ __device__ __forceinline__ uint32_t max_of_quad(uint32_t v) {
   return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true));  // lanes 2 3 0 1
 }
 
+// Sums up to and with each lane, in the lanes' registers (six steps of data
+// parallel primitives; each shuffle through LDS would cost several times one).
+__device__ __forceinline__ int sums_upto(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // the lane one to the left in its row of 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);   // two
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);   // four
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);   // eight
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // the last of row 0 to row 1, of 2 to 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // the last of row 1 to rows 2 and 3
+  return v;
+}
+
 // The 8 values of one word, exact in f32.
 __device__ __forceinline__ void mx_decode8(uint32_t q, float scale, float* v) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));

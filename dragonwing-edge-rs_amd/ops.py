@@ -13,6 +13,8 @@ import numpy as np
 from ._lib import check, load
 
 ACT_NONE, ACT_RELU, ACT_SILU = 0, 1, 2
+ACT_SWIGLU = 3  # gemm_mxfp4_experts
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 DTYPE_F32, DTYPE_F16, DTYPE_I8, DTYPE_U8, DTYPE_I32 = 0, 1, 2, 3, 4
 DTYPE_MXFP4 = 5  # an operand of gemm_mxfp4
 
@@ -293,6 +295,36 @@ def attention_mxfp4(be, q, q_stride, q_off, k_cache, k_scales, v_cache, v_scales
                                         _h(v_scales), _h(block_table), _h(q_start), _h(kv_len), _h(y), tokens, batch,
                                         heads, kv_heads, head_dim, page_size, num_pages, max_pages, float(scale),
                                         int(causal), window))
+
+
+# --- a mixture of experts in 4 bits ---------------------------------------------
+
+def route_experts(be, dtype, logits, stride, off, bias, ids, weights, tokens, experts, top_k, score=SCORE_SOFTMAX,
+                  groups=1, top_groups=1, group_best=1, renorm=True, scale=1.0):
+    """Each token's top_k experts (ids int32, weights f32, both [tokens, top_k]) from its row of logits (dtype F32 or
+    F16); bias f32 [experts] or None (see dw_hip.h for scores and groups)."""
+    check(load().dw_hip_route_experts(be.handle, dtype, _h(logits), stride, off, _h(bias), _h(ids), _h(weights), tokens,
+                                      experts, top_k, score, groups, top_groups, group_best, int(renorm), float(scale)))
+
+
+def order_experts(be, ids, offsets, order, slots, experts):
+    """The slots sorted by expert: order int32 [slots], offsets int32 [experts + 1]."""
+    check(load().dw_hip_order_experts(be.handle, _h(ids), _h(offsets), _h(order), slots, experts))
+
+
+def gemm_mxfp4_experts(be, a_dtype, a, a_scales, w, w_scales, bias, c_dtype, c, offsets, order, slots, experts, n, k,
+                       act=ACT_NONE, gather=0, scatter=False):
+    """Rows times the MXFP4 weights w [experts, n, k] of their own expert; gather > 0 takes A's row order[r] / gather
+    for place r, scatter writes C's row order[r] (see dw_hip.h)."""
+    check(load().dw_hip_gemm_mxfp4_experts(be.handle, a_dtype, _h(a), _h(a_scales), _h(w), _h(w_scales), _h(bias),
+                                           c_dtype, _h(c), _h(offsets), _h(order), slots, experts, n, k, act, gather,
+                                           int(scatter)))
+
+
+def combine_experts(be, dtype, x, ids, weights, base, y, tokens, top_k, experts, n):
+    """y [tokens, n] = base (or None) + the weighted sum of each token's rows of x [tokens * top_k, n]."""
+    check(load().dw_hip_combine_experts(be.handle, dtype, _h(x), _h(ids), _h(weights), _h(base), _h(y), tokens, top_k,
+                                        experts, n))
 
 
 # --- layout and BN fold on the device -----------------------------------------

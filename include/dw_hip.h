@@ -97,6 +97,7 @@ int dw_hip_synchronize(dw_hip_backend* be);
 #define DW_ACT_NONE 0
 #define DW_ACT_RELU 1 /* ops::relu_f32 / relu_fp16 (ops.rs:189-220, 345-352) */
 #define DW_ACT_SILU 2 /* sigmoid_fp16 then mul_fp16 (ops.rs:1881, 1959)     */
+#define DW_ACT_SWIGLU 3 /* SiLU of even columns times odd ones; dw_hip_gemm_mxfp4_experts only */
 
 /* conv2d_f32_nhwc (crates/dragonwing-vulkan/src/ops.rs:1308; CPU
  * crates/dragonwing-cpu/src/ops.rs:1356-1436).  Direct convolution with the
@@ -440,6 +441,70 @@ int dw_hip_attention_mxfp4(dw_hip_backend* be, const dw_hip_buffer* q, size_t q_
                            const dw_hip_buffer* q_start, const dw_hip_buffer* kv_len, dw_hip_buffer* y, size_t tokens,
                            size_t batch, size_t heads, size_t kv_heads, size_t head_dim, size_t page_size,
                            size_t num_pages, size_t max_pages, float scale, int causal, size_t window);
+
+/* A mixture of experts in 4 bits (no counterpart in the reference): each
+ * token's experts from a router's logits, the choices sorted by expert, products
+ * with their own expert's MXFP4 weights, and the weighted sum of each token's
+ * rows.  Slot t * top_k + j is choice j of token t.  How many rows an expert
+ * has stays on the device; the calls follow each other without the host.
+ * tokens * top_k at most 2^24, experts at most 1024.
+ *
+ * Route: row t of the logits (dtype F32 or F16) is `experts` elements from
+ * column `off` of rows of `stride` elements.  With scores
+ *   p_e = exp(x_e) / sum exp(x) (DW_SCORE_SOFTMAX) or 1 / (1 + exp(-x_e))
+ *   (DW_SCORE_SIGMOID)
+ * a token's choices are the top_k experts of largest p_e + bias_e (bias f32
+ * [experts], or NULL), largest first and ties to the lowest index.  groups > 1:
+ * the experts are `groups` neighbourhoods of experts / groups, and only those of
+ * the top_groups groups of largest value take part, ties to the lowest index; a
+ * group's value is the largest p_e + bias_e in it (group_best 1) or the sum of
+ * the two largest (2; of the only one where one takes part).  Values are
+ * compared in 64 bits, without a bias and a sum as the logits themselves.
+ * ids int32 [tokens][top_k]; weights f32 [tokens][top_k], scale * p_e, with
+ * renorm scale * p_e / (the sum of the chosen p), formed in f32 (a difference d
+ * of two logits is rounded to it, d 2^-24 of the weight).  An expert
+ * whose logit or p_e + bias_e is NaN or -inf is never chosen; a choice that
+ * finds no expert has id -1 and weight 0 (all choices of a row that is -inf as a
+ * whole).  Experts of infinite logits share a softmax equally.  top_k at most
+ * 32 and at most top_groups * experts / groups; scale finite. */
+#define DW_SCORE_SOFTMAX 0
+#define DW_SCORE_SIGMOID 1
+int dw_hip_route_experts(dw_hip_backend* be, int dtype, const dw_hip_buffer* logits, size_t stride, size_t off,
+                         const dw_hip_buffer* bias, dw_hip_buffer* ids, dw_hip_buffer* weights, size_t tokens,
+                         size_t experts, size_t top_k, int score, size_t groups, size_t top_groups, int group_best,
+                         int renorm, float scale);
+
+/* The slots sorted by their expert, those of one expert ascending: ids int32
+ * [slots]; order int32 [slots] holds the slot of each place, and expert e's places are
+ * offsets[e] to offsets[e + 1] (int32 [experts + 1]).  Ids outside 0 to
+ * experts - 1 belong to no expert; places from offsets[experts] on hold -1. */
+int dw_hip_order_experts(dw_hip_backend* be, const dw_hip_buffer* ids, dw_hip_buffer* offsets, dw_hip_buffer* order,
+                         size_t slots, size_t experts);
+
+/* For each place r of an expert e, offsets[e] <= r < offsets[e + 1]:
+ *   C[r] = act(A[row] W[e]^T + bias[e])
+ * as dw_hip_gemm_mxfp4 computes it: W [experts][n] MXFP4 rows of k elements, bias
+ * [experts][n] or NULL, A f16 or MXFP4 rows.  A's row is r (gather 0; A has `slots` rows)
+ * or order[r] / gather (gather = top_k takes the tokens' rows; A has slots / gather
+ * rows, gather divides slots).  C's row is r, or order[r] with scatter (rows
+ * back at their slots).  order may be NULL where neither asks for it.  act:
+ * DW_ACT_*; with DW_ACT_SWIGLU n is even and C has n / 2 columns,
+ * silu(column 2i) * (column 2i + 1).  Rows of C that no place writes are left as
+ * they were.  Offsets that descend or pass `slots`, and orders of other numbers
+ * than slots, give unspecified rows, never an access outside the buffers.
+ * slots and n at most 2^24, k at most 2^22, A at most 64 GiB. */
+int dw_hip_gemm_mxfp4_experts(dw_hip_backend* be, int a_dtype, const dw_hip_buffer* a, const dw_hip_buffer* a_scales,
+                              const dw_hip_buffer* w, const dw_hip_buffer* w_scales, const dw_hip_buffer* bias,
+                              int c_dtype, dw_hip_buffer* c, const dw_hip_buffer* offsets, const dw_hip_buffer* order,
+                              size_t slots, size_t experts, size_t n, size_t k, int act, size_t gather, int scatter);
+
+/* y [tokens][n] = base [tokens][n] + sum_j weights[t][j] * x[t * top_k + j], over
+ * the choices j whose id is 0 to experts - 1 (the others' rows of x are not
+ * read).  dtype F32 or F16: of x, base (or NULL for 0) and y, which may be base.
+ * Sums are f32, choice after choice, and rounded once.  n at most 2^24. */
+int dw_hip_combine_experts(dw_hip_backend* be, int dtype, const dw_hip_buffer* x, const dw_hip_buffer* ids,
+                           const dw_hip_buffer* weights, const dw_hip_buffer* base, dw_hip_buffer* y, size_t tokens,
+                           size_t top_k, size_t experts, size_t n);
 
 /* YOLOv8 detect tail: the exported graph's ops after the head convs
  * (ultralytics Detect: DFL softmax over each side's reg_max bins and the 1x1
