@@ -3,6 +3,8 @@
 // rows, and tiles through LDS.
 #pragma once
 
+#include <type_traits>
+
 #include "dw_common.h"
 #include "mxfp4.h"
 
@@ -201,18 +203,14 @@ __device__ __forceinline__ f32x4 times_exact(bf16x8 v, f16x8 x, f32x4 acc) {
 // FEW: f16 rows, at most four, that a wave brings to LDS whole, an element
 // once: the matrix instruction's operand has 16 columns, and as loads of its
 // own each would cost 64 bytes a lane and step.
-// LIST: rows of A as a list has them (g.a and g.as from row 0 on, `from` the
-// first place), else g's own, one after the other.
-template <bool MX, int MT, int NT, bool FEW, bool LIST = false>
+template <bool MX, int MT, int NT, bool FEW>
 struct Rows {
   const GemmMxArgs& g;
   const uint8_t *w[NT], *ws[NT], *x[MT], *xs[MT];
   int lane, col, quad, blocks;
   uint8_t* few;  // this wave's rows in LDS
-  uint32_t line[FEW && LIST ? 4 : 1];  // their places in A
   static constexpr int kFewLine = 1024 + 16;
-  __device__ __forceinline__ Rows(const GemmMxArgs& args, int n0, uint8_t* lds, const RowList& list = {}, int from = 0)
-      : g(args), few(lds) {
+  __device__ __forceinline__ Rows(const GemmMxArgs& args, int n0, uint8_t* lds) : g(args), few(lds) {
     lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4, blocks = (g.k + 31) / 32;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -222,14 +220,10 @@ struct Rows {
     }
 #pragma unroll
     for (int u = 0; u < MT; ++u) {
-      size_t m = min(u * 16 + col, g.m - 1);
-      if constexpr (LIST) m = list.row(from + (int)m);
+      const size_t m = min(u * 16 + col, g.m - 1);
       x[u] = (const uint8_t*)g.a + (MX ? (m * blocks + quad) * 16 : (m * g.lda + quad * 32) * 2);
       xs[u] = MX ? g.as + m * blocks : nullptr;
     }
-    if constexpr (FEW && LIST)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) line[r] = list.row(from + min(r, g.m - 1));
   }
   // Four steps from s0; ALL: none of them reaches behind the end of K.
   template <bool EXACT, bool ALL>
@@ -260,7 +254,7 @@ struct Rows {
           if (r >= g.m) break;
           const int k = s0 * 128 + lane * 8;
           const uint4 v = ALL || (k < g.lda && s0 + lane / 16 < to)
-                              ? *(const uint4*)((const uint8_t*)g.a + ((size_t)(LIST ? line[LIST ? r : 0] : r) * g.lda + k) * 2)
+                              ? *(const uint4*)((const uint8_t*)g.a + ((size_t)r * g.lda + k) * 2)
                               : make_uint4(0, 0, 0, 0);
           *(uint4*)(few + r * kFewLine + lane * 16) = v;
         }
@@ -369,9 +363,11 @@ typedef __attribute__((address_space(3))) void* LdsPtr;
 // larger tiles share among more rows (128 x 128: 508 us).
 //
 // LIST: rows of A as a list has them, place m0 + i of it for row i of the tile
-// (g.a and g.as from row 0 on; at most 2^32 pieces of 16 bytes each).
-template <bool MX, int WM, int WN, int TM, int TN, bool LIST = false>
+// (g.a and g.as from row 0 on; at most 2^32 pieces of 16 bytes).  LOOSE: scale rows
+// of `blocks` bytes as they are, of any alignment.
+template <bool MX, int WM, int WN, int TM, int TN, bool LIST = false, bool LOOSE = false>
 struct Tile {
+  static_assert(LIST || !LOOSE, "with a list");
   static constexpr int kWaves = WM * WN, kRowsA = WM * TM * 16, kRowsW = WN * TN * 16;
   static constexpr int kDepth = MX ? 256 : 64, kParts = 2, kSpan = 512 / kDepth;
   static constexpr int kLineA = 128, kLineW = MX ? 128 : 32;  // bytes of a row and stage
@@ -387,7 +383,8 @@ struct Tile {
   uint8_t* lds;
   int m0, n0, wave, lane, col, quad, wm, wn;
   // a lane's pieces of the first stage, from the tile's rows (LIST: those of A in 16 bytes, from row 0)
-  uint32_t at_a[kLoadsA], at_w[kLoadsW], at_s[kLoadsS];
+  uint32_t at_a[kLoadsA], at_w[kLoadsW];
+  typename std::conditional<LOOSE, size_t, uint32_t>::type at_s[kLoadsS];
   const uint8_t *base_a, *base_w;
 
   // LDS keeps rows of A (and, for MXFP4 rows, of W) as they are, but the pieces
@@ -416,7 +413,10 @@ struct Tile {
 #pragma unroll
     for (int i = 0; i < kLoadsS; ++i) {
       const int r = scale_row(i);
-      if (LIST && MX && r < kRowsA)
+      if constexpr (LOOSE)
+        at_s[i] = (MX && r < kRowsA ? (size_t)list.row(m0 + min(r, g.m - 1 - m0))
+                                    : (size_t)min(r - (MX ? kRowsA : 0), g.n - 1 - n0)) * blocks;
+      else if (LIST && MX && r < kRowsA)
         at_s[i] = list.row(m0 + min(r, g.m - 1 - m0)) * (uint32_t)(g.pitch / 16);
       else
         at_s[i] = (uint32_t)((MX && r < kRowsA ? min(r, g.m - 1 - m0) : min(r - (MX ? kRowsA : 0), g.n - 1 - n0)) * g.pitch);
@@ -448,6 +448,29 @@ struct Tile {
       if (LAST && piece_w() >= pieces_w) p = (const uint8_t*)kZeros;
       __builtin_amdgcn_global_load_lds((const void*)p, (LdsPtr)(slot + kA + (wave * kLoadsW + i) * 1024), 16, 0, 0);
     }
+  }
+  // LOOSE: the scales of 512 elements through registers
+  // (loads to LDS want whole words); bytes behind a row's end are 127.
+  struct Loose16 {
+    uint4 v[kLoadsS];
+  };
+  __device__ __forceinline__ void fetch_scales(Loose16& r, int span) const {
+    const int blocks = (g.k + 31) / 32, b = span * 16;
+    if (b >= blocks) return;
+#pragma unroll
+    for (int i = 0; i < kLoadsS; ++i) {
+      const bool of_a = MX && scale_row(i) < kRowsA;  // the same for the wave
+      const uint8_t* p = (of_a ? g.as : g.ws + (size_t)n0 * blocks) + at_s[i];
+      if (b + 16 <= blocks)
+        __builtin_memcpy(&r.v[i], p + b, 16);
+      else
+        r.v[i] = scales16(p, b, blocks);
+    }
+  }
+  __device__ __forceinline__ void place_scales(uint8_t* __restrict__ slot, const Loose16& r, int span) const {
+    if (span * 16 >= (g.k + 31) / 32) return;
+#pragma unroll
+    for (int i = 0; i < kLoadsS; ++i) *(uint4*)(slot + scale_row(i) * 16) = r.v[i];
   }
   // The scales of 512 elements.
   __device__ __forceinline__ void load_scales(uint8_t* __restrict__ slot, int span) const {
@@ -541,16 +564,28 @@ struct Tile {
   __device__ __forceinline__ void stage(const uint8_t* __restrict__ cur, const uint8_t* __restrict__ scales,
                                         uint8_t* __restrict__ next, uint8_t* __restrict__ next_scales, int s,
                                         Operands& one, Operands& two, uint32_t* far, f32x4 (&acc)[TN][TM]) const {
+    Loose16 loose;
+    const bool turn = MORE != 0 && s % kSpan == 0;
     if constexpr (MORE != 0) {
-      if (s % kSpan == 0) load_scales(next_scales, s / kSpan + 1);
+      if (turn) {
+        if constexpr (LOOSE)
+          fetch_scales(loose, s / kSpan + 1);
+        else
+          load_scales(next_scales, s / kSpan + 1);
+      }
       load<MORE == 1>(next, s + 1);
     }
+    auto placed = [&] {
+      if constexpr (LOOSE && MORE != 0)
+        if (turn) place_scales(next_scales, loose, s / kSpan + 1);
+    };
     if constexpr (!kAhead) {
 #pragma unroll
       for (int i = 0; i < kParts; ++i) {
         read(cur, scales, s, i, one);
         products<EXACT>(one, i, far, acc);
       }
+      placed();
       return;
     }
     read(cur, scales, s, 0, one);
@@ -562,6 +597,7 @@ struct Tile {
       read(cur, scales, s, i, then);
       products<EXACT>(now, i - 1, far, acc);
     }
+    placed();
   }
   template <bool EXACT>
   __device__ __forceinline__ uint32_t sum(int from, int to, f32x4 (&acc)[TN][TM]) const {
@@ -575,8 +611,15 @@ struct Tile {
 #pragma unroll
       for (int t = 0; t < TN; ++t) two.fw[t] = 0x7070u;
     }
-    load_scales(lds + 2 * kStage, from / kSpan);
-    load<true>(lds, from);
+    if constexpr (LOOSE) {
+      Loose16 loose;
+      fetch_scales(loose, from / kSpan);
+      load<true>(lds, from);
+      place_scales(lds + 2 * kStage, loose, from / kSpan);
+    } else {
+      load_scales(lds + 2 * kStage, from / kSpan);
+      load<true>(lds, from);
+    }
     auto slot = [&](int i) { return lds + ((i - from) & 1) * kStage; };
     auto scales = [&](int span) { return lds + 2 * kStage + ((span - from / kSpan) & 1) * kScales; };
     int s = from;
@@ -601,7 +644,7 @@ struct Tile {
     bool odd = false;
     for (int i = threadIdx.x; i < (b1 - b0) * kRowsW; i += kWaves * 64) {
       const size_t r = min(n0 + i / (b1 - b0), g.n - 1), b = b0 + i % (b1 - b0);
-      if (g.ws[r * g.pitch + b] - 104u > 36u) {
+      if (g.ws[r * (LOOSE ? blocks : g.pitch) + b] - 104u > 36u) {
         const uint4 q = *(const uint4*)(g.w + (r * blocks + b) * 16);
         odd |= ((q.x | q.y | q.z | q.w) & 0x77777777u) != 0;
       }

@@ -21,7 +21,7 @@ struct Share {
 
 // Expert number `mine` of those that have 1 to `most` rows.  All lanes of a wave
 // ask for the same.
-__device__ __forceinline__ bool few_rows_expert(const GemmExpertsArgs& x, int most, int mine, Share* s) {
+__device__ __forceinline__ bool expert_of(const GemmExpertsArgs& x, int most, int mine, Share* s) {
   const int lane = threadIdx.x & 63;
   for (int e0 = 0; e0 < x.experts; e0 += 64) {
     const int e = e0 + lane;
@@ -69,45 +69,216 @@ __device__ __forceinline__ int row_of(const GemmExpertsArgs& x, int place) {
 
 constexpr int kFew = 16;
 
-template <bool MX, bool FEW>
-__device__ __forceinline__ void rows_of_expert(const GemmExpertsArgs& x, const GemmMxArgs& a, const Share& s, f32x4* sums) {
-  using R = Rows<MX, 1, 1, FEW, true>;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  const int n0 = blockIdx.x * 16, steps = ((a.k + 31) / 32 + 3) / 4, groups = (steps + 3) / 4;
-  const int from = groups * wave / waves * 4, to = min(steps, groups * (wave + 1) / waves * 4);
-  f32x4 acc[1][1];
-  const R r(a, n0, (uint8_t*)sums + wave * 4 * R::kFewLine, list_of(x), s.first);
-  const uint32_t odd = r.template sum<false>(from, to, acc);
-  if constexpr (!MX)
-    if (__ballot(odd != 0)) r.template sum<true>(from, to, acc);
-  f32x4 c = acc[0][0];
-  if (waves > 1) {
-    if (FEW) __syncthreads();  // the rows' place becomes the sums'
-    sums[wave * 64 + lane] = c;
-    __syncthreads();
-    if (wave) return;
-    for (int i = 1; i < waves; ++i) c += sums[i * 64 + lane];
-  }
-  const int m = lane & 15, n = n0 + (lane >> 4) * 4;
-  if (m >= s.count) return;
-  const int row = row_of(x, s.first + m);
-  if (row >= 0) store4<true>(a, row, n, c, bias4(a, n));
-}
+// Up to 16 rows of an expert times NT x 16 of its columns (rows of W), a share of
+// K, by one wave.
+//
+// Bound by the weights' bytes, read once, straight into the lanes that multiply
+// them: a lane's operand is a block of 32 elements, four lanes side by side read
+// 64 bytes of a row.  What carries it is bytes in flight: the loads of a batch (256
+// elements of K) are issued before the products of the batch ahead of it, and the
+// weights' first ones before the rows' list is known.  NT divides what is read of
+// A again.
+template <bool MX, int NT>
+struct Stream {
+  static constexpr int kSteps = 2;  // of 128 elements, a batch
+  struct Batch {
+    uint4 w[NT][kSteps];
+    uint32_t sw[NT][kSteps];
+    uint4 x[kSteps][MX ? 1 : 4];
+    uint32_t sx[kSteps];
+  };
+  const GemmMxArgs& g;
+  const uint8_t *w, *ws, *x, *xs;    // w, ws: the first row's, the same for all lanes
+  uint32_t at_w[NT], at_s[NT];  // this lane's rows behind it
+  int lane, col, quad, blocks, to;
 
-template <bool MX>
-__global__ __launch_bounds__(512) void expert_rows_kernel(GemmExpertsArgs x) {
-  extern __shared__ __align__(16) f32x4 sums[];
+  __device__ __forceinline__ Stream(const GemmMxArgs& args, int n0, int end) : g(args), to(end) {
+    lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4, blocks = (g.k + 31) / 32;
+    w = g.w + (size_t)n0 * blocks * 16;
+    ws = g.ws + (size_t)n0 * blocks;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {  // rows behind the end are not stored
+      at_s[t] = min(t * 16 + col, g.n - 1 - n0) * blocks;
+      at_w[t] = (at_s[t] + quad) * 16;
+    }
+  }
+  __device__ __forceinline__ void rows(const RowList& list, int first) {
+    const size_t m = list.row(first + min(col, g.m - 1));
+    x = (const uint8_t*)g.a + (MX ? (m * blocks + quad) * 16 : (m * g.lda + quad * 32) * 2);
+    xs = MX ? g.as + m * blocks : nullptr;
+  }
+  // Steps from which on a batch needs care.
+  __device__ __forceinline__ int whole() const { return min(to, MX ? blocks / 4 : g.lda / 128); }
+  // The scale bytes of step s of a row: those behind its end are 127, the factor one.
+  __device__ __forceinline__ uint32_t scale4(const uint8_t* row, int s) const {
+    uint32_t v = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v |= (s * 4 + j < blocks ? (uint32_t)row[s * 4 + j] : 127u) << (8 * j);
+    return v;
+  }
+  template <bool ALL>
+  __device__ __forceinline__ void load_w(Batch& b, int s) const {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i)
+        b.w[t][i] = ALL || (s + i < to && (s + i) * 4 + quad < blocks)
+                        ? *(const uint4*)(w + (size_t)(uint32_t)s * 64 + at_w[t] + i * 64)
+                        : make_uint4(0, 0, 0, 0);
+      if constexpr (ALL) {
+        __builtin_memcpy(b.sw[t], ws + (size_t)(uint32_t)s * 4 + at_s[t], 4 * kSteps);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) b.sw[t][i] = scale4(ws + at_s[t], s + i);
+      }
+    }
+  }
+  template <bool ALL>
+  __device__ __forceinline__ void load_x(Batch& b, int s) const {
+    if constexpr (MX) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i)
+        b.x[i][0] = ALL || (s + i < to && (s + i) * 4 + quad < blocks) ? *(const uint4*)(x + (size_t)(uint32_t)s * 64 + i * 64)
+                                                                     : make_uint4(0, 0, 0, 0);
+      if constexpr (ALL) {
+        __builtin_memcpy(b.sx, xs + (size_t)(uint32_t)s * 4, 4 * kSteps);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) b.sx[i] = scale4(xs, s + i);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          b.x[i][j] = ALL || (s + i < to && ((s + i) * 4 + quad) * 32 + j * 8 < g.lda)
+                          ? *(const uint4*)(x + (size_t)(uint32_t)s * 256 + i * 256 + j * 16)
+                          : make_uint4(0, 0, 0, 0);
+    }
+  }
+  template <bool EXACT>
+  __device__ __forceinline__ void multiply(const Batch& b, uint32_t* odd, f32x4 (&acc)[NT]) const {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const uint4 q = b.w[t][i];
+        if constexpr (MX) {
+          const i32x8 p = {(int)q.x, (int)q.y, (int)q.z, (int)q.w, 0, 0, 0, 0};
+          const uint4 y = b.x[i][0];
+          const i32x8 v = {(int)y.x, (int)y.y, (int)y.z, (int)y.w, 0, 0, 0, 0};
+          acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(p, v, acc[t], 4, 4, 0, (int)(b.sw[t][i] >> (8 * quad)), 0,
+                                                                   (int)(b.sx[i] >> (8 * quad)));
+        } else {
+          const uint32_t fb = __builtin_amdgcn_alignbit(b.sw[t][i], b.sw[t][i], 8 * quad + 9);  // byte `quad` to bits 30:23
+          const float f = __builtin_bit_cast(float, fb);
+          if constexpr (!EXACT) {
+            const uint32_t some = (q.x | q.y | q.z | q.w) & 0x77777777u;
+            *odd |= (fb & 0x7F800000u) - (104u << 23) > (36u << 23) ? some : 0u;
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const f16x8 v = __builtin_bit_cast(f16x8, b.x[i][j]);
+            if constexpr (EXACT)
+              acc[t] = times_exact(quarters_bf16(word(q, j), f), v, acc[t]);
+            else
+              acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eight_f16(word(q, j), f), v, acc[t], 0, 0, 0);
+          }
+        }
+      }
+  }
+  // Steps from `s` on; those of the first batch have their weights in `one`, if
+  // they are whole.
+  __device__ __forceinline__ uint32_t sum(int s, Batch& one, f32x4 (&acc)[NT]) const {
+    uint32_t odd = 0;
+    const int end = whole();
+    if (s + kSteps <= end) {
+      Batch two;
+      load_x<true>(one, s);
+      // two batches a turn, each loaded ahead of the other's products
+      while (s + 3 * kSteps <= end) {
+        load_w<true>(two, s + kSteps), load_x<true>(two, s + kSteps);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply<false>(one, &odd, acc);
+        __builtin_amdgcn_sched_barrier(0);
+        load_w<true>(one, s + 2 * kSteps), load_x<true>(one, s + 2 * kSteps);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply<false>(two, &odd, acc);
+        __builtin_amdgcn_sched_barrier(0);
+        s += 2 * kSteps;
+      }
+      if (s + 2 * kSteps <= end) {
+        load_w<true>(two, s + kSteps), load_x<true>(two, s + kSteps);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply<false>(one, &odd, acc);
+        multiply<false>(two, &odd, acc);
+        s += 2 * kSteps;
+      } else {
+        multiply<false>(one, &odd, acc);
+        s += kSteps;
+      }
+    }
+#pragma unroll 1
+    for (; s < to; s += kSteps) {
+      load_w<false>(one, s), load_x<false>(one, s);
+      multiply<false>(one, &odd, acc);
+    }
+    return odd;
+  }
+  // The same in a form that holds for every factor of the weights.
+  __device__ __forceinline__ void sum_exact(int s, f32x4 (&acc)[NT]) const {
+    Batch b;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[t] = f32x4{};
+#pragma unroll 1
+    for (; s < to; s += kSteps) {
+      load_w<false>(b, s), load_x<false>(b, s);
+      multiply<true>(b, nullptr, acc);
+    }
+  }
+};
+
+// The waves of a workgroup share K, and their sums meet in LDS in order.
+constexpr int kRowWaves = 4;
+template <bool MX, int NT>
+__global__ __launch_bounds__(64 * kRowWaves) void expert_rows_kernel(GemmExpertsArgs x) {
+  __shared__ __align__(16) f32x4 sums[kRowWaves][NT][64];
+  using S = Stream<MX, NT>;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles = (x.g.n + 16 * NT - 1) / (16 * NT), item = blockIdx.x / tiles, tile = blockIdx.x - item * tiles;
+  const int n0 = tile * 16 * NT, steps = ((x.g.k + 31) / 32 + 3) / 4, batches = (steps + S::kSteps - 1) / S::kSteps;
+  const int from = batches * wave / kRowWaves * S::kSteps, to = min(steps, batches * (wave + 1) / kRowWaves * S::kSteps);
   Share s;
-  if (!few_rows_expert(x, kFew, blockIdx.y, &s)) return;
+  if (!expert_of(x, kFew, item, &s)) return;
   GemmMxArgs a = of_expert(x, s.expert, (x.g.k + 31) / 32);
   a.m = s.count;
-  if (!MX && s.count <= 4)
-    rows_of_expert<MX, true>(x, a, s, sums);
-  else
-    rows_of_expert<MX, false>(x, a, s, sums);
+  S stream(a, n0, to);
+  typename S::Batch first;
+  if (from + S::kSteps <= stream.whole()) stream.template load_w<true>(first, from);
+  stream.rows(list_of(x), s.first);
+  f32x4 acc[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) acc[t] = f32x4{};
+  const uint32_t odd = stream.sum(from, first, acc);
+  if constexpr (!MX)
+    if (__ballot(odd != 0)) stream.sum_exact(from, acc);
+#pragma unroll
+  for (int t = 0; t < NT; ++t) sums[wave][t][lane] = acc[t];
+  __syncthreads();
+  const int m = lane & 15, row = m < s.count ? row_of(x, s.first + m) : -1;
+  if (row < 0) return;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    if (t % kRowWaves != wave) continue;
+    f32x4 c = sums[0][t][lane];
+#pragma unroll
+    for (int i = 1; i < kRowWaves; ++i) c += sums[i][t][lane];
+    const int n = n0 + t * 16 + (lane >> 4) * 4;
+    store4<true>(a, row, n, c, bias4(a, n));
+  }
 }
 
-// --- experts of many rows -----------------------------------------------------------
+// --- experts of more rows -----------------------------------------------------------
 
 // Tile `id` of the grid: which expert's, and which rows and columns of it.
 template <class T>
@@ -149,14 +320,14 @@ __device__ __forceinline__ bool tile_of(const GemmExpertsArgs& x, int id, int ti
   return false;
 }
 
-template <bool MX, int WM, int WN, int TM, int TN>
+template <bool MX, int WM, int WN, int TM, int TN, bool LOOSE>
 __global__ __launch_bounds__(WM* WN * 64) void expert_tile_kernel(GemmExpertsArgs x, int tiles_n) {
-  using T = Tile<MX, WM, WN, TM, TN, true>;
+  using T = Tile<MX, WM, WN, TM, TN, true, LOOSE>;
   extern __shared__ __align__(16) uint8_t lds[];
   Share s;
   int m0, n0;
   if (!tile_of<T>(x, blockIdx.x, tiles_n, &s, &m0, &n0)) return;
-  GemmMxArgs a = of_expert(x, s.expert, x.g.pitch);
+  GemmMxArgs a = of_expert(x, s.expert, LOOSE ? (x.g.k + 31) / 32 : x.g.pitch);
   m0 += s.first;
   a.m = s.first + s.count;
   const int stages = (a.k + T::kDepth - 1) / T::kDepth;
@@ -181,11 +352,12 @@ __global__ __launch_bounds__(WM* WN * 64) void expert_tile_kernel(GemmExpertsArg
   }
 }
 
-// How a product is cut, and where its workspace lies.
+// How a product is cut, and where its workspace lies.  Which experts have how many
+// rows only the device knows: each kernel takes those of its size.
 struct Plan {
-  bool rows;   // experts of up to kFew rows apart
-  int height;  // of the others' tiles, square ones; 0: there are none
-  size_t tiles;  // of them at most
+  int height, width;  // of the tiles of experts of more than kFew rows; 0: there are none
+  size_t tiles;       // of them at most
+  bool pads;          // scales laid out anew
   size_t a_rows, rows_at, scales_a, scales_w, bytes;
 };
 Plan plan(const GemmExpertsArgs& x) {
@@ -197,37 +369,44 @@ Plan plan(const GemmExpertsArgs& x) {
     return at;
   };
   p.a_rows = x.gather ? g.m / x.gather : g.m;
-  p.rows = g.m <= kFew || g.m / x.experts <= 2 * kFew;
-  p.height = g.m <= kFew ? 0 : g.m / x.experts >= 256 ? 256 : 128;
-  if (p.height) {
+  if (g.m > kFew) {
+    const int mean = g.m / x.experts;
+    p.height = mean >= 192 ? 256 : mean >= 64 ? 128 : 64;
+    p.width = p.height == 64 && !g.as ? 128 : p.height;
     // whole tiles, and one that is not for each expert that has some
-    const size_t most = g.m / p.height + std::min(x.experts, p.rows ? g.m / (kFew + 1) : g.m);
-    p.tiles = most * ((g.n + p.height - 1) / p.height);
+    const size_t most = g.m / p.height + std::min(x.experts, g.m / (kFew + 1));
+    p.tiles = most * ((g.n + p.width - 1) / p.width);
     if (p.tiles >= (size_t)1 << 23)  // of up to 512 threads: a grid has under 2^32
       fail(DW_ERR_UNSUPPORTED, "gemm_mxfp4_experts: more than 2^23 tiles");
   }
   const size_t blocks = (g.k + 31) / 32, pitch = (blocks + 15) / 16 * 16;
   if (!g.as && g.k % 8) p.rows_at = take(p.a_rows * ((g.k + 7) / 8 * 8) * 2);
-  if (p.height && blocks % 16) {
-    if (g.as) p.scales_a = take(p.a_rows * pitch);
+  p.pads = g.as && p.height == 256 && blocks % 16;
+  if (p.pads) {
+    p.scales_a = take(p.a_rows * pitch);
     p.scales_w = take((size_t)x.experts * g.n * pitch);
   }
   return p;
 }
 
-template <bool MX>
+template <bool MX, int NT>
 void launch_expert_rows(hipStream_t st, const GemmExpertsArgs& x) {
-  const int tiles = (x.g.n + 15) / 16, groups = ((x.g.k + 31) / 32 + 15) / 16, items = std::min(x.experts, x.g.m);
-  int waves = 1;
-  while (waves < 8 && waves < groups && (long long)tiles * items * waves < 4096) waves *= 2;
-  const size_t lds = (size_t)waves * (MX ? 1024 : 4 * Rows<MX, 1, 1, true, true>::kFewLine);
-  hipLaunchKernelGGL(expert_rows_kernel<MX>, dim3((unsigned)tiles, (unsigned)items), dim3(64u * waves), lds, st, x);
+  const int tiles = (x.g.n + 16 * NT - 1) / (16 * NT);
+  hipLaunchKernelGGL((expert_rows_kernel<MX, NT>), dim3((unsigned)(tiles * std::min(x.experts, x.g.m))), dim3(64 * kRowWaves), 0, st, x);
 }
 
-template <bool MX, int WM, int WN, int TM, int TN>
+template <bool MX>
+void launch_expert_rows(hipStream_t st, const GemmExpertsArgs& x) {
+  if (MX ? (size_t)x.g.m * x.g.n >= (size_t)1 << 21 : x.g.m >= 64)
+    launch_expert_rows<MX, 4>(st, x);
+  else
+    launch_expert_rows<MX, 2>(st, x);
+}
+
+template <bool MX, int WM, int WN, int TM, int TN, bool LOOSE = true>
 void launch_expert_tiles(hipStream_t st, const GemmExpertsArgs& x, size_t tiles) {
-  using T = Tile<MX, WM, WN, TM, TN, true>;
-  auto* k = expert_tile_kernel<MX, WM, WN, TM, TN>;
+  using T = Tile<MX, WM, WN, TM, TN, true, LOOSE>;
+  auto* k = expert_tile_kernel<MX, WM, WN, TM, TN, LOOSE>;
   hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(WM * WN * 64), T::kLds, st, x, (x.g.n + T::kRowsW - 1) / T::kRowsW);
 }
 
@@ -245,30 +424,30 @@ void launch_gemm_experts(hipStream_t st, GemmExpertsArgs x, void* space) {
   auto groups = [](size_t units) { return (unsigned)std::min<size_t>((units + 255) / 256, 4096); };
   Pads pads{};
   pads.m = (int)p.a_rows, pads.k = g.k, pads.lda = g.lda, pads.blocks = blocks, pads.words = words;
-  GemmExpertsArgs few = x;
   if (!g.as && g.k % 8) {
     pads.x = (const uint16_t*)g.a;
-    g.a = few.g.a = pads.x_to = (uint16_t*)(base + p.rows_at);
+    g.a = pads.x_to = (uint16_t*)(base + p.rows_at);
     pads.first = groups(p.a_rows * (g.lda / 8));
   }
+  GemmExpertsArgs few = x;  // scales as they are
   unsigned others = 0;
-  if (p.height && blocks % 16) {
-    if (g.as) {
-      pads.s[0] = g.as, pads.rows[0] = p.a_rows;
-      g.as = (const uint8_t*)(pads.s_to[0] = (uint32_t*)(base + p.scales_a));
-      pads.first = groups(p.a_rows * words);
-    }
+  if (p.pads) {
+    pads.s[0] = g.as, pads.rows[0] = p.a_rows;
+    g.as = (const uint8_t*)(pads.s_to[0] = (uint32_t*)(base + p.scales_a));
+    pads.first = groups(p.a_rows * words);
     pads.s[1] = g.ws, pads.rows[1] = (size_t)x.experts * g.n;
     g.ws = (const uint8_t*)(pads.s_to[1] = (uint32_t*)(base + p.scales_w));
     others = groups(pads.rows[1] * words);
   }
   launch_pads(st, pads, others);
-  if (p.rows) g.as ? launch_expert_rows<true>(st, few) : launch_expert_rows<false>(st, few);
-  x.few = p.rows ? kFew : 0;
+  g.as ? launch_expert_rows<true>(st, few) : launch_expert_rows<false>(st, few);
+  x.few = kFew;
   if (p.height == 256)
-    g.as ? launch_expert_tiles<true, 2, 4, 8, 4>(st, x, p.tiles) : launch_expert_tiles<false, 2, 4, 8, 4>(st, x, p.tiles);
-  else if (p.height)
+    g.as ? launch_expert_tiles<true, 2, 4, 8, 4, false>(st, x, p.tiles) : launch_expert_tiles<false, 2, 4, 8, 4>(st, x, p.tiles);
+  else if (p.height == 128)
     g.as ? launch_expert_tiles<true, 2, 2, 4, 4>(st, x, p.tiles) : launch_expert_tiles<false, 2, 2, 4, 4>(st, x, p.tiles);
+  else if (p.height)
+    g.as ? launch_expert_tiles<true, 1, 4, 4, 1>(st, x, p.tiles) : launch_expert_tiles<false, 2, 2, 2, 4>(st, x, p.tiles);
   DW_HIP(hipGetLastError());
 }
 
