@@ -2,6 +2,8 @@
 // each token takes and with what weights, the choices sorted by expert, and
 // the weighted sum of a token's experts' rows.
 #include <algorithm>
+#include <type_traits>
+#include <utility>
 
 #include "dw_common.h"
 #include "mxfp4.h"
@@ -12,43 +14,38 @@ namespace {
 
 // --- routing --------------------------------------------------------------------
 
-// Over each row of 16 lanes, the result in all of them (rotations by 8, 4, 2
-// and 1 lanes).
-template <int BY>
-__device__ __forceinline__ uint32_t rotated(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + BY, 0xF, 0xF, true);
+// A lane's number moved by data-parallel primitives (within each row of 16 lanes).
+template <int CTRL>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
 }
-template <int BY>
-__device__ __forceinline__ float rotated(float v) {
-  return __builtin_bit_cast(float, rotated<BY>(__builtin_bit_cast(uint32_t, v)));
-}
-template <int BY>
-__device__ __forceinline__ double rotated(double v) {
-  const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
-  const unsigned long long lo = rotated<BY>((uint32_t)b), hi = rotated<BY>((uint32_t)(b >> 32));
-  return __builtin_bit_cast(double, lo | hi << 32);
+template <int CTRL>
+__device__ __forceinline__ float moved(float v) {
+  return __builtin_bit_cast(float, moved<CTRL>(__builtin_bit_cast(uint32_t, v)));
 }
 __device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
-__device__ __forceinline__ double larger(double a, double b) { return fmax(a, b); }
-template <typename C>
-__device__ __forceinline__ C max16(C v) {
-  v = larger(v, rotated<8>(v));
-  v = larger(v, rotated<4>(v));
-  v = larger(v, rotated<2>(v));
-  return larger(v, rotated<1>(v));
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return max(a, b); }
+// Over the L lanes of a token, the same result in all of them: exchanges with the
+// lane beside, two on, and mirrored in 8 and 16 lanes.
+template <int L, typename T, typename F>
+__device__ __forceinline__ T over(T v, F f) {
+  if constexpr (L >= 2) v = f(v, moved<0xB1>(v));
+  if constexpr (L >= 4) v = f(v, moved<0x4E>(v));
+  if constexpr (L >= 8) v = f(v, moved<0x141>(v));
+  if constexpr (L >= 16) v = f(v, moved<0x140>(v));
+  if constexpr (L == 64) {
+    v = f(v, __shfl_xor(v, 16));
+    v = f(v, __shfl_xor(v, 32));
+  }
+  return v;
 }
-template <typename C>
-__device__ __forceinline__ C sum16(C v) {
-  v += rotated<8>(v);
-  v += rotated<4>(v);
-  v += rotated<2>(v);
-  return v + rotated<1>(v);
+template <int L, typename T>
+__device__ __forceinline__ T largest(T v) {
+  return over<L>(v, [](T a, T b) { return larger(a, b); });
 }
-__device__ __forceinline__ uint32_t min16(uint32_t v) {
-  v = min(v, rotated<8>(v));
-  v = min(v, rotated<4>(v));
-  v = min(v, rotated<2>(v));
-  return min(v, rotated<1>(v));
+template <int L, typename T>
+__device__ __forceinline__ T total(T v) {
+  return over<L>(v, [](T a, T b) { return a + b; });
 }
 
 __device__ __forceinline__ float exponential(float x) { return expf(x); }
@@ -67,123 +64,477 @@ __device__ __forceinline__ void own_lds() {
 }
 
 constexpr int kMostTop = 32;
+constexpr float kNone = -INFINITY;  // of experts that are not chosen
 
-// Sixteen lanes a token, expert v * 16 + lane being value v of a lane.  C: the
-// type of the choice values: f32 where they are the logits themselves, else
-// f64, because scores plus biases may lie closer than f32 can tell.
-template <typename C, int V, bool GROUPS>
-__global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
-  extern __shared__ __align__(16) double route_lds[];
-  const float kNone = -INFINITY;
-  const int lane = threadIdx.x & 15;
-  const size_t t = (size_t)blockIdx.x * (blockDim.x / 16) + threadIdx.x / 16;
-  const bool real = t < a.tokens;
-  const size_t row = (real ? t : a.tokens - 1) * a.stride;
-  float x[V];
-  float top = kNone;
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = v * 16 + lane;
-    x[v] = kNone;
-    if (e < a.experts) {
-      const float l = a.half ? h2f_ieee(((const uint16_t*)a.x)[row + e]) : ((const float*)a.x)[row + e];
-      x[v] = l > kNone ? l : kNone;  // a NaN is never chosen
-    }
-    top = fmaxf(top, x[v]);
+// Whole numbers in the order of f32 numbers, and back.  Those of numbers above -inf
+// are above kLowest.
+constexpr uint32_t kLowest = 0x007FFFFFu;
+__device__ __forceinline__ uint32_t ordered(float f) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, f);
+  return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t k) {
+  return __builtin_bit_cast(float, k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+
+// Batcher's odd-even merges: the pairs that sort V numbers, in order.
+template <int V>
+struct Pairs {
+  int n = 0;
+  int first[V * 8] = {}, second[V * 8] = {};
+  constexpr Pairs() {
+    for (int p = 1; p < V; p *= 2)
+      for (int q = p; q >= 1; q /= 2)
+        for (int j = q % p; j + q < V; j += 2 * q)
+          for (int i = 0; i < q && i + j + q < V; ++i)
+            if ((i + j) / (2 * p) == (i + j + q) / (2 * p)) first[n] = i + j, second[n++] = i + j + q;
   }
-  top = max16(top);
-  C c[V];
-  constexpr bool kScores = sizeof(C) == 8;  // else choices are logits
-  if constexpr (kScores) {
-    C all = 1;
-    if (!a.sigmoid) {
-      all = 0;
+};
+// The keys of a lane, largest first.  (The pairs are expanded by the compiler's front
+// end: a register's number must be a constant.)
+template <int V, size_t... S>
+__device__ __forceinline__ void sort_down(uint32_t (&k)[V], std::index_sequence<S...>) {
+  constexpr Pairs<V> kPairs;
+  auto order = [&](uint32_t& a, uint32_t& b) {
+    const uint32_t c = max(a, b);
+    b = min(a, b), a = c;
+  };
+  (order(k[kPairs.first[S]], k[kPairs.second[S]]), ...);
+}
+template <int V>
+__device__ __forceinline__ void sort_down(uint32_t (&k)[V]) {
+  if constexpr (V > 1) sort_down(k, std::make_index_sequence<(size_t)Pairs<V>().n>());
+}
+
+// LDS of a wave in 8 bytes: f64 values of a token's experts and groups, its choices
+// and 64 experts to choose from, or f32 values of all its tokens.
+template <int L>
+__host__ __device__ __forceinline__ size_t route_space(const RouteArgs& a) {
+  const size_t n = a.experts + a.groups, one = n + (kMostTop + 64) / 2, all = n * (64 / L) / 2;
+  return one > all ? one : all;
+}
+
+// L lanes have a token's row, values lane * V to lane * V + V - 1 each.
+template <int L, int V>
+struct Router {
+  const RouteArgs& a;
+  int lane;    // of the token's
+  float x[V];  // logits; kNone for NaN and behind the end
+  float top;   // the largest, of a softmax
+
+  __device__ __forceinline__ Router(const RouteArgs& args, size_t row) : a(args), lane(threadIdx.x & (L - 1)) {
+    if (a.half)
+      load((const uint16_t*)a.x + row, x);
+    else
+      load((const float*)a.x + row, x);
+    top = kNone;
 #pragma unroll
-      for (int v = 0; v < V; ++v) all += x[v] > kNone ? below((C)x[v], (C)top) : (C)0;
-      all = sum16(all);
+    for (int v = 0; v < V; ++v) x[v] = fmaxf(x[v], kNone);  // a NaN is never chosen
+    if (!a.sigmoid) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) top = fmaxf(top, x[v]);
+      top = largest<L>(top);
     }
+  }
+  template <typename T>
+  __device__ __forceinline__ void load(const T* row, float (&to)[V]) const {
+    const int e = lane * V;
+    if (e + V <= a.experts) {
+      const Loose<T, V> l = load_loose<T, V>(row + e);
+#pragma unroll
+      for (int v = 0; v < V; ++v) to[v] = widen(l.v[v]);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) to[v] = e + v < a.experts ? widen(row[e + v]) : kNone;
+    }
+  }
+
+  // Values by which experts are chosen, scores and biases, and what a score may be off:
+  // in roundings (2^-24) of the largest score, a sigmoid by 4 (exponent, its product,
+  // sum, reciprocal), one of a softmax by those and the sum's V + 5.
+  __device__ __forceinline__ float values(const float (&bias)[V], float (&c)[V]) const {
+    constexpr float kLog2e = 1.44269504f;
+    float all = 1.0f;
+    if (!a.sigmoid) {
+      all = 0.0f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        c[v] = x[v] == top ? 1.0f : __builtin_amdgcn_exp2f((x[v] - top) * kLog2e);
+        all += x[v] > kNone ? c[v] : 0.0f;
+      }
+      all = __builtin_amdgcn_rcpf(total<L>(all));
+#pragma unroll
+      for (int v = 0; v < V; ++v) c[v] *= all;
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) c[v] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[v] * -kLog2e));
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) c[v] = x[v] > kNone ? fmaxf(c[v] + bias[v], kNone) : kNone;
+    return (a.sigmoid ? 5.0f : V + 10.0f) * 0x1p-24f * all;
+  }
+  // Whether values of this size (the larger of two magnitudes) that are `gap` apart may
+  // be in the other order: scores are off by `off`, and sums round once.
+  static __device__ __forceinline__ bool near(float gap, float size, float off, float keys) {
+    return !(gap > 2 * off + size * (0x1p-23f + keys));
+  }
+
+  // Leaves the values of the groups that are kept; true if values off by `off` might
+  // give others.  mine: LDS of this token.
+  __device__ __forceinline__ bool keep_groups(float (&c)[V], float off, float* mine) const {
+    const int size = a.experts / a.groups, each = size / V;
+    float dropped = kNone, kept = INFINITY, most = 0.0f;  // most: the largest magnitude in a sum
+    if (L >= 8 && L <= 16 && each * V == size && (each & (each - 1)) == 0) {
+      // a group is 1, 2, 4 or 8 lanes
+      float one = c[0], two = kNone;
+#pragma unroll
+      for (int v = 1; v < V; ++v) two = fmaxf(two, fminf(one, c[v])), one = fmaxf(one, c[v]);
+      auto join = [&](float o, float t) { two = fmaxf(fminf(one, o), fmaxf(two, t)), one = fmaxf(one, o); };
+      if (each >= 2) join(moved<0xB1>(one), moved<0xB1>(two));
+      if (each >= 4) join(moved<0x4E>(one), moved<0x4E>(two));
+      if (each >= 8) join(moved<0x141>(one), moved<0x141>(two));
+      const bool both = a.group_best == 2 && two > kNone;
+      const float y = both ? one + two : one;
+      most = fmaxf(one > kNone ? fabsf(one) : 0.0f, both ? fabsf(two) : 0.0f);
+      // lanes of groups that come before this one: those of the token in turn
+      int before = 0;
+      const int shift = __ffs(each) - 1, group = lane >> shift;
+      float z = y;
+#pragma unroll
+      for (int i = 1; i < L; ++i) {
+        z = next(z);
+        before += z > y || (z == y && ((lane + i) & (L - 1)) >> shift < group);
+      }
+      const bool in = before < a.top_groups * each;
+      kept = in ? y : INFINITY, dropped = in ? kNone : y;
+#pragma unroll
+      for (int v = 0; v < V; ++v) c[v] = in ? c[v] : kNone;
+    } else {
+      float* value = mine + a.experts;
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (lane * V + v < a.experts) mine[lane * V + v] = c[v];
+      own_lds();
+      for (int g = lane; g < a.groups; g += L) {
+        float one = kNone, two = kNone;
+        for (int i = 0, j = lane % size; i < size; ++i, j = j + 1 == size ? 0 : j + 1) {
+          const float y = mine[g * size + j];
+          two = fmaxf(two, fminf(one, y)), one = fmaxf(one, y);
+        }
+        const bool both = a.group_best == 2 && two > kNone;
+        value[g] = both ? one + two : one;
+        most = fmaxf(most, fmaxf(one > kNone ? fabsf(one) : 0.0f, both ? fabsf(two) : 0.0f));
+      }
+      own_lds();
+      for (int g = lane; g < a.groups; g += L) {
+        const float y = value[g];
+        int before = 0;
+        for (int h = 0; h < a.groups; ++h) before += value[h] > y || (value[h] == y && h < g);
+        if (before < a.top_groups) {
+          kept = fminf(kept, y);
+        } else {
+          dropped = fmaxf(dropped, y);
+          for (int i = 0; i < size; ++i) mine[g * size + i] = kNone;
+        }
+      }
+      own_lds();
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (lane * V + v < a.experts) c[v] = mine[lane * V + v];
+      own_lds();
+    }
+    dropped = largest<L>(dropped), kept = -largest<L>(-kept), most = largest<L>(most);
+    // two sums of two values each
+    return dropped > kNone && near(kept - dropped, 3 * most, 2 * off, 0.0f);
+  }
+  // The number of the token's next lane.
+  static __device__ __forceinline__ float next(float v) {
+    if constexpr (L == 16) return moved<0x12F>(v);  // a rotation to the right by 15
+    // 8 lanes: a rotation of all 16, and of the others' by 8, which the last lane takes
+    const float f = moved<0x12F>(v), g = moved<0x127>(v);
+    return (threadIdx.x & 7) == 7 ? g : f;
+  }
+
+  // The largest by keys of 32 bits: each lane sorts its own, and the largest first one
+  // is taken top_k times; choice j comes to lane j % L, id[j / L].  WHOLE: the values are
+  // f16 numbers and keys hold them and their expert, else a value's upper bits and
+  // the place in the lane, which leaves out log2 V bits of 24.  True if values, off by
+  // `off`, lie closer than keys tell apart: the chosen ones are then not below `least`
+  // (in lane 0).  KEEP: how many of a lane's keys may be taken.
+  static constexpr int kEach = kMostTop / L > 0 ? kMostTop / L : 1;
+  template <int KEEP, bool WHOLE>
+  __device__ __forceinline__ bool choose(const float (&c)[V], float off, int (&id)[kEach], float* least) const {
+    constexpr uint32_t kLow = V - 1;
+    uint32_t k[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int e = v * 16 + lane;
-      const C p = a.sigmoid ? 1 / (1 + exponential(-(C)x[v])) : below((C)x[v], (C)top) / all;
-      const C y = a.bias && e < a.experts ? p + (C)a.bias[e] : p;
-      c[v] = x[v] > kNone && y > (C)kNone ? y : (C)kNone;
+      const uint32_t e = lane * V + v;
+      // f16 numbers leave 13 bits of an f32 one; their zeros are equal
+      const uint32_t key = WHOLE ? (ordered(c[v] + 0.0f) & ~0x1FFFu) | (0x1FFFu - e) : (ordered(c[v]) & ~kLow) | (kLow - v);
+      k[v] = c[v] > kNone ? key : e;  // experts that are not chosen have keys of their own, too
     }
-  } else {
+    sort_down(k);
+    const int base = (threadIdx.x & 63) - lane;
+    uint32_t taken[kEach];
+    int owner[kEach];
+    bool twice = false;  // some token's largest key stood in two lanes
 #pragma unroll
-    for (int v = 0; v < V; ++v) c[v] = x[v];
-  }
-  if constexpr (GROUPS) {
-    // the groups' values from LDS, 16 at a time
-    const int size = a.experts / a.groups;
-    C* mine = (C*)route_lds + (size_t)(threadIdx.x / 16) * (a.experts + a.groups);
-    C* value = mine + a.experts;
+    for (int i = 0; i < kEach; ++i) {
+      taken[i] = 0, owner[i] = 0;
+      if (i * L >= a.top_k) continue;
+      const int most = min(L, a.top_k - i * L);
+#pragma unroll 1
+      for (int j = 0; j < most; ++j) {
+        const uint32_t first = largest<L>(k[0]);
+        const unsigned long long hits = __ballot(k[0] == first);
+        const bool here = lane == j;
+        if constexpr (!WHOLE) {
+          twice |= __popcll(hits) != 64 / L;
+          const int from = L == 64 ? __ffsll(hits) - 1 : __ffs((uint32_t)(hits >> base)) - 1;
+          owner[i] = here ? from : owner[i];
+        }
+        taken[i] = here ? first : taken[i];
+        // the owner's next key moves up (by masks: a choice between two of an array's
+        // numbers would become one number that is looked up)
+        const uint32_t moves = k[0] == first ? ~0u : 0u;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (v * 16 + lane < a.experts) mine[v * 16 + lane] = c[v];
-    own_lds();
-    for (int g = lane; g < a.groups; g += 16) {
-      C one = (C)kNone, two = (C)kNone;
-      for (int i = 0, j = lane % size; i < size; ++i, j = j + 1 == size ? 0 : j + 1) {
-        const C y = mine[g * size + j];
-        two = larger(two, y < one ? y : one);
-        one = larger(one, y);
+        for (int v = 0; v + 1 < KEEP; ++v) k[v] = (k[v + 1] & moves) | (k[v] & ~moves);
+        k[KEEP - 1] &= ~moves;
       }
-      value[g] = a.group_best == 2 && two > (C)kNone ? one + two : one;
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      id[i] = taken[i] <= kLowest ? -1 : WHOLE ? (int)(0x1FFFu - (taken[i] & 0x1FFFu)) : owner[i] * V + (int)(kLow - (taken[i] & kLow));
+    if constexpr (WHOLE) return false;
+    {
+      const int j = a.top_k - 1;
+      uint32_t of = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) of = j / L == i ? taken[i] : of;
+      of = __shfl(of, base + (j & (L - 1)));
+      const float v = unordered(of & ~kLow);
+      *least = of > kLowest && fabsf(v) < INFINITY ? v - (2 * off + fabsf(v) * 0x1p-22f) : kNone;
+    }
+    // each choice and the one before it, and the last one and the next that was not taken
+    const uint32_t next = largest<L>(k[0]);
+    bool close = twice;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (i * L >= a.top_k) continue;
+      const int j = i * L + lane;
+      // all lanes take part in both
+      const uint32_t beside = __shfl(taken[i], base + (lane ? lane - 1 : 0)), ahead = __shfl(taken[i > 0 ? i - 1 : 0], base + L - 1);
+      const uint32_t up = lane ? beside : ahead;
+      auto same = [&](uint32_t high, uint32_t low) {
+        const float h = unordered(high & ~kLow), l = unordered(low & ~kLow);
+        return low > kLowest && (off > 0.0f ? near(h - l, fmaxf(fabsf(h), fabsf(l)), off, V * 0x1p-23f) : h == l);
+      };
+      close |= j > 0 && j < a.top_k && same(up, taken[i]);
+      close |= j == a.top_k - 1 && same(taken[i], next);
+    }
+    return close;
+  }
+};
+
+// A token's choices by a whole wave, from values as they are compared: scores and biases
+// in 64 bits, or logits.  None is below `least`.  values: LDS for experts + groups of
+// them; ids: for kMostTop choices and 64 more.
+template <bool SCORES>
+__device__ __forceinline__ void choose_exactly(const RouteArgs& a, size_t row, float least, double* values, int* ids) {
+  const int lane = threadIdx.x & 63;
+  const double none = kNone;
+  auto logit = [&](int e) {
+    const float l = a.half ? h2f_ieee(((const uint16_t*)a.x)[row + e]) : ((const float*)a.x)[row + e];
+    return l > kNone ? l : kNone;
+  };
+  auto over_wave = [](double v, auto f) {
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) v = f(v, __shfl_xor(v, i));
+    return v;
+  };
+  auto most = [](double p, double q) { return p > q ? p : q; };
+  double top = none, all = 1;
+  if (SCORES && !a.sigmoid) {
+    for (int e = lane; e < a.experts; e += 64) top = most(top, logit(e));
+    top = over_wave(top, most);
+    all = 0;
+    for (int e = lane; e < a.experts; e += 64)
+      if (logit(e) > kNone) all += below((double)logit(e), top);
+    all = over_wave(all, [](double p, double q) { return p + q; });
+  }
+  for (int e = lane; e < a.experts; e += 64) {
+    const double x = logit(e);
+    double y = x;
+    if (SCORES) {
+      y = a.sigmoid ? 1 / (1 + exp(-x)) : below(x, top) / all;
+      if (a.bias) y += (double)a.bias[e];
+    }
+    values[e] = x > none && y > none ? y : none;
+  }
+  own_lds();
+  if (a.top_groups < a.groups) {
+    double* of = values + a.experts;
+    const int size = a.experts / a.groups;
+    for (int g = lane; g < a.groups; g += 64) {
+      double one = none, two = none;
+      for (int i = 0; i < size; ++i) {
+        const double y = values[g * size + i];
+        two = most(two, y < one ? y : one), one = most(one, y);
+      }
+      of[g] = a.group_best == 2 && two > none ? one + two : one;
     }
     own_lds();
-    for (int g = lane; g < a.groups; g += 16) {
-      const C y = value[g];
+    for (int g = lane; g < a.groups; g += 64) {
       int before = 0;
-      for (int h = 0; h < a.groups; ++h) before += value[h] > y || (value[h] == y && h < g);
+      for (int h = 0; h < a.groups; ++h) before += of[h] > of[g] || (of[h] == of[g] && h < g);
       if (before >= a.top_groups)
-        for (int i = 0; i < size; ++i) mine[g * size + i] = (C)kNone;
+        for (int i = 0; i < size; ++i) values[g * size + i] = none;
     }
     own_lds();
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (v * 16 + lane < a.experts) c[v] = mine[v * 16 + lane];
   }
-  // choice j and its logit in lane j % 16
-  int id[kMostTop / 16];
-  float logit[kMostTop / 16];
-  float best_logit = kNone;
-#pragma unroll
-  for (int i = 0; i < kMostTop / 16; ++i) id[i] = -1, logit[i] = kNone;
+  // those that may be chosen, usually one or two more than top_k: each counts the ones
+  // that come before it
+  int* some = ids + kMostTop;
+  double bound = least;
+  int n = 0;
+  for (int turn = 0; turn < 2; ++turn) {
+    n = 0;
+    for (int e0 = 0; e0 < a.experts; e0 += 64) {
+      const int e = e0 + lane;
+      const bool in = e < a.experts && values[e] > none && values[e] >= bound;
+      const unsigned long long all_in = __ballot(in);
+      const int at = n + __popcll(all_in & ((1ull << lane) - 1));
+      if (in && at < 64) some[at] = e;
+      n += __popcll(all_in);
+    }
+    own_lds();
+    if (n <= 64 || turn == 1) break;
+    // choice top_k of the lanes' largest has top_k - 1 of them before it
+    double best = none;
+    for (int e = lane; e < a.experts; e += 64) best = most(best, values[e]);
+    int before = 0;
+    for (int i = 0; i < 64; ++i) {
+      const double z = __shfl(best, i);
+      before += z > best || (z == best && i < lane);
+    }
+    bound = __shfl(best, __ffsll(__ballot(before == a.top_k - 1)) - 1);
+  }
+  if (n <= 64) {
+    if (lane < a.top_k) ids[lane] = -1;
+    own_lds();
+    if (lane < n) {
+      const int e = some[lane];
+      const double y = values[e];
+      int before = 0;
+      for (int i = 0; i < n; ++i) {
+        const double z = values[some[i]];
+        before += z > y || (z == y && some[i] < e);
+      }
+      if (before < a.top_k) ids[before] = e;
+    }
+    own_lds();
+    return;
+  }
   for (int j = 0; j < a.top_k; ++j) {
-    C best = c[0];
-    int at = 0;
+    double best = none;
+    int at = 0x10000;
+    for (int e = lane; e < a.experts; e += 64)
+      if (values[e] > best) best = values[e], at = e;
+    const double first = over_wave(best, most);
+    at = best == first ? at : 0x10000;
 #pragma unroll
-    for (int v = 1; v < V; ++v)
-      if (c[v] > best) best = c[v], at = v;
-    const C first = max16(best);
-    const uint32_t e = min16(best == first && first > (C)kNone ? (uint32_t)(at * 16 + lane) : ~0u);
-    if (__ballot(e != ~0u) == 0) break;  // the same for the wave
-    float l = kNone;
+    for (int i = 1; i < 64; i *= 2) at = min(at, __shfl_xor(at, i));
+    if (lane == 0) {
+      ids[j] = at < 0x10000 ? at : -1;
+      if (at < 0x10000) values[at] = none;
+    }
+    own_lds();
+  }
+}
+
+// L lanes a token.  SCORES: experts, or groups of them, are chosen by scores
+// and biases, else by the logits.  Scores and biases may lie closer than f32 can
+// tell: rows in which they do (some in a thousand, of scores that are no ties) are
+// decided again in 64 bits, rows of f32 logits by comparing these as they are.
+//
+// Bound by instructions: 32,768 f32 rows of 256 take 13 us by their logits (10.6 of
+// f16 ones, 7 us their bytes), 23 with sigmoids and biases, and 30 in 8 groups.  A
+// wave that decides one row again takes some us more than the others.  32,768 rows of 256 in 8 groups, biases, 8 of 4 groups chosen: see launch_route.
+template <int L, int V, bool SCORES, bool GROUPS>
+__global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
+  extern __shared__ __align__(16) double route_lds[];
+  const size_t t = (size_t)blockIdx.x * (blockDim.x / L) + threadIdx.x / L;
+  const bool real = t < a.tokens;
+  const size_t row = (real ? t : a.tokens - 1) * a.stride;
+  using R = Router<L, V>;
+  // of a wave: f64 values of one token and its choices, or f32 ones of each
+  double* wave = route_lds + (size_t)(threadIdx.x / 64) * route_space<L>(a);
+  int id[R::kEach];
+  float all = 1.0f, top;
+  {
+    const R r(a, row);
+    float c[V], off = 0.0f;
+    top = r.top;
+    if (!a.sigmoid && !a.renorm) {
+      all = 0.0f;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (e == (uint32_t)(v * 16 + lane)) l = x[v], c[v] = (C)kNone;
-    l = max16(l);
-    best_logit = fmaxf(best_logit, l);
-    if (e != ~0u && lane == (j & 15)) {
-      if (j < 16) id[0] = (int)e, logit[0] = l;
-      else id[1] = (int)e, logit[1] = l;
+      for (int v = 0; v < V; ++v) all += r.x[v] > kNone ? below(r.x[v], top) : 0.0f;
+      all = total<L>(all);
+    }
+    if constexpr (SCORES) {
+      float bias[V] = {};
+      if (a.bias) r.load(a.bias, bias);
+      off = r.values(bias, c);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) c[v] = r.x[v];
+    }
+    bool close = false;
+    float least = kNone;
+    if constexpr (GROUPS) close = r.keep_groups(c, off, (float*)wave + (size_t)(threadIdx.x & 63) / L * (a.experts + a.groups)) && SCORES;
+    auto choose = [&](auto whole) {
+      constexpr bool kWhole = decltype(whole)::value;
+      return V > 9 && a.top_k <= 8 ? r.template choose<(V > 9 ? 9 : V), kWhole>(c, off, id, &least)
+                                     : r.template choose<V, kWhole>(c, off, id, &least);
+    };
+    if (!SCORES && a.half) {
+      choose(std::true_type());
+    } else {
+      const bool groups = close;
+      close |= choose(std::false_type());
+      least = groups ? kNone : least;  // of groups that may be others
+    }
+    for (unsigned long long left = __ballot(close); left;) {
+      const int first = (__ffsll(left) - 1) / L * L;  // lane of the next token
+      int* ids = (int*)(wave + a.experts + a.groups);
+      own_lds();
+      choose_exactly<SCORES>(a, ((size_t)__builtin_amdgcn_readlane((int)(row >> 32), first) << 32) |
+                                    (uint32_t)__builtin_amdgcn_readlane((int)row, first),
+                             __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, least), first)), wave, ids);
+      if ((int)(threadIdx.x & 63) / L * L == first)
+#pragma unroll
+        for (int i = 0; i < R::kEach; ++i)
+          if (i * L + r.lane < a.top_k) id[i] = ids[i * L + r.lane];
+      left &= ~((L == 64 ? ~0ull : (1ull << (L & 63)) - 1) << first);
     }
   }
-  // the weights: renormalised ones relative to the largest chosen logit, so that
-  // they are sums of no vanishing terms
-  float w[kMostTop / 16], sum = 0.0f, all = 1.0f;
-  if (!a.sigmoid && !a.renorm) {
-    all = 0.0f;
+  // The weights, relative to the largest chosen logit where they are renormalised, so
+  // that none of the sums' terms vanish.
+  const int lane = threadIdx.x & (L - 1);
+  float logit[R::kEach], w[R::kEach], best = kNone, sum = 0.0f;
 #pragma unroll
-    for (int v = 0; v < V; ++v) all += x[v] > kNone ? below(x[v], top) : 0.0f;
-    all = sum16(all);
+  for (int i = 0; i < R::kEach; ++i) {
+    logit[i] = kNone;
+    if (i * L < a.top_k && id[i] >= 0)
+      logit[i] = a.half ? h2f_ieee(((const uint16_t*)a.x)[row + id[i]]) : ((const float*)a.x)[row + id[i]];
+    best = fmaxf(best, logit[i]);
   }
-  const float m = a.sigmoid ? fminf(best_logit, 0.0f) : a.renorm ? best_logit : top;
+  best = largest<L>(best);
+  const float m = a.sigmoid ? fminf(best, 0.0f) : a.renorm ? best : top;
 #pragma unroll
-  for (int i = 0; i < kMostTop / 16; ++i) {
+  for (int i = 0; i < R::kEach; ++i) {
     w[i] = 0.0f;
-    if (id[i] >= 0) {
+    if (i * L < a.top_k && id[i] >= 0) {
       if (!a.sigmoid)
         w[i] = below(logit[i], m);
       else if (a.renorm)
@@ -193,44 +544,43 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
     }
     sum += w[i];
   }
-  if (a.renorm) all = sum16(sum);
+  if (a.renorm) all = total<L>(sum);
   if (!real) return;
 #pragma unroll
-  for (int i = 0; i < kMostTop / 16; ++i) {
-    const int j = i * 16 + lane;
+  for (int i = 0; i < R::kEach; ++i) {
+    const int j = i * L + lane;
     if (j >= a.top_k) continue;
     a.ids[t * a.top_k + j] = id[i];
     a.weights[t * a.top_k + j] = id[i] >= 0 ? a.scale * (w[i] / all) : 0.0f;
   }
 }
 
-template <typename C, int V>
+template <int L, int V, bool SCORES>
 void launch_route_v(hipStream_t st, const RouteArgs& a) {
-  const int threads = a.experts <= 256 ? 256 : 64, rows = threads / 16;
+  const int rows = 256 / L;
   const dim3 grid((unsigned)((a.tokens + rows - 1) / rows));
-  if (a.groups > 1 && a.top_groups < a.groups)
-    hipLaunchKernelGGL((route_kernel<C, V, true>), grid, dim3(threads), (size_t)rows * (a.experts + a.groups) * sizeof(C), st,
-                       a);
-  else
-    hipLaunchKernelGGL((route_kernel<C, V, false>), grid, dim3(threads), 0, st, a);
+  auto* k = a.top_groups < a.groups ? route_kernel<L, V, SCORES, true> : route_kernel<L, V, SCORES, false>;
+  hipLaunchKernelGGL(k, grid, dim3(256), 4 * 8 * route_space<L>(a), st, a);
 }
 
-template <typename C>
-void launch_route_c(hipStream_t st, const RouteArgs& a) {
+// Up to 256 experts 16 a lane, so that a wave has as many tokens as it can: its
+// instructions are the bound.
+template <bool SCORES>
+void launch_route_s(hipStream_t st, const RouteArgs& a) {
   if (a.experts <= 16)
-    launch_route_v<C, 1>(st, a);
+    launch_route_v<4, 4, SCORES>(st, a);
   else if (a.experts <= 32)
-    launch_route_v<C, 2>(st, a);
+    launch_route_v<4, 8, SCORES>(st, a);
   else if (a.experts <= 64)
-    launch_route_v<C, 4>(st, a);
+    launch_route_v<4, 16, SCORES>(st, a);
   else if (a.experts <= 128)
-    launch_route_v<C, 8>(st, a);
+    launch_route_v<8, 16, SCORES>(st, a);
   else if (a.experts <= 256)
-    launch_route_v<C, 16>(st, a);
+    launch_route_v<16, 16, SCORES>(st, a);
   else if (a.experts <= 512)
-    launch_route_v<C, 32>(st, a);
+    launch_route_v<64, 8, SCORES>(st, a);
   else
-    launch_route_v<C, 64>(st, a);
+    launch_route_v<64, 16, SCORES>(st, a);
 }
 
 // --- the choices by expert ------------------------------------------------------
@@ -412,11 +762,10 @@ void launch_combine_t(hipStream_t st, const CombineArgs& a) {
 }  // namespace
 
 void launch_route(hipStream_t st, const RouteArgs& a) {
-  const bool kept = a.top_groups < a.groups;
-  if (a.bias || (kept && a.group_best == 2))
-    launch_route_c<double>(st, a);
+  if (a.bias || (a.top_groups < a.groups && a.group_best == 2))
+    launch_route_s<true>(st, a);
   else
-    launch_route_c<float>(st, a);
+    launch_route_s<false>(st, a);
   DW_HIP(hipGetLastError());
 }
 
