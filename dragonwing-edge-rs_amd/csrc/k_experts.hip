@@ -617,47 +617,77 @@ __global__ __launch_bounds__(kOrderThreads) void count_kernel(OrderArgs a, int p
   for (int e = threadIdx.x; e < a.experts; e += kOrderThreads) counts[(size_t)blockIdx.x * a.experts + e] = count[e];
 }
 
-// counts: those of each piece, or null where the workgroup counts them itself.
+// counts: those of each piece, or null where the workgroup counts them itself.  EACH:
+// a lane's slots, kept in registers; 0: any number, read twice.
+template <int EACH>
 __global__ __launch_bounds__(kOrderThreads) void order_kernel(OrderArgs a, int piece, const int* counts, int bits) {
   constexpr int kWaves = kOrderThreads / 64;
   __shared__ int all[kMostExperts], at[kMostExperts], sums[kWaves];
   __shared__ uint16_t wave_count[kWaves][kMostExperts];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int from = blockIdx.x * piece, to = min(from + piece, a.slots), pieces = gridDim.x;
+  // this wave's slots, in order
+  const int each = piece / kWaves, w0 = min(from + wave * each, to), w1 = min(w0 + each, to);
+  int id[EACH ? EACH : 1], rank[EACH ? EACH : 1];
+#pragma unroll
+  for (int u = 0; u < EACH; ++u) {
+    const int i = w0 + u * 64 + lane;
+    id[u] = i < w1 ? a.ids[i] : -1;
+  }
   all[tid] = at[tid] = 0;
-  for (int e = lane; e < kMostExperts; e += 64) wave_count[wave][e] = 0;
+  for (int e = lane; e < kMostExperts / 2; e += 64) ((uint32_t*)wave_count[wave])[e] = 0;
   __syncthreads();
+  // The number of this wave's slots ahead of lane's that have its id, and one more in
+  // the count of the id for each.
+  auto count = [&](int of) {
+    const bool valid = (uint32_t)of < (uint32_t)a.experts;
+    const unsigned long long same = same_id(valid ? of : 0, bits) & __ballot(valid);
+    const int ahead = __popcll(same & ((1ull << lane) - 1));
+    int before = 0;
+    if (valid) before = wave_count[wave][of];
+    own_lds();
+    if (valid && ahead == 0) wave_count[wave][of] = (uint16_t)(before + __popcll(same));
+    own_lds();
+    return valid ? before + ahead : -1;
+  };
+  if constexpr (EACH > 0) {
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) rank[u] = count(id[u]);
+  } else {
+    for (int i = w0 + lane; i < w1; i += 64) {
+      const int of = a.ids[i];
+      // two counts share a word
+      if ((uint32_t)of < (uint32_t)a.experts) atomicAdd((uint32_t*)wave_count[wave] + of / 2, 1u << (16 * (of & 1)));
+    }
+  }
   if (counts) {
-    if (tid < a.experts) {
+    // several threads an expert, each some of the pieces
+    const int several = kOrderThreads / a.experts, e = tid % a.experts, share = tid / a.experts;
+    if (share < several) {
       int before = 0, sum = 0;
 #pragma unroll 8
-      for (int p = 0; p < pieces; ++p) {
-        const int n = counts[(size_t)p * a.experts + tid];
-        if (p < (int)blockIdx.x) before += n;
+      for (int p = share; p < pieces; p += several) {
+        const int n = counts[(size_t)p * a.experts + e];
+        before += p < (int)blockIdx.x ? n : 0;
         sum += n;
       }
-      all[tid] = sum, at[tid] = before;
+      atomicAdd(&all[e], sum), atomicAdd(&at[e], before);
     }
-  } else {
+  } else if (pieces > 1) {
     count_ids(a, 0, from, at);
     count_ids(a, 0, a.slots, all);
   }
-  // this wave's slots, in order
-  const int each = piece / kWaves, w0 = min(from + wave * each, to), w1 = min(w0 + each, to);
-  for (int i = w0 + lane; i < w1; i += 64) {
-    const int id = a.ids[i];
-    if ((uint32_t)id < (uint32_t)a.experts) {
-      // two counts share a word
-      atomicAdd((uint32_t*)wave_count[wave] + id / 2, 1u << (16 * (id & 1)));
-    }
-  }
   __syncthreads();
+  if (pieces == 1)
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) all[tid] += wave_count[w][tid];
   // where each expert's begin, and where this workgroup's do
   const int mine = all[tid];
   const int upto = sums_upto(mine);
   if (lane == 63) sums[wave] = upto;
   __syncthreads();
   int begin = upto - mine, total = 0;
+#pragma unroll
   for (int w = 0; w < kWaves; ++w) {
     if (w < wave) begin += sums[w];
     total += sums[w];
@@ -666,30 +696,28 @@ __global__ __launch_bounds__(kOrderThreads) void order_kernel(OrderArgs a, int p
     a.offsets[tid] = begin;
     if (tid == a.experts - 1) a.offsets[a.experts] = total;
   }
-  int place = begin + at[tid];
-  __syncthreads();
-  for (int w = 0; w < kWaves; ++w) {  // of each wave: its first place
+  int ahead = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {  // of each wave: its first place, from the workgroup's on, below 2^16
     const int n = wave_count[w][tid];
-    // places are kept from the workgroup's first on, below 2^16
-    wave_count[w][tid] = (uint16_t)(place - begin - at[tid]);
-    place += n;
+    wave_count[w][tid] = (uint16_t)ahead;
+    ahead += n;
   }
   all[tid] = begin + at[tid];
   __syncthreads();
-  for (int i0 = w0; i0 < w1; i0 += 64) {
-    const int i = i0 + lane;
-    const int id = i < w1 ? a.ids[i] : -1;
-    const bool valid = (uint32_t)id < (uint32_t)a.experts;
-    const unsigned long long same = same_id(valid ? id : 0, bits) & __ballot(valid);
-    const int rank = __popcll(same & ((1ull << lane) - 1));
-    int first = 0;
-    if (valid) first = wave_count[wave][id];
-    own_lds();
-    if (valid && rank == 0) wave_count[wave][id] = (uint16_t)(first + __popcll(same));
-    own_lds();
-    if (valid) {
-      const int to_place = all[id] + first + rank;
-      if (to_place < a.slots) a.order[to_place] = i;
+  auto put = [&](int of, int place, int i) {
+    if (place >= 0 && all[of] + place < a.slots) a.order[all[of] + place] = i;
+  };
+  if constexpr (EACH > 0) {
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) {
+      const int of = rank[u] >= 0 ? id[u] : 0;
+      put(of, rank[u] >= 0 ? wave_count[wave][of] + rank[u] : -1, w0 + u * 64 + lane);
+    }
+  } else {
+    for (int i0 = w0; i0 < w1; i0 += 64) {
+      const int of = i0 + lane < w1 ? a.ids[i0 + lane] : -1, place = count(of);
+      put(place >= 0 ? of : 0, place, i0 + lane);
     }
   }
   // places behind the last
@@ -709,54 +737,75 @@ constexpr int kCountedApart = 4;  // pieces from which on a launch of its own co
 
 // --- the weighted sum -----------------------------------------------------------
 
-// N elements (16 bytes) a thread, the token's rows one after the other.
+// N neighbours of a token's row, from column i on: eight of its experts' rows in flight.
 template <typename T, int N>
+__device__ __forceinline__ void combine(const CombineArgs& a, size_t t, int i) {
+  const int32_t* ids = a.ids + t * a.top_k;
+  const float* weights = a.weights + t * a.top_k;
+  const T* x = (const T*)a.x + t * a.top_k * a.n + i;
+  float y[N] = {};
+  if (a.base) {
+    const Loose<T, N> v = load_loose<T, N>((const T*)a.base + t * a.n + i);
+#pragma unroll
+    for (int e = 0; e < N; ++e) y[e] = widen(v.v[e]);
+  }
+  int j0 = 0;
+  auto some = [&](auto rows) {
+    constexpr int kRows = decltype(rows)::value;
+    Loose<T, N> v[kRows];
+    float w[kRows];
+    bool in[kRows];
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      in[j] = (uint32_t)ids[j0 + j] < (uint32_t)a.experts;
+      w[j] = weights[j0 + j];
+    }
+    // rows of no expert are not read: another stands in, and counts nothing
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) v[j] = load_loose<T, N>(in[j] ? x + (size_t)(j0 + j) * a.n : (const T*)a.x + i);
+#pragma unroll
+    for (int j = 0; j < kRows; ++j)
+      if (in[j])
+#pragma unroll
+        for (int e = 0; e < N; ++e) y[e] = fmaf(w[j], widen(v[j].v[e]), y[e]);
+    j0 += kRows;
+  };
+  while (a.top_k - j0 >= 8) some(std::integral_constant<int, 8>());
+  if (a.top_k - j0 >= 4) some(std::integral_constant<int, 4>());
+  if (a.top_k - j0 >= 2) some(std::integral_constant<int, 2>());
+  if (a.top_k - j0 >= 1) some(std::integral_constant<int, 1>());
+  Loose<T, N> out;
+#pragma unroll
+  for (int e = 0; e < N; ++e) out.v[e] = narrow<T>(y[e]);
+  store_loose<T, N>((T*)a.y + t * a.n + i, out);
+}
+
+// N elements (16 bytes) a thread, the last ones of a row one by one.  Bound by the
+// rows' bytes.  WAVES: a wave has one token, whose ids and weights are scalars then.
+template <typename T, int N, bool WAVES>
 __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a) {
   const int i = (blockIdx.y * blockDim.x + threadIdx.x) * N;
   if (i >= a.n) return;
-  const bool whole = i + N <= a.n;
-  auto load = [&](const T* p) {
-    Loose<T, N> v = {};
-    if (whole)
-      v = load_loose<T, N>(p);
-    else
-      for (int e = 0; i + e < a.n; ++e) v.v[e] = p[e];
-    return v;
-  };
-  for (size_t t = (size_t)blockIdx.x * blockDim.y + threadIdx.y; t < a.tokens; t += (size_t)gridDim.x * blockDim.y) {
-    float y[N] = {};
-    if (a.base) {
-      const Loose<T, N> v = load((const T*)a.base + t * a.n + i);
-#pragma unroll
-      for (int e = 0; e < N; ++e) y[e] = widen(v.v[e]);
+  for (size_t t0 = (size_t)blockIdx.x * blockDim.y + threadIdx.y; t0 < a.tokens; t0 += (size_t)gridDim.x * blockDim.y) {
+    const size_t t = WAVES ? (size_t)__builtin_amdgcn_readfirstlane((int)t0) : t0;
+    if (i + N <= a.n) {
+      combine<T, N>(a, t, i);
+    } else {
+#pragma unroll 1
+      for (int e = i; e < a.n; ++e) combine<T, 1>(a, t, e);
     }
-    for (int j = 0; j < a.top_k; ++j) {
-      const size_t slot = t * a.top_k + j;
-      if ((uint32_t)a.ids[slot] >= (uint32_t)a.experts) continue;
-      const float w = a.weights[slot];
-      const Loose<T, N> v = load((const T*)a.x + slot * a.n + i);
-#pragma unroll
-      for (int e = 0; e < N; ++e) y[e] = fmaf(w, widen(v.v[e]), y[e]);
-    }
-    Loose<T, N> out;
-#pragma unroll
-    for (int e = 0; e < N; ++e) out.v[e] = narrow<T>(y[e]);
-    T* p = (T*)a.y + t * a.n + i;
-    if (whole)
-      store_loose<T, N>(p, out);
-    else
-      for (int e = 0; i + e < a.n; ++e) p[e] = out.v[e];
   }
 }
 
 template <typename T, int N>
 void launch_combine_t(hipStream_t st, const CombineArgs& a) {
   const int units = (a.n + N - 1) / N;
-  unsigned tx = 32;
+  unsigned tx = 16;
   while (tx < 256 && tx < (unsigned)units) tx *= 2;
   const dim3 block(tx, 256 / tx);
   const dim3 grid((unsigned)std::min<size_t>((a.tokens + block.y - 1) / block.y, 1 << 20), (units + tx - 1) / tx);
-  hipLaunchKernelGGL((combine_kernel<T, N>), grid, block, 0, st, a);
+  auto* k = tx >= 64 ? combine_kernel<T, N, true> : combine_kernel<T, N, false>;
+  hipLaunchKernelGGL(k, grid, block, 0, st, a);
 }
 
 }  // namespace
@@ -780,7 +829,8 @@ void launch_order(hipStream_t st, const OrderArgs& a, void* space) {
   while (1 << bits < a.experts) ++bits;
   int* counts = pieces < kCountedApart ? nullptr : (int*)space;
   if (counts) hipLaunchKernelGGL(count_kernel, dim3(pieces), dim3(kOrderThreads), 0, st, a, piece_of(a), counts);
-  hipLaunchKernelGGL(order_kernel, dim3(pieces), dim3(kOrderThreads), 0, st, a, piece_of(a), counts, bits);
+  auto* k = piece_of(a) == 4096 ? order_kernel<4> : order_kernel<0>;
+  hipLaunchKernelGGL(k, dim3(pieces), dim3(kOrderThreads), 0, st, a, piece_of(a), counts, bits);
   DW_HIP(hipGetLastError());
 }
 
