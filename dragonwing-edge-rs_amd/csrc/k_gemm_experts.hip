@@ -7,7 +7,7 @@
 #include <algorithm>
 
 #include "dw_hip.h"
-#include "gemm_mx.h"
+#include "gemm_mx_ring.h"
 #include "kv_lists.h"
 
 namespace dw {
@@ -320,36 +320,138 @@ __device__ __forceinline__ bool tile_of(const GemmExpertsArgs& x, int id, int ti
   return false;
 }
 
-template <bool MX, int WM, int WN, int TM, int TN, bool LOOSE>
+// The sums of rows from r0 of a part of a tile in LDS to C: four columns a lane, a
+// step's rows apart, kAtOnce rows whose reads and activations overlap.
+template <class OUT, int ACT, int kLine, int kStep, int kPart, int kTall, int kFull>
+__device__ __forceinline__ void store_part(const GemmMxArgs& a, const uint8_t* lds, const int* rows, int piece, int n, f32x4 bias) {
+  constexpr int kAtOnce = 4, N = ACT == ACT_SWIGLU ? 2 : 4;
+  static_assert(kPart % (kAtOnce * kStep) == 0, "whole steps");
+  const int line = ACT == ACT_SWIGLU ? a.n / 2 : a.n, c0 = ACT == ACT_SWIGLU ? n / 2 : n;  // n and a.n are even there
+  auto silu_of = [](float s) { return std::is_same<OUT, float>::value ? silu(s) : silu_f16(s); };
+#pragma unroll 1
+  for (int r0 = threadIdx.x / (kLine / 16); r0 < kPart; r0 += kAtOnce * kStep) {
+    int row[kAtOnce];
+    f32x4 v[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int r = r0 + i * kStep;
+      row[i] = rows[r / kTall * kFull + r % kTall];
+      v[i] = *(const f32x4*)(lds + r * kLine + (piece ^ (r & 7)) * 16) + bias;
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      Loose<OUT, N> y;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float s = ACT == ACT_SWIGLU ? silu_of(v[i][2 * j % 4]) * v[i][(2 * j + 1) % 4]
+                        : ACT == ACT_SILU ? silu_of(v[i][j])
+                        : ACT == ACT_RELU && v[i][j] < 0.0f ? 0.0f : v[i][j];  // a NaN stays
+        y.v[j] = narrow<OUT>(s);
+      }
+      OUT* to = (OUT*)a.c + (size_t)(uint32_t)row[i] * (uint32_t)line + c0;
+      if (row[i] < 0) continue;
+      if (c0 + N <= line)
+        store_loose<OUT, N>(to, y);
+      else
+#pragma unroll
+        for (int j = 0; j < N - 1; ++j)
+          if (c0 + j < line) to[j] = y.v[j];
+    }
+  }
+}
+
+// A tile's sums to C, through LDS (behind `rows`, which keeps C's rows), in kPieces
+// parts: a wave's stores cover rows of C whole, and the code of an activation is
+// short (written out for every sum, a 256 x 256 tile spent 17 us on it, a fourth of its
+// time at K = 4,096).  A row's pieces of 16 bytes stand at their index xor the row's,
+// so that eight rows' writes meet all banks.
+template <int WM, int WN, int TM, int TN, int kPieces>
+__device__ __forceinline__ void store_tile(const GemmMxArgs& a, uint8_t* lds, const int* rows, int n0, const f32x4 (&acc)[TN][TM]) {
+  constexpr int kLine = WN * TN * 64, kLanes = kLine / 16, kTall = TM / kPieces * 16, kStep = WM * WN * 64 / kLanes;
+  static_assert(TM % kPieces == 0, "whole parts");
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % WM, wn = wave / WM, col = lane & 15, quad = lane >> 4;
+  const int piece = threadIdx.x % kLanes, n = n0 + piece * 4;
+  const f32x4 bias = bias4(a, n);
+#pragma unroll 1
+  for (int part = 0; part < kPieces; ++part) {
+    if (part) __syncthreads();
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      if (p != part) continue;
+#pragma unroll
+      for (int u = 0; u < TM / kPieces; ++u)
+#pragma unroll
+        for (int t = 0; t < TN; ++t) {
+          const int r = wm * kTall + u * 16 + col;
+          *(f32x4*)(lds + r * kLine + (((wn * TN + t) * 4 + quad) ^ (r & 7)) * 16) = acc[t][p * (TM / kPieces) + u];
+        }
+    }
+    __syncthreads();
+    auto store = [&](auto out, auto act) {
+      store_part<decltype(out), act.value, kLine, kStep, WM * kTall, kTall, TM * 16>(a, lds, rows + part * kTall, piece, n, bias);
+    };
+    auto as = [&](auto act) { a.c_half ? store(uint16_t(), act) : store(float(), act); };
+    if (a.act == ACT_SWIGLU)
+      as(std::integral_constant<int, ACT_SWIGLU>());
+    else if (a.act == ACT_SILU)
+      as(std::integral_constant<int, ACT_SILU>());
+    else if (a.act == ACT_RELU)
+      as(std::integral_constant<int, ACT_RELU>());
+    else
+      as(std::integral_constant<int, ACT_NONE>());
+  }
+}
+
+// C's rows of a tile's, below 0 for none, to LDS.
+template <int ROWS>
+__device__ __forceinline__ void rows_of(const GemmExpertsArgs& x, int m0, int end, int* rows) {
+  if (threadIdx.x < ROWS) rows[threadIdx.x] = m0 + (int)threadIdx.x < end ? row_of(x, m0 + threadIdx.x) : -1;
+}
+
+template <bool MX, int WM, int WN, int TM, int TN>
 __global__ __launch_bounds__(WM* WN * 64) void expert_tile_kernel(GemmExpertsArgs x, int tiles_n) {
-  using T = Tile<MX, WM, WN, TM, TN, true, LOOSE>;
+  using T = Tile<MX, WM, WN, TM, TN, true, true>;
   extern __shared__ __align__(16) uint8_t lds[];
   Share s;
   int m0, n0;
   if (!tile_of<T>(x, blockIdx.x, tiles_n, &s, &m0, &n0)) return;
-  GemmMxArgs a = of_expert(x, s.expert, LOOSE ? (x.g.k + 31) / 32 : x.g.pitch);
+  GemmMxArgs a = of_expert(x, s.expert, (x.g.k + 31) / 32);
   m0 += s.first;
   a.m = s.first + s.count;
   const int stages = (a.k + T::kDepth - 1) / T::kDepth;
+  int* rows = (int*)(lds + T::kLds);
+  rows_of<T::kRowsA>(x, m0, a.m, rows);
   f32x4 acc[TN][TM];
   const T t(a, lds, m0, n0, list_of(x));
   const uint32_t far = t.template sum<false>(0, stages, acc);
   if constexpr (!MX) {
     if (__syncthreads_or(far != 0) && __syncthreads_or(t.outside(0, stages))) t.template sum<true>(0, stages, acc);
   }
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int m1 = m0 + wave % WM * TM * 16 + (lane & 15), n1 = n0 + wave / WM * TN * 16 + (lane >> 4) * 4;
-  f32x4 bias[TN];
-#pragma unroll
-  for (int i = 0; i < TN; ++i) bias[i] = bias4(a, n1 + i * 16);
-#pragma unroll
-  for (int u = 0; u < TM; ++u) {
-    if (m1 + u * 16 >= a.m) continue;
-    const int row = row_of(x, m1 + u * 16);
-    if (row < 0) continue;
-#pragma unroll
-    for (int i = 0; i < TN; ++i) store4<true>(a, row, n1 + i * 16, acc[i][u], bias[i]);
+  constexpr int kBytes = T::kRowsA * T::kRowsW * 4, kPieces = kBytes <= T::kLds ? 1 : kBytes <= 2 * T::kLds ? 2 : 4;
+  static_assert(kBytes <= kPieces * T::kLds && T::kRowsA <= WM * WN * 64, "fits");
+  store_tile<WM, WN, TM, TN, kPieces>(a, lds, rows, n0, acc);
+}
+
+template <bool MX>
+__global__ __launch_bounds__(512) void expert_ring_kernel(GemmExpertsArgs x, int tiles_n) {
+  using R = Ring<MX>;
+  extern __shared__ __align__(16) uint8_t lds[];
+  Share s;
+  int m0, n0;
+  if (!tile_of<R>(x, blockIdx.x, tiles_n, &s, &m0, &n0)) return;
+  GemmMxArgs a = of_expert(x, s.expert, x.g.pitch);
+  m0 += s.first;
+  a.m = s.first + s.count;
+  int* rows = (int*)(lds + R::kLds);
+  rows_of<R::kRowsA>(x, m0, a.m, rows);
+  f32x4 acc[R::TN][R::TM];
+  const R r(a, lds, m0, n0, list_of(x));
+  const uint32_t far = r.template sum<false>(acc);
+  if constexpr (!MX) {
+    if (__syncthreads_or(far != 0) && __syncthreads_or(r.outside())) r.template sum<true>(acc);
   }
+  static_assert(R::kRowsA * R::kRowsW * 4 <= 2 * R::kLds, "fits");
+  store_tile<2, 4, R::TM, R::TN, 2>(a, lds, rows, n0, acc);
 }
 
 // How a product is cut, and where its workspace lies.  Which experts have how many
@@ -357,9 +459,12 @@ __global__ __launch_bounds__(WM* WN * 64) void expert_tile_kernel(GemmExpertsArg
 struct Plan {
   int height, width;  // of the tiles of experts of more than kFew rows; 0: there are none
   size_t tiles;       // of them at most
-  bool pads;          // scales laid out anew
+  bool pads;          // rows of scales laid out anew, of whole 16 bytes
   size_t a_rows, rows_at, scales_a, scales_w, bytes;
 };
+// Columns / 16 of a workgroup of expert_rows_kernel.
+int tiles_a_row(const GemmMxArgs& g) { return (g.as ? (size_t)g.m * g.n >= (size_t)1 << 21 : g.m >= 64) ? 4 : 2; }
+
 Plan plan(const GemmExpertsArgs& x) {
   Plan p{};
   const GemmMxArgs& g = x.g;
@@ -379,11 +484,14 @@ Plan plan(const GemmExpertsArgs& x) {
     if (p.tiles >= (size_t)1 << 23)  // of up to 512 threads: a grid has under 2^32
       fail(DW_ERR_UNSUPPORTED, "gemm_mxfp4_experts: more than 2^23 tiles");
   }
+  const size_t rows_n = 16 * tiles_a_row(g);
+  if ((g.n + rows_n - 1) / rows_n * std::min(x.experts, g.m) >= (size_t)1 << 24)  // of 256 threads
+    fail(DW_ERR_UNSUPPORTED, "gemm_mxfp4_experts: a grid of more than 2^32 threads");
   const size_t blocks = (g.k + 31) / 32, pitch = (blocks + 15) / 16 * 16;
   if (!g.as && g.k % 8) p.rows_at = take(p.a_rows * ((g.k + 7) / 8 * 8) * 2);
-  p.pads = g.as && p.height == 256 && blocks % 16;
+  p.pads = p.height == 256 && blocks % 16;
   if (p.pads) {
-    p.scales_a = take(p.a_rows * pitch);
+    if (g.as) p.scales_a = take(p.a_rows * pitch);
     p.scales_w = take((size_t)x.experts * g.n * pitch);
   }
   return p;
@@ -397,17 +505,19 @@ void launch_expert_rows(hipStream_t st, const GemmExpertsArgs& x) {
 
 template <bool MX>
 void launch_expert_rows(hipStream_t st, const GemmExpertsArgs& x) {
-  if (MX ? (size_t)x.g.m * x.g.n >= (size_t)1 << 21 : x.g.m >= 64)
-    launch_expert_rows<MX, 4>(st, x);
-  else
-    launch_expert_rows<MX, 2>(st, x);
+  tiles_a_row(x.g) == 4 ? launch_expert_rows<MX, 4>(st, x) : launch_expert_rows<MX, 2>(st, x);
 }
 
-template <bool MX, int WM, int WN, int TM, int TN, bool LOOSE = true>
+template <bool MX, int WM, int WN, int TM, int TN>
 void launch_expert_tiles(hipStream_t st, const GemmExpertsArgs& x, size_t tiles) {
-  using T = Tile<MX, WM, WN, TM, TN, true, LOOSE>;
-  auto* k = expert_tile_kernel<MX, WM, WN, TM, TN, LOOSE>;
-  hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(WM * WN * 64), T::kLds, st, x, (x.g.n + T::kRowsW - 1) / T::kRowsW);
+  using T = Tile<MX, WM, WN, TM, TN, true, true>;
+  auto* k = expert_tile_kernel<MX, WM, WN, TM, TN>;
+  hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(WM * WN * 64), T::kLds + T::kRowsA * 4, st, x, (x.g.n + T::kRowsW - 1) / T::kRowsW);
+}
+
+template <bool MX>
+void launch_expert_rings(hipStream_t st, const GemmExpertsArgs& x, size_t tiles) {
+  hipLaunchKernelGGL(expert_ring_kernel<MX>, dim3((unsigned)tiles), dim3(512), Ring<MX>::kLds + 1024, st, x, (x.g.n + 255) / 256);
 }
 
 }  // namespace
@@ -429,12 +539,14 @@ void launch_gemm_experts(hipStream_t st, GemmExpertsArgs x, void* space) {
     g.a = pads.x_to = (uint16_t*)(base + p.rows_at);
     pads.first = groups(p.a_rows * (g.lda / 8));
   }
-  GemmExpertsArgs few = x;  // scales as they are
+  const GemmExpertsArgs few = x;  // scales as they are
   unsigned others = 0;
   if (p.pads) {
-    pads.s[0] = g.as, pads.rows[0] = p.a_rows;
-    g.as = (const uint8_t*)(pads.s_to[0] = (uint32_t*)(base + p.scales_a));
-    pads.first = groups(p.a_rows * words);
+    if (g.as) {
+      pads.s[0] = g.as, pads.rows[0] = p.a_rows;
+      g.as = (const uint8_t*)(pads.s_to[0] = (uint32_t*)(base + p.scales_a));
+      pads.first = groups(p.a_rows * words);
+    }
     pads.s[1] = g.ws, pads.rows[1] = (size_t)x.experts * g.n;
     g.ws = (const uint8_t*)(pads.s_to[1] = (uint32_t*)(base + p.scales_w));
     others = groups(pads.rows[1] * words);
@@ -443,7 +555,7 @@ void launch_gemm_experts(hipStream_t st, GemmExpertsArgs x, void* space) {
   g.as ? launch_expert_rows<true>(st, few) : launch_expert_rows<false>(st, few);
   x.few = kFew;
   if (p.height == 256)
-    g.as ? launch_expert_tiles<true, 2, 4, 8, 4, false>(st, x, p.tiles) : launch_expert_tiles<false, 2, 4, 8, 4>(st, x, p.tiles);
+    g.as ? launch_expert_rings<true>(st, x, p.tiles) : launch_expert_rings<false>(st, x, p.tiles);
   else if (p.height == 128)
     g.as ? launch_expert_tiles<true, 2, 2, 4, 4>(st, x, p.tiles) : launch_expert_tiles<false, 2, 2, 4, 4>(st, x, p.tiles);
   else if (p.height)

@@ -264,6 +264,40 @@ def test_products(backend, shape, kind):
         c.check(backend, bias, act, dtype)
 
 
+LONG = [([513, 300], 260, 1024), ([700, 17, 200], 516, 512), ([400], 300, 2048), ([257, 256, 255], 256, 1536), ([0, 900], 34, 4000)]
+
+
+@pytest.mark.parametrize("kind", ["f16", "mxfp4"])
+@pytest.mark.parametrize("shape", range(len(LONG)))
+def test_products_of_prompts(backend, shape, kind):
+    counts, n, k = LONG[shape]
+    for i, (none, gather, scatter, use, act, dtype) in enumerate([
+            (0, 2, False, True, 3, np.float16), (5, 0, True, False, 2, np.float32), (0, 0, False, False, 0, np.float16)]):
+        rng = np.random.default_rng(500 + shape * 10 + i)
+        c = Case(rng, counts, n, k, kind, none, gather, scatter)
+        c.check(backend, rng.normal(0, 1, (c.experts, n)).astype(dtype) if use else None, act, dtype)
+
+
+def test_products_of_prompts_with_weights_beyond_f16(backend):
+    rng = np.random.default_rng(17)
+    for k in (512, 544):
+        c = Case(rng, [300, 200], 280, k, "f16", gather=0)
+        q, s = c.q.reshape(c.experts, c.n, -1), c.s.reshape(c.experts, c.n, -1)
+        s[1, ::3, 1] = 1
+        s[1, 270, 9] = 200
+        c.w = ref.decode(q, s, c.k)
+        c.q, c.s = q.reshape(-1, q.shape[-1]), s.reshape(-1, s.shape[-1])
+        c.check(backend, None, 0, np.float32)
+
+
+def test_products_of_more_workgroups_than_a_grid_has_are_refused(backend):
+    experts, n, slots = 1024, 1 << 20, 1024
+    a, s, c = backend.alloc(slots * 64), backend.alloc(experts * n), backend.alloc(slots * n * 2)
+    w, offsets = backend.alloc(experts * n * 16), backend.alloc((experts + 1) * 4)
+    with pytest.raises(HipError, match="2\\^32 threads"):
+        ops.gemm_mxfp4_experts(backend, F16, a, None, w, s, None, F16, c, offsets, None, slots, experts, n, 32)
+
+
 @pytest.mark.parametrize("kind", ["f16", "mxfp4"])
 def test_products_of_many_slots_without_an_expert(backend, kind):
     rng = np.random.default_rng(12)
