@@ -240,41 +240,45 @@ struct Stream {
 
 // The waves of a workgroup share K, and their sums meet in LDS in order.
 constexpr int kRowWaves = 4;
-template <bool MX, int NT>
+// LOOP: workgroups take one piece of work after the other.
+template <bool MX, int NT, bool LOOP>
 __global__ __launch_bounds__(64 * kRowWaves) void expert_rows_kernel(GemmExpertsArgs x) {
   __shared__ __align__(16) f32x4 sums[kRowWaves][NT][64];
   using S = Stream<MX, NT>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tiles = (x.g.n + 16 * NT - 1) / (16 * NT), item = blockIdx.x / tiles, tile = blockIdx.x - item * tiles;
-  const int n0 = tile * 16 * NT, steps = ((x.g.k + 31) / 32 + 3) / 4, batches = (steps + S::kSteps - 1) / S::kSteps;
+  const int tiles = (x.g.n + 16 * NT - 1) / (16 * NT), steps = ((x.g.k + 31) / 32 + 3) / 4, batches = (steps + S::kSteps - 1) / S::kSteps;
   const int from = batches * wave / kRowWaves * S::kSteps, to = min(steps, batches * (wave + 1) / kRowWaves * S::kSteps);
-  Share s;
-  if (!expert_of(x, kFew, item, &s)) return;
-  GemmMxArgs a = of_expert(x, s.expert, (x.g.k + 31) / 32);
-  a.m = s.count;
-  S stream(a, n0, to);
-  typename S::Batch first;
-  if (from + S::kSteps <= stream.whole()) stream.template load_w<true>(first, from);
-  stream.rows(list_of(x), s.first);
-  f32x4 acc[NT];
+  for (unsigned id = blockIdx.x;; id += gridDim.x) {
+    const int item = id / tiles, n0 = (id - item * tiles) * 16 * NT;
+    Share s;
+    if (!expert_of(x, kFew, item, &s)) return;
+    GemmMxArgs a = of_expert(x, s.expert, (x.g.k + 31) / 32);
+    a.m = s.count;
+    S stream(a, n0, to);
+    typename S::Batch first;
+    if (from + S::kSteps <= stream.whole()) stream.template load_w<true>(first, from);
+    stream.rows(list_of(x), s.first);
+    f32x4 acc[NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) acc[t] = f32x4{};
-  const uint32_t odd = stream.sum(from, first, acc);
-  if constexpr (!MX)
-    if (__ballot(odd != 0)) stream.sum_exact(from, acc);
+    for (int t = 0; t < NT; ++t) acc[t] = f32x4{};
+    const uint32_t odd = stream.sum(from, first, acc);
+    if constexpr (!MX)
+      if (__ballot(odd != 0)) stream.sum_exact(from, acc);
 #pragma unroll
-  for (int t = 0; t < NT; ++t) sums[wave][t][lane] = acc[t];
-  __syncthreads();
-  const int m = lane & 15, row = m < s.count ? row_of(x, s.first + m) : -1;
-  if (row < 0) return;
+    for (int t = 0; t < NT; ++t) sums[wave][t][lane] = acc[t];
+    __syncthreads();
+    const int m = lane & 15, row = m < s.count ? row_of(x, s.first + m) : -1;
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    if (t % kRowWaves != wave) continue;
-    f32x4 c = sums[0][t][lane];
+    for (int t = 0; t < NT; ++t) {
+      if (row < 0 || t % kRowWaves != wave) continue;
+      f32x4 c = sums[0][t][lane];
 #pragma unroll
-    for (int i = 1; i < kRowWaves; ++i) c += sums[i][t][lane];
-    const int n = n0 + t * 16 + (lane >> 4) * 4;
-    store4<true>(a, row, n, c, bias4(a, n));
+      for (int i = 1; i < kRowWaves; ++i) c += sums[i][t][lane];
+      const int n = n0 + t * 16 + (lane >> 4) * 4;
+      store4<true>(a, row, n, c, bias4(a, n));
+    }
+    if (!LOOP) return;
+    __syncthreads();
   }
 }
 
@@ -462,6 +466,8 @@ struct Plan {
   bool pads;          // rows of scales laid out anew, of whole 16 bytes
   size_t a_rows, rows_at, scales_a, scales_w, bytes;
 };
+constexpr int kRare = 64;  // rows an expert has on average, from which on those of kFew are rare
+
 // Columns / 16 of a workgroup of expert_rows_kernel.
 int tiles_a_row(const GemmMxArgs& g) { return (g.as ? (size_t)g.m * g.n >= (size_t)1 << 21 : g.m >= 64) ? 4 : 2; }
 
@@ -476,7 +482,7 @@ Plan plan(const GemmExpertsArgs& x) {
   p.a_rows = x.gather ? g.m / x.gather : g.m;
   if (g.m > kFew) {
     const int mean = g.m / x.experts;
-    p.height = mean >= 192 ? 256 : mean >= 64 ? 128 : 64;
+    p.height = mean >= 192 ? 256 : mean >= kRare ? 128 : 64;
     p.width = p.height == 64 && !g.as ? 128 : p.height;
     // whole tiles, and one that is not for each expert that has some
     const size_t most = g.m / p.height + std::min(x.experts, g.m / (kFew + 1));
@@ -497,10 +503,18 @@ Plan plan(const GemmExpertsArgs& x) {
   return p;
 }
 
+// Where experts of few rows are rare, 512 workgroups look for them, all that run at a
+// time: the 8,192 of 65,536 x 4,096 x 4,096 for 128 experts take 9 us to find none.  Where
+// they are most of the work, a workgroup for each piece is faster (64 x 8 of 118 experts,
+// MXFP4 rows x 4,096 x 4,096: 199 us, 212 in a loop).
 template <bool MX, int NT>
 void launch_expert_rows(hipStream_t st, const GemmExpertsArgs& x) {
-  const int tiles = (x.g.n + 16 * NT - 1) / (16 * NT);
-  hipLaunchKernelGGL((expert_rows_kernel<MX, NT>), dim3((unsigned)(tiles * std::min(x.experts, x.g.m))), dim3(64 * kRowWaves), 0, st, x);
+  const unsigned all = (unsigned)((x.g.n + 16 * NT - 1) / (16 * NT) * std::min(x.experts, x.g.m));
+  constexpr bool kLoops = MX || NT == 4;  // kRare f16 rows come with NT = 4
+  if (kLoops && x.g.m / x.experts >= kRare)
+    hipLaunchKernelGGL((expert_rows_kernel<MX, NT, kLoops>), dim3(std::min(all, 512u)), dim3(64 * kRowWaves), 0, st, x);
+  else
+    hipLaunchKernelGGL((expert_rows_kernel<MX, NT, false>), dim3(all), dim3(64 * kRowWaves), 0, st, x);
 }
 
 template <bool MX>

@@ -278,6 +278,13 @@ def test_products_of_prompts(backend, shape, kind):
         c.check(backend, rng.normal(0, 1, (c.experts, n)).astype(dtype) if use else None, act, dtype)
 
 
+@pytest.mark.parametrize("kind", ["f16", "mxfp4"])
+def test_products_of_few_rows_beside_many_take_turns(backend, kind):
+    # more pieces of few rows than workgroups that look for them
+    rng = np.random.default_rng(18)
+    Case(rng, [300, 2, 1, 16], 16390, 96, kind, none=2).check(backend, None, 3, np.float16)
+
+
 def test_products_of_prompts_with_weights_beyond_f16(backend):
     rng = np.random.default_rng(17)
     for k in (512, 544):
