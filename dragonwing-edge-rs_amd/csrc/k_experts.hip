@@ -457,9 +457,9 @@ __device__ __forceinline__ void choose_exactly(const RouteArgs& a, size_t row, f
 // tell: rows in which they do (some in a thousand, of scores that are no ties) are
 // decided again in 64 bits, rows of f32 logits by comparing these as they are.
 //
-// Bound by instructions: 32,768 f32 rows of 256 take 13 us by their logits (10.6 of
-// f16 ones, 7 us their bytes), 23 with sigmoids and biases, and 30 in 8 groups.  A
-// wave that decides one row again takes some us more than the others.  32,768 rows of 256 in 8 groups, biases, 8 of 4 groups chosen: see launch_route.
+// Bound by instructions: 32,768 f32 rows of 256 take 13 us by their logits (10.7 of
+// f16 ones, 7 us their bytes), 23 with sigmoids and biases, and 33 to 35 in 8 groups.  A
+// wave that decides one row again takes some us more than the others.
 template <int L, int V, bool SCORES, bool GROUPS>
 __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
   extern __shared__ __align__(16) double route_lds[];
@@ -733,7 +733,10 @@ int piece_of(const OrderArgs& a) {
   return piece;
 }
 int pieces_of(const OrderArgs& a) { return (a.slots + piece_of(a) - 1) / piece_of(a); }
-constexpr int kCountedApart = 4;  // pieces from which on a launch of its own counts
+// Pieces from which on a launch of its own counts; below, each workgroup counts them all
+// by itself.  2,048 slots 6.5 us (8.4 with the launch), 12,288 8.2 to 9.3 (8.8), 16,384 9.0
+// (10.5 without), 32,000 9.8 (14.9).
+constexpr int kCountedApart = 4;
 
 // --- the weighted sum -----------------------------------------------------------
 

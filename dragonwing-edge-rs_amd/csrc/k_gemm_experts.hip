@@ -67,7 +67,7 @@ __device__ __forceinline__ int row_of(const GemmExpertsArgs& x, int place) {
 
 // --- experts of few rows ------------------------------------------------------------
 
-constexpr int kFew = 16;
+constexpr int kFew = 16;  // the columns of a matrix instruction
 
 // Up to 16 rows of an expert times NT x 16 of its columns (rows of W), a share of
 // K, by one wave.
@@ -77,7 +77,9 @@ constexpr int kFew = 16;
 // 64 bytes of a row.  What carries it is bytes in flight: the loads of a batch (256
 // elements of K) are issued before the products of the batch ahead of it, and the
 // weights' first ones before the rows' list is known.  NT divides what is read of
-// A again.
+// A again.  Times in us for 16 tokens of 8 of 64 experts x 2,816 x 2,048, 48 of them
+// hit: f16 rows 39.6, MXFP4 rows 34.4 (30.1 at a copy's rate); 64 tokens of 8 of 128 x
+// 4,096 x 4,096, 118 hit: 229 and 199 (215).
 template <bool MX, int NT>
 struct Stream {
   static constexpr int kSteps = 2;  // of 128 elements, a batch
@@ -238,7 +240,8 @@ struct Stream {
   }
 };
 
-// The waves of a workgroup share K, and their sums meet in LDS in order.
+// The waves of a workgroup share K, and their sums meet in LDS in order.  Of the 230 and
+// 200 us of 118 experts (above), two waves make 236 and 212, eight 295 and 239.
 constexpr int kRowWaves = 4;
 // LOOP: workgroups take one piece of work after the other.
 template <bool MX, int NT, bool LOOP>
@@ -246,7 +249,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void expert_rows_kernel(GemmExperts
   __shared__ __align__(16) f32x4 sums[kRowWaves][NT][64];
   using S = Stream<MX, NT>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tiles = (x.g.n + 16 * NT - 1) / (16 * NT), steps = ((x.g.k + 31) / 32 + 3) / 4, batches = (steps + S::kSteps - 1) / S::kSteps;
+  const int tiles = (x.g.n + 16 * NT - 1) / (16 * NT), steps = ((x.g.k + 31) / 32 + 3) / 4;
+  const int batches = (steps + S::kSteps - 1) / S::kSteps;
   const int from = batches * wave / kRowWaves * S::kSteps, to = min(steps, batches * (wave + 1) / kRowWaves * S::kSteps);
   for (unsigned id = blockIdx.x;; id += gridDim.x) {
     const int item = id / tiles, n0 = (id - item * tiles) * 16 * NT;
@@ -327,7 +331,8 @@ __device__ __forceinline__ bool tile_of(const GemmExpertsArgs& x, int id, int ti
 // The sums of rows from r0 of a part of a tile in LDS to C: four columns a lane, a
 // step's rows apart, kAtOnce rows whose reads and activations overlap.
 template <class OUT, int ACT, int kLine, int kStep, int kPart, int kTall, int kFull>
-__device__ __forceinline__ void store_part(const GemmMxArgs& a, const uint8_t* lds, const int* rows, int piece, int n, f32x4 bias) {
+__device__ __forceinline__ void store_part(const GemmMxArgs& a, const uint8_t* lds, const int* rows, int piece, int n,
+                                           f32x4 bias) {
   constexpr int kAtOnce = 4, N = ACT == ACT_SWIGLU ? 2 : 4;
   static_assert(kPart % (kAtOnce * kStep) == 0, "whole steps");
   const int line = ACT == ACT_SWIGLU ? a.n / 2 : a.n, c0 = ACT == ACT_SWIGLU ? n / 2 : n;  // n and a.n are even there
@@ -370,10 +375,12 @@ __device__ __forceinline__ void store_part(const GemmMxArgs& a, const uint8_t* l
 // time at K = 4,096).  A row's pieces of 16 bytes stand at their index xor the row's,
 // so that eight rows' writes meet all banks.
 template <int WM, int WN, int TM, int TN, int kPieces>
-__device__ __forceinline__ void store_tile(const GemmMxArgs& a, uint8_t* lds, const int* rows, int n0, const f32x4 (&acc)[TN][TM]) {
+__device__ __forceinline__ void store_tile(const GemmMxArgs& a, uint8_t* lds, const int* rows, int n0,
+                                           const f32x4 (&acc)[TN][TM]) {
   constexpr int kLine = WN * TN * 64, kLanes = kLine / 16, kTall = TM / kPieces * 16, kStep = WM * WN * 64 / kLanes;
   static_assert(TM % kPieces == 0, "whole parts");
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % WM, wn = wave / WM, col = lane & 15, quad = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % WM, wn = wave / WM;
+  const int col = lane & 15, quad = lane >> 4;
   const int piece = threadIdx.x % kLanes, n = n0 + piece * 4;
   const f32x4 bias = bias4(a, n);
 #pragma unroll 1
@@ -392,7 +399,8 @@ __device__ __forceinline__ void store_tile(const GemmMxArgs& a, uint8_t* lds, co
     }
     __syncthreads();
     auto store = [&](auto out, auto act) {
-      store_part<decltype(out), act.value, kLine, kStep, WM * kTall, kTall, TM * 16>(a, lds, rows + part * kTall, piece, n, bias);
+      store_part<decltype(out), act.value, kLine, kStep, WM * kTall, kTall, TM * 16>(a, lds, rows + part * kTall, piece,
+                                                                                     n, bias);
     };
     auto as = [&](auto act) { a.c_half ? store(uint16_t(), act) : store(float(), act); };
     if (a.act == ACT_SWIGLU)
@@ -431,7 +439,7 @@ __global__ __launch_bounds__(WM* WN * 64) void expert_tile_kernel(GemmExpertsArg
   if constexpr (!MX) {
     if (__syncthreads_or(far != 0) && __syncthreads_or(t.outside(0, stages))) t.template sum<true>(0, stages, acc);
   }
-  constexpr int kBytes = T::kRowsA * T::kRowsW * 4, kPieces = kBytes <= T::kLds ? 1 : kBytes <= 2 * T::kLds ? 2 : 4;
+  constexpr int kBytes = T::kRowsA * T::kRowsW * 4, kPieces = kBytes <= T::kLds ? 1 : 2;
   static_assert(kBytes <= kPieces * T::kLds && T::kRowsA <= WM * WN * 64, "fits");
   store_tile<WM, WN, TM, TN, kPieces>(a, lds, rows, n0, acc);
 }
@@ -459,7 +467,12 @@ __global__ __launch_bounds__(512) void expert_ring_kernel(GemmExpertsArgs x, int
 }
 
 // How a product is cut, and where its workspace lies.  Which experts have how many
-// rows only the device knows: each kernel takes those of its size.
+// rows only the device knows: expert_rows_kernel takes those of up to kFew, and the
+// tiles of the others have a height that suits the mean.  In us: 32 rows on average, f16 rows
+// 111 in tiles of 64 x 128 and 157 in 128 x 128, MXFP4 rows 79 in 64 x 64 and 90 in 128 x 128;
+// 128 rows 237 and 145 in 128 x 128, 262 and 177 in 256 x 256; 175 rows 466 and 228 in 128
+// x 128, 487 and 228 in 256 x 256; 1,024 rows 1,047 and 537 in 128 x 128, 813 and 389
+// in 256 x 256 with their scales laid out anew.
 struct Plan {
   int height, width;  // of the tiles of experts of more than kFew rows; 0: there are none
   size_t tiles;       // of them at most
@@ -468,7 +481,10 @@ struct Plan {
 };
 constexpr int kRare = 64;  // rows an expert has on average, from which on those of kFew are rare
 
-// Columns / 16 of a workgroup of expert_rows_kernel.
+// Columns / 16 of a workgroup of expert_rows_kernel: four where that leaves workgroups
+// enough (64 tokens of 8 of 118 experts x 4,096 x 4,096: f16 rows 230 us, with two 270, MXFP4
+// rows 200 and 213), two for fewer (a token of 8 experts x 2,816 x 2,048: 8.9 and 7.9 us,
+// with four 9.8 and 9.0).
 int tiles_a_row(const GemmMxArgs& g) { return (g.as ? (size_t)g.m * g.n >= (size_t)1 << 21 : g.m >= 64) ? 4 : 2; }
 
 Plan plan(const GemmExpertsArgs& x) {
@@ -526,12 +542,14 @@ template <bool MX, int WM, int WN, int TM, int TN>
 void launch_expert_tiles(hipStream_t st, const GemmExpertsArgs& x, size_t tiles) {
   using T = Tile<MX, WM, WN, TM, TN, true, true>;
   auto* k = expert_tile_kernel<MX, WM, WN, TM, TN>;
-  hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(WM * WN * 64), T::kLds + T::kRowsA * 4, st, x, (x.g.n + T::kRowsW - 1) / T::kRowsW);
+  hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(WM * WN * 64), T::kLds + T::kRowsA * 4, st, x,
+                     (x.g.n + T::kRowsW - 1) / T::kRowsW);
 }
 
 template <bool MX>
 void launch_expert_rings(hipStream_t st, const GemmExpertsArgs& x, size_t tiles) {
-  hipLaunchKernelGGL(expert_ring_kernel<MX>, dim3((unsigned)tiles), dim3(512), Ring<MX>::kLds + 1024, st, x, (x.g.n + 255) / 256);
+  hipLaunchKernelGGL(expert_ring_kernel<MX>, dim3((unsigned)tiles), dim3(512), Ring<MX>::kLds + 1024, st, x,
+                     (x.g.n + 255) / 256);
 }
 
 }  // namespace

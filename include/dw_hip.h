@@ -492,7 +492,10 @@ int dw_hip_order_experts(dw_hip_backend* be, const dw_hip_buffer* ids, dw_hip_bu
  * silu(column 2i) * (column 2i + 1).  Rows of C that no place writes are left as
  * they were.  Offsets that descend or pass `slots`, and orders of other numbers
  * than slots, give unspecified rows, never an access outside the buffers.
- * slots and n at most 2^24, k at most 2^22, A at most 64 GiB. */
+ * slots and n at most 2^24, k at most 2^22, A at most 64 GiB.  What takes more
+ * workgroups than a grid holds is refused: products with n * min(experts, slots) of 2^29
+ * and more may be, and those of 2^23 tiles of C.  SiLU holds to 2^-22 of its value
+ * for an f32 C, to 2^-17 for an f16 one. */
 int dw_hip_gemm_mxfp4_experts(dw_hip_backend* be, int a_dtype, const dw_hip_buffer* a, const dw_hip_buffer* a_scales,
                               const dw_hip_buffer* w, const dw_hip_buffer* w_scales, const dw_hip_buffer* bias,
                               int c_dtype, dw_hip_buffer* c, const dw_hip_buffer* offsets, const dw_hip_buffer* order,
