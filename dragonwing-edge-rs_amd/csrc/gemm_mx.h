@@ -372,11 +372,10 @@ typedef __attribute__((address_space(3))) void* LdsPtr;
 // larger tiles share among more rows (128 x 128: 508 us).
 //
 // LIST: rows of A as a list has them, place m0 + i of it for row i of the tile
-// (g.a and g.as from row 0 on; at most 2^32 pieces of 16 bytes).  LOOSE: scale rows
+// (g.a and g.as from row 0 on; at most 2^32 pieces of 16 bytes), and scale rows
 // of `blocks` bytes as they are, of any alignment.
-template <bool MX, int WM, int WN, int TM, int TN, bool LIST = false, bool LOOSE = false>
+template <bool MX, int WM, int WN, int TM, int TN, bool LIST = false>
 struct Tile {
-  static_assert(LIST || !LOOSE, "with a list");
   static constexpr int kWaves = WM * WN, kRowsA = WM * TM * 16, kRowsW = WN * TN * 16;
   static constexpr int kDepth = MX ? 256 : 64, kParts = 2, kSpan = 512 / kDepth;
   static constexpr int kLineA = 128, kLineW = MX ? 128 : 32;  // bytes of a row and stage
@@ -393,7 +392,7 @@ struct Tile {
   int m0, n0, wave, lane, col, quad, wm, wn;
   // a lane's pieces of the first stage, from the tile's rows (LIST: those of A in 16 bytes, from row 0)
   uint32_t at_a[kLoadsA], at_w[kLoadsW];
-  typename std::conditional<LOOSE, size_t, uint32_t>::type at_s[kLoadsS];
+  typename std::conditional<LIST, size_t, uint32_t>::type at_s[kLoadsS];
   const uint8_t *base_a, *base_w;
 
   // LDS keeps rows of A (and, for MXFP4 rows, of W) as they are, but the pieces
@@ -422,11 +421,9 @@ struct Tile {
 #pragma unroll
     for (int i = 0; i < kLoadsS; ++i) {
       const int r = scale_row(i);
-      if constexpr (LOOSE)
+      if constexpr (LIST)
         at_s[i] = (MX && r < kRowsA ? (size_t)list.row(m0 + min(r, g.m - 1 - m0))
                                     : (size_t)min(r - (MX ? kRowsA : 0), g.n - 1 - n0)) * blocks;
-      else if (LIST && MX && r < kRowsA)
-        at_s[i] = list.row(m0 + min(r, g.m - 1 - m0)) * (uint32_t)(g.pitch / 16);
       else
         at_s[i] = (uint32_t)((MX && r < kRowsA ? min(r, g.m - 1 - m0) : min(r - (MX ? kRowsA : 0), g.n - 1 - n0)) * g.pitch);
     }
@@ -458,7 +455,7 @@ struct Tile {
       __builtin_amdgcn_global_load_lds((const void*)p, (LdsPtr)(slot + kA + (wave * kLoadsW + i) * 1024), 16, 0, 0);
     }
   }
-  // LOOSE: the scales of 512 elements through registers
+  // LIST: the scales of 512 elements through registers
   // (loads to LDS want whole words); bytes behind a row's end are 127.
   struct Loose16 {
     uint4 v[kLoadsS];
@@ -487,8 +484,7 @@ struct Tile {
 #pragma unroll
     for (int i = 0; i < kLoadsS; ++i) {
       const bool of_a = MX && scale_row(i) < kRowsA;  // the same for the wave
-      const uint8_t* p = (of_a ? g.as + (LIST ? 0 : (size_t)m0 * g.pitch) : g.ws + (size_t)n0 * g.pitch) + at +
-                         (LIST && of_a ? (size_t)at_s[i] * 16 : (size_t)at_s[i]);
+      const uint8_t* p = (of_a ? g.as + (size_t)m0 * g.pitch : g.ws + (size_t)n0 * g.pitch) + at + at_s[i];
       __builtin_amdgcn_global_load_lds((const void*)p, (LdsPtr)(slot + (wave + i * kWaves) % (kScaleRows / 64) * 1024), 16,
                                        0, 0);
     }
@@ -577,7 +573,7 @@ struct Tile {
     const bool turn = MORE != 0 && s % kSpan == 0;
     if constexpr (MORE != 0) {
       if (turn) {
-        if constexpr (LOOSE)
+        if constexpr (LIST)
           fetch_scales(loose, s / kSpan + 1);
         else
           load_scales(next_scales, s / kSpan + 1);
@@ -585,7 +581,7 @@ struct Tile {
       load<MORE == 1>(next, s + 1);
     }
     auto placed = [&] {
-      if constexpr (LOOSE && MORE != 0)
+      if constexpr (LIST && MORE != 0)
         if (turn) place_scales(next_scales, loose, s / kSpan + 1);
     };
     if constexpr (!kAhead) {
@@ -620,7 +616,7 @@ struct Tile {
 #pragma unroll
       for (int t = 0; t < TN; ++t) two.fw[t] = 0x7070u;
     }
-    if constexpr (LOOSE) {
+    if constexpr (LIST) {
       Loose16 loose;
       fetch_scales(loose, from / kSpan);
       load<true>(lds, from);
@@ -653,7 +649,7 @@ struct Tile {
     bool odd = false;
     for (int i = threadIdx.x; i < (b1 - b0) * kRowsW; i += kWaves * 64) {
       const size_t r = min(n0 + i / (b1 - b0), g.n - 1), b = b0 + i % (b1 - b0);
-      if (g.ws[r * (LOOSE ? blocks : g.pitch) + b] - 104u > 36u) {
+      if (g.ws[r * (LIST ? blocks : g.pitch) + b] - 104u > 36u) {
         const uint4 q = *(const uint4*)(g.w + (r * blocks + b) * 16);
         odd |= ((q.x | q.y | q.z | q.w) & 0x77777777u) != 0;
       }

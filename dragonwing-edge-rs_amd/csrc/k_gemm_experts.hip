@@ -422,7 +422,7 @@ __device__ __forceinline__ void rows_of(const GemmExpertsArgs& x, int m0, int en
 
 template <bool MX, int WM, int WN, int TM, int TN>
 __global__ __launch_bounds__(WM* WN * 64) void expert_tile_kernel(GemmExpertsArgs x, int tiles_n) {
-  using T = Tile<MX, WM, WN, TM, TN, true, true>;
+  using T = Tile<MX, WM, WN, TM, TN, true>;
   extern __shared__ __align__(16) uint8_t lds[];
   Share s;
   int m0, n0;
@@ -540,7 +540,7 @@ void launch_expert_rows(hipStream_t st, const GemmExpertsArgs& x) {
 
 template <bool MX, int WM, int WN, int TM, int TN>
 void launch_expert_tiles(hipStream_t st, const GemmExpertsArgs& x, size_t tiles) {
-  using T = Tile<MX, WM, WN, TM, TN, true, true>;
+  using T = Tile<MX, WM, WN, TM, TN, true>;
   auto* k = expert_tile_kernel<MX, WM, WN, TM, TN>;
   hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(WM * WN * 64), T::kLds + T::kRowsA * 4, st, x,
                      (x.g.n + T::kRowsW - 1) / T::kRowsW);
