@@ -297,6 +297,33 @@ def test_products_of_prompts_with_weights_beyond_f16(backend):
         c.check(backend, None, 0, np.float32)
 
 
+def test_products_one_after_the_other_on_two_backends(backend):
+    # workspaces that grow while earlier calls are in flight, of two backends on one device
+    other, calls = type(backend)(0), []
+    try:
+        rng = np.random.default_rng(19)
+        cases = [Case(rng, counts, 70, k, kind) for counts, k, kind in
+                 (([40, 30], 99, "f16"), ([300, 250], 545, "mxfp4"), ([30, 3], 1001, "f16"), ([400, 9], 1130, "f16"))]
+        alone = [c.run(backend, None, 0, np.float32) for c in cases]
+        for be in (backend, other, backend, other):
+            for c, want in zip(cases, alone):
+                rows, scales = c.a if isinstance(c.a, tuple) else (c.a, None)
+                held = [be.from_numpy(x) for x in (rows, c.q, c.s, c.offsets, c.order)]
+                held.append(None if scales is None else be.from_numpy(scales))
+                calls.append((be, c, want, held, be.alloc(c.slots * c.n * 4)))
+        for be, c, _, (a, w, ws, offsets, order, scales), y in calls:
+            ops.gemm_mxfp4_experts(be, F16 if scales is None else MX, a, scales, w, ws, None, F32, y, offsets, order,
+                                   c.slots, c.experts, c.n, c.k)
+        for be, c, want, _, y in calls:
+            np.testing.assert_array_equal(be.to_numpy(y, np.float32, (c.slots, c.n)), want)
+    finally:
+        for _, _, _, held, y in calls:
+            for buffer in (*held, y):
+                if buffer is not None:
+                    buffer.free()
+        other.close()
+
+
 def test_products_of_more_workgroups_than_a_grid_has_are_refused(backend):
     experts, n, slots = 1024, 1 << 20, 1024
     a, s, c = backend.alloc(slots * 64), backend.alloc(experts * n), backend.alloc(slots * n * 2)
