@@ -371,9 +371,9 @@ __device__ __forceinline__ void store_part(const GemmMxArgs& a, const uint8_t* l
 
 // A tile's sums to C, through LDS (behind `rows`, which keeps C's rows), in kPieces
 // parts: a wave's stores cover rows of C whole, and the code of an activation is
-// short (written out for every sum, a 256 x 256 tile spent 17 us on it, a fourth of its
-// time at K = 4,096).  A row's pieces of 16 bytes stand at their index xor the row's,
-// so that eight rows' writes meet all banks.
+// short (written out for every sum, a 256 x 256 tile of f16 rows with SiLU spent 17 of 134 us
+// on it at K = 4,096, and spends 9).  A row's pieces of 16 bytes stand at their index
+// xor the row's, so that eight rows' writes meet all banks.
 template <int WM, int WN, int TM, int TN, int kPieces>
 __device__ __forceinline__ void store_tile(const GemmMxArgs& a, uint8_t* lds, const int* rows, int n0,
                                            const f32x4 (&acc)[TN][TM]) {
