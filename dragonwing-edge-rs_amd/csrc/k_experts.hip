@@ -119,7 +119,7 @@ template <int L, int V>
 struct Router {
   const RouteArgs& a;
   int lane;    // of the token's
-  float x[V];  // logits; kNone for NaN and behind the end
+  float x[V];  // logits; kNone for NaN and behind the end, no -0
   float top;   // the largest, of a softmax
 
   __device__ __forceinline__ Router(const RouteArgs& args, size_t row) : a(args), lane(threadIdx.x & (L - 1)) {
@@ -129,7 +129,7 @@ struct Router {
       load((const float*)a.x + row, x);
     top = kNone;
 #pragma unroll
-    for (int v = 0; v < V; ++v) x[v] = fmaxf(x[v], kNone);  // a NaN is never chosen
+    for (int v = 0; v < V; ++v) x[v] = fmaxf(x[v] + 0.0f, kNone);  // a NaN is never chosen, and -0 is the same as 0
     if (!a.sigmoid) {
 #pragma unroll
       for (int v = 0; v < V; ++v) top = fmaxf(top, x[v]);
@@ -255,9 +255,9 @@ struct Router {
     return (threadIdx.x & 7) == 7 ? g : f;
   }
 
-  // The largest by keys of 32 bits: each lane sorts its own, and the largest first one
-  // is taken top_k times; choice j comes to lane j % L, id[j / L].  WHOLE: the values are
-  // f16 numbers and keys hold them and their expert, else a value's upper bits and
+  // The largest by keys of 32 bits, which want values without -0: each lane sorts its own,
+  // and the largest first one is taken top_k times; choice j comes to lane j % L,
+  // id[j / L].  WHOLE: the values are f16 numbers and keys hold them and their expert, else a value's upper bits and
   // the place in the lane, which leaves out log2 V bits of 24.  True if values, off by
   // `off`, lie closer than keys tell apart: the chosen ones are then not below `least`
   // (in lane 0).  KEEP: how many of a lane's keys may be taken.
@@ -269,8 +269,8 @@ struct Router {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const uint32_t e = lane * V + v;
-      // f16 numbers leave 13 bits of an f32 one; their zeros are equal
-      const uint32_t key = WHOLE ? (ordered(c[v] + 0.0f) & ~0x1FFFu) | (0x1FFFu - e) : (ordered(c[v]) & ~kLow) | (kLow - v);
+      // f16 numbers leave 13 bits of an f32 one
+      const uint32_t key = WHOLE ? (ordered(c[v]) & ~0x1FFFu) | (0x1FFFu - e) : (ordered(c[v]) & ~kLow) | (kLow - v);
       k[v] = c[v] > kNone ? key : e;  // experts that are not chosen have keys of their own, too
     }
     sort_down(k);
