@@ -244,8 +244,9 @@ struct Router {
       own_lds();
     }
     dropped = largest<L>(dropped), kept = -largest<L>(-kept), most = largest<L>(most);
-    // two sums of two values each
-    return dropped > kNone && near(kept - dropped, 3 * most, 2 * off, 0.0f);
+    // two sums of two values each: a value is rounded by 2^-24 of `most`, a sum by twice that, so
+    // that two sums may be 8 x 2^-24 of it off, and four times what a score may be
+    return dropped > kNone && near(kept - dropped, 4 * most, 2 * off, 0.0f);
   }
   // The number of the token's next lane.
   static __device__ __forceinline__ float next(float v) {
