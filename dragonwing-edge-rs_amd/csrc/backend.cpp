@@ -25,7 +25,9 @@ static thread_local std::string g_last_error;
 void set_last_error(const std::string& m) { g_last_error = m; }
 void fail(int code, const std::string& msg) { throw Error{code, msg}; }
 void hip_check(hipError_t e, const char* what) {
-  if (e != hipSuccess) fail(DW_ERR_BACKEND, std::string(what) + ": " + hipGetErrorString(e));
+  if (e == hipSuccess) return;
+  (void)hipGetLastError();  // reported here: the check behind a later call's launches must not find it
+  fail(DW_ERR_BACKEND, std::string(what) + ": " + hipGetErrorString(e));
 }
 
 void* Backend::workspace(int slot, size_t bytes) {
@@ -329,10 +331,8 @@ int dw_hip_alloc(dw_hip_backend* be, size_t len_bytes, int kind, dw_hip_buffer**
   if (kind != DW_BUFFER_STORAGE) dw::fail(DW_ERR_UNSUPPORTED, "unknown buffer kind");
   if (!out) dw::fail(DW_ERR_INVALID, "null out");
   void* p = nullptr;
-  hipError_t e = hipMalloc(&p, std::max<size_t>(len_bytes, 1));
-  if (e != hipSuccess)
-    dw::fail(DW_ERR_BACKEND, "alloc of " + std::to_string(len_bytes) + " bytes failed: " +
-                                 hipGetErrorString(e));
+  dw::hip_check(hipMalloc(&p, std::max<size_t>(len_bytes, 1)),
+                ("alloc of " + std::to_string(len_bytes) + " bytes failed").c_str());
   *out = new dw_hip_buffer{b, p, len_bytes};
   dw::hold(b);
   API_END
