@@ -6,21 +6,10 @@
 #include <type_traits>
 
 #include "dw_common.h"
+#include "expert_lists.h"
 #include "mxfp4.h"
 
 namespace dw {
-
-// Rows of A that a list names: place p of C's rows reads row list[p] / each
-// (row 0 where the list says what is no place), or row p without a list.
-struct RowList {
-  const int32_t* list;
-  uint32_t places, each;
-  __device__ __forceinline__ uint32_t row(int p) const {
-    if (!list) return (uint32_t)p;
-    const uint32_t v = (uint32_t)list[p];
-    return v < places ? v / each : 0u;
-  }
-};
 
 // What is laid out anew before a product: f16 rows of A at a stride of whole 16
 // bytes, zeros behind their ends; scale bytes with each row at a stride of 16

@@ -60,9 +60,7 @@ __device__ __forceinline__ RowList list_of(const GemmExpertsArgs& x) {
 
 // C's row of a place, below 0 for none.
 __device__ __forceinline__ int row_of(const GemmExpertsArgs& x, int place) {
-  if (!x.scatter) return place;
-  const int r = x.order[place];
-  return r < x.g.m ? r : -1;
+  return x.scatter ? row_named(x.order[place], x.g.m) : place;
 }
 
 // --- experts of few rows ------------------------------------------------------------
@@ -290,7 +288,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void expert_rows_kernel(GemmExperts
 
 // Tile `id` of the grid: which expert's, and which rows and columns of it.
 template <class T>
-__device__ __forceinline__ bool tile_of(const GemmExpertsArgs& x, int id, int tiles_n, Share* s, int* m0, int* n0) {
+__device__ __forceinline__ bool tile_of(const GemmExpertsArgs& x, uint32_t id, int tiles_n, Share* s, int* m0, int* n0) {
   const int lane = threadIdx.x & 63;
   NewTokens t{0, 0};
   auto tiles = [&](int e) {
@@ -300,10 +298,9 @@ __device__ __forceinline__ bool tile_of(const GemmExpertsArgs& x, int id, int ti
   };
   int all = 0;
   for (int e0 = 0; e0 < x.experts; e0 += 64) all += __builtin_amdgcn_readlane(sums_upto(tiles(e0 + lane)), 63);
-  // Neighbouring workgroups go to the 8 XCDs in turn: each takes a run of tiles.
-  const int total = all * tiles_n, per = total / 8, rest = total % 8, xcd = id % 8, in = id / 8;
-  if (in >= per + (xcd < rest)) return false;
-  const int tile = xcd * per + min(xcd, rest) + in, row = tile / tiles_n;
+  int tile;
+  if (!tile_number(id, all, tiles_n, &tile)) return false;
+  const int row = tile / tiles_n;
   int before = 0;
   for (int e0 = 0; e0 < x.experts; e0 += 64) {
     const int n = tiles(e0 + lane), upto = sums_upto(n);
