@@ -288,7 +288,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void expert_rows_kernel(GemmExperts
 
 // Tile `id` of the grid: which expert's, and which rows and columns of it.
 template <class T>
-__device__ __forceinline__ bool tile_of(const GemmExpertsArgs& x, uint32_t id, int tiles_n, Share* s, int* m0, int* n0) {
+__device__ __forceinline__ bool tile_of(const GemmExpertsArgs& x, int id, int tiles_n, Share* s, int* m0, int* n0) {
   const int lane = threadIdx.x & 63;
   NewTokens t{0, 0};
   auto tiles = [&](int e) {
