@@ -34,9 +34,10 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 // e^-s is 2^(hi + lo), hi + lo = -s log2(e) to 2^-48 of it: exp2 and the
 // reciprocal leave 2^-22 of the result, below an f16 C's 2^-11 and near the
-// sum's own error in an f32 one.  1,209 x 7,712 x 832: MXFP4 rows 28.5 us, 33.4
-// us with expf and a division, which leave 2^-24, and 23.6 us without SiLU; f16
-// rows 39.4, 44.3 and 34.5 us.
+// sum's own error in an f32 one; where e is beyond f32 the result, under 2^-121,
+// is 0.  1,209 x 7,712 x 832: MXFP4 rows 28.5 us, 33.4 us with expf and a
+// division, which leave 2^-24, and 23.6 us without SiLU; f16 rows 39.4, 44.3 and
+// 34.5 us.
 __device__ __forceinline__ float silu(float s) {
   const float hi = s * -1.44269504f, lo = fmaf(s, -1.44269504f, -hi) + s * -1.92596300e-8f;
   const float e = __builtin_amdgcn_exp2f(hi);

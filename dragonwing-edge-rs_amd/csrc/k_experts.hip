@@ -258,10 +258,10 @@ struct Router {
 
   // The largest by keys of 32 bits, which want values without -0: each lane sorts its own,
   // and the largest first one is taken top_k times; choice j comes to lane j % L,
-  // id[j / L].  WHOLE: the values are f16 numbers and keys hold them and their expert, else a value's upper bits and
-  // the place in the lane, which leaves out log2 V bits of 24.  True if values, off by
-  // `off`, lie closer than keys tell apart: the chosen ones are then not below `least`
-  // (in lane 0).  KEEP: how many of a lane's keys may be taken.
+  // id[j / L].  WHOLE: the values are f16 numbers and keys hold them and their expert,
+  // else a value's upper bits and the place in the lane, which leaves out log2 V bits
+  // of 24.  True if values, off by `off`, lie closer than keys tell apart: the chosen
+  // ones are then not below `least` (in lane 0).  KEEP: how many of a lane's keys may be taken.
   static constexpr int kEach = kMostTop / L > 0 ? kMostTop / L : 1;
   template <int KEEP, bool WHOLE>
   __device__ __forceinline__ bool choose(const float (&c)[V], float off, int (&id)[kEach], float* least) const {

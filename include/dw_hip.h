@@ -362,7 +362,8 @@ int dw_hip_dequantize_mxfp4(dw_hip_backend* be, int dtype, const dw_hip_buffer* 
  * c_dtype: of C and of the bias (may be NULL), F32 or F16.  Products are
  * exact and summed in f32 in an order of the library's own; bias and
  * activation (DW_ACT_*) are f32, SiLU to 2^-22 of its value, and C is rounded
- * once; terms and sums below 2^-126 may be lost.  Elements of W and A behind a
+ * once; terms and sums below 2^-126 may be lost, and SiLU's values below 2^-121
+ * (of sums under -88).  Elements of W and A behind a
  * row's k must be 0, as quantize writes them.  m and n at most 2^24, k at most
  * 2^22. */
 int dw_hip_gemm_mxfp4(dw_hip_backend* be, int a_dtype, const dw_hip_buffer* a, const dw_hip_buffer* a_scales,
@@ -459,10 +460,13 @@ int dw_hip_attention_mxfp4(dw_hip_backend* be, const dw_hip_buffer* q, size_t q_
  * the top_groups groups of largest value take part, ties to the lowest index; a
  * group's value is the largest p_e + bias_e in it (group_best 1) or the sum of
  * the two largest (2; of the only one where one takes part).  Values are
- * compared in 64 bits, without a bias and a sum as the logits themselves.
+ * compared in 64 bits, where there is neither a bias nor a sum as the logits
+ * themselves (else those tie whose scores 64 bits round to one value, as sigmoids
+ * of logits above 37).
  * ids int32 [tokens][top_k]; weights f32 [tokens][top_k], scale * p_e, with
  * renorm scale * p_e / (the sum of the chosen p), formed in f32 (a difference d
- * of two logits is rounded to it, d 2^-24 of the weight).  An expert
+ * of two logits is rounded to it, d 2^-24 of the weight; p_e below 2^-126 may be
+ * 0).  An expert
  * whose logit or p_e + bias_e is NaN or -inf is never chosen; a choice that
  * finds no expert has id -1 and weight 0 (all choices of a row that is -inf as a
  * whole).  Experts of infinite logits share a softmax equally.  top_k at most
@@ -495,7 +499,7 @@ int dw_hip_order_experts(dw_hip_backend* be, const dw_hip_buffer* ids, dw_hip_bu
  * slots and n at most 2^24, k at most 2^22, A at most 64 GiB.  What takes more
  * workgroups than a grid holds is refused: products with n * min(experts, slots) of 2^29
  * and more may be, and those of 2^23 tiles of C.  SiLU holds to 2^-22 of its value
- * for an f32 C, to 2^-17 for an f16 one. */
+ * for an f32 C, to 2^-17 for an f16 one; its values below 2^-121 may be lost. */
 int dw_hip_gemm_mxfp4_experts(dw_hip_backend* be, int a_dtype, const dw_hip_buffer* a, const dw_hip_buffer* a_scales,
                               const dw_hip_buffer* w, const dw_hip_buffer* w_scales, const dw_hip_buffer* bias,
                               int c_dtype, dw_hip_buffer* c, const dw_hip_buffer* offsets, const dw_hip_buffer* order,
